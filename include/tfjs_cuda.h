@@ -271,6 +271,45 @@ int tfjs_cuda_reduce_last(tfjs_cuda_ctx* ctx, int op, tfjs_tensor_id x, tfjs_ten
  * rounding of the op-layer chain (ops/softmax.ts:57-63, ops/reduction_ops.ts:56-73). */
 int tfjs_cuda_softmax_last(tfjs_cuda_ctx* ctx, tfjs_tensor_id x, tfjs_tensor_id out, int64_t outer,
                            int64_t inner);
+/* ---- extensions for token and feature models: a normalisation, a lookup and a loss, each with its
+ *      gradient.  No counterpart as one kernel in the reference's surface (the op layer would compose
+ *      them from reductions, gather and binary ops).  Activations (x, y, dy, table, out, logits) may be
+ *      stored as float32 or float16; statistics, losses and gradients are float32, because half
+ *      gradients underflow without loss scaling.  Every result is the same bits on every run.
+ *
+ * y = (x - mean) * rstd * gamma + beta over the last axis, x viewed as [rows, width];
+ * rstd = 1 / sqrt(mean((x - mean)^2) + epsilon).  gamma and beta are [width] or 0 (absent: 1 and 0);
+ * stats, [rows, 2] (mean, rstd of each row) or 0, is what the gradient reads. */
+int tfjs_cuda_layer_norm(tfjs_cuda_ctx* ctx, tfjs_tensor_id x, tfjs_tensor_id gamma, tfjs_tensor_id beta,
+                         tfjs_tensor_id y, tfjs_tensor_id stats, int64_t rows, int64_t width, float epsilon);
+/* Gradients of layer_norm: dx [rows, width], dgamma and dbeta [width]; each may be 0 (not wanted). */
+int tfjs_cuda_layer_norm_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id dy, tfjs_tensor_id x, tfjs_tensor_id gamma,
+                                  tfjs_tensor_id stats, tfjs_tensor_id dx, tfjs_tensor_id dgamma,
+                                  tfjs_tensor_id dbeta, int64_t rows, int64_t width);
+/* out[t] = scale * table[indices[t]], table [vocab, width], indices int32; a row of zeros where the
+ * index lies outside [0, vocab) (padding).  The table may also be a quantised tensor: its bytes are
+ * decoded as they are read. */
+int tfjs_cuda_embedding_lookup(tfjs_cuda_ctx* ctx, tfjs_tensor_id table, tfjs_tensor_id indices, tfjs_tensor_id out,
+                               int64_t tokens, int64_t vocab, int64_t width, float scale);
+/* dtable[v] = scale * sum of dy[t] over the tokens with indices[t] == v (zeros where there is none). */
+int tfjs_cuda_embedding_lookup_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id dy, tfjs_tensor_id indices,
+                                        tfjs_tensor_id dtable, int64_t tokens, int64_t vocab, int64_t width,
+                                        float scale);
+/* Knowledge distillation from a teacher's `top` largest logits of each row, T = temperature:
+ *   loss[r] = T^2 sum_k p_k (log p_k - log q[i_k]),
+ * q = softmax(logits[r] / T) over all classes, p = softmax(teacher_logits[r] / T) over the entries
+ * whose index lies in [0, classes) and whose logit is above -inf (so -1 ends a shorter list; a class
+ * named twice counts twice).  A row without such an entry has loss 0 and gradient 0.  top <= 1024.
+ * stats, [rows, 2] (log-sum-exp of the student's and of the teacher's scaled logits) or 0, is what the
+ * gradient reads. */
+int tfjs_cuda_distillation_loss(tfjs_cuda_ctx* ctx, tfjs_tensor_id logits, tfjs_tensor_id teacher_logits,
+                                tfjs_tensor_id teacher_indices, tfjs_tensor_id loss, tfjs_tensor_id stats,
+                                int64_t rows, int64_t classes, int64_t top, float temperature);
+/* dlogits[r, v] = dloss[r] * T * (q_v - sum of p_k over the entries with i_k == v). */
+int tfjs_cuda_distillation_loss_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id dloss, tfjs_tensor_id logits,
+                                         tfjs_tensor_id teacher_logits, tfjs_tensor_id teacher_indices,
+                                         tfjs_tensor_id stats, tfjs_tensor_id dlogits, int64_t rows, int64_t classes,
+                                         int64_t top, float temperature);
 /* KernelBackend.cast (backend.ts:484-486; backend_util.ts:36-71) where a copy is needed:
  * converts x's stored dtype to out's dtype (float->int truncates, ->bool is != 0). */
 int tfjs_cuda_cast(tfjs_cuda_ctx* ctx, tfjs_tensor_id x, tfjs_tensor_id out);

@@ -8,9 +8,10 @@
  * enqueues work on the context's stream and returns.
  *
  * Methods outside the reference's surface are extensions (named as such below): a clip / relu6
- * activation for the fused ops, fusedDepthwiseConv2D, fusedSeparableConv2d, softmax, quantised
- * weight registration, asynchronous writes, CUDA-graph capture, per-kernel profiling.  Each has
- * an unfused equivalent through the plain methods, which is what unmodified tf.* code reaches.
+ * activation for the fused ops, fusedDepthwiseConv2D, fusedSeparableConv2d, softmax, layerNorm,
+ * embeddingLookup and distillationLoss with their gradients, quantised weight registration, device
+ * arrays, asynchronous writes, CUDA-graph capture, per-kernel profiling.  The fused ones have an
+ * unfused equivalent through the plain methods, which is what unmodified tf.* code reaches.
  *
  * The Python class tfjs-core_b200/backend_cuda.py mirrors this file method for method; it is the
  * form the test-suite executes on machines without a JavaScript runtime.
@@ -325,6 +326,25 @@ export class BackendCuda extends KernelBackend {
     binding.tensorDispose(this.ctx, rec.id);
     this.data.set(t.dataId, {id: r.out_id, dtype: 'float32', shape: shape.slice(), quantized: true});
     return t;
+  }
+
+  /** Extension: a tensor with the named storage, 'float32', 'int32' or 'float16' (a float32 tensor
+   * stored as IEEE half).  Without `values` its contents are undefined until they are written. */
+  registerStored(shape: number[], storage: 'float32'|'int32'|'float16', values?: Float32Array|Int32Array): Tensor {
+    if (storage !== 'float32' && storage !== 'int32' && storage !== 'float16') {
+      throw new Error(`storage must be 'float32', 'int32' or 'float16', got ${storage}`);
+    }
+    const t = storage === 'int32' ? this.makeOutput<Tensor>(shape, 'int32') : this.makeActivation<Tensor>(shape, storage);
+    if (values != null) this.write(t.dataId, values);
+    return t;
+  }
+
+  /** Extension: the address and byte size of `t`'s storage, for another CUDA library on the same
+   * device.  Valid until `t`'s data is disposed; work on another stream is ordered by the caller. */
+  deviceArray(t: Tensor): {ptr: bigint, nbytes: number, stream: bigint} {
+    const r = binding.tensorDevicePtr(this.ctx, this.data.get(t.dataId).id);
+    this.check(r.status);
+    return {ptr: r.ptr, nbytes: r.nbytes, stream: this.stream()};
   }
 
   // ---- fused epilogue marshalling ------------------------------------------------------------
@@ -699,6 +719,131 @@ export class BackendCuda extends KernelBackend {
     const out = this.makeOutput<T>(logits.shape);
     this.check(binding.softmaxLast(this.ctx, xid, this.outId(out), outer, inner));
     this.freeTmp(tx);
+    return out;
+  }
+
+  // ---- normalisation, lookup and loss of token and feature models (extensions) ---------------------
+  /** Ends a kernel method: frees the converted operands and, if the call failed, its outputs. */
+  private enqueued(rc: number, outputs: Array<Tensor|null>, temporaries: Array<number|null>): void {
+    this.freeTmp(...temporaries);
+    if (rc !== 0) {
+      for (const t of outputs) {
+        if (t != null) t.dispose();
+      }
+      this.check(rc);
+    }
+  }
+
+  private optionalId(t: Tensor|null): [number, number|null] {
+    return t == null ? [0, null] : this.id(t);
+  }
+
+  /** (x - mean) * rstd * gamma + beta over the inner-most axis; gamma and beta are [width] or null.
+   * Returns y and the statistics [..., 2] that the gradient reads (null unless `withStats`). */
+  layerNorm<T extends Tensor>(x: T, gamma: Tensor|null, beta: Tensor|null, epsilon: number, withStats = false,
+                              outputStorage?: 'float32'|'float16'): [T, Tensor|null] {
+    this.assertNumeric([x, gamma, beta], 'layerNorm');
+    if (x.rank === 0) throw new Error('layerNorm needs a tensor of rank 1 or more');
+    const outer = x.shape.slice(0, -1);
+    const [xid, tx] = this.activationId(x);
+    const [gid, tg] = this.optionalId(gamma);
+    const [bid, tb] = this.optionalId(beta);
+    const y = this.makeActivation<T>(x.shape, outputStorage);
+    const stats = withStats ? this.makeOutput<Tensor>([...outer, 2]) : null;
+    const rc = binding.layerNorm(this.ctx, xid, gid, bid, this.outId(y), stats == null ? 0 : this.outId(stats),
+                                 util.sizeFromShape(outer), x.shape[x.rank - 1], epsilon);
+    this.enqueued(rc, [y, stats], [tx, tg, tb]);
+    return [y, stats];
+  }
+
+  /** dx, dgamma and dbeta of layerNorm, from the statistics of its forward pass. */
+  layerNormBackprop<T extends Tensor>(dy: T, x: T, gamma: Tensor|null, stats: Tensor): [T, Tensor, Tensor] {
+    this.assertNumeric([dy, x, gamma, stats], 'layerNormBackprop');
+    if (x.rank === 0) throw new Error('layerNorm needs a tensor of rank 1 or more');
+    const width = x.shape[x.rank - 1];
+    const [did, td] = this.activationId(dy);
+    const [xid, tx] = this.activationId(x);
+    const [gid, tg] = this.optionalId(gamma);
+    const [sid, ts] = this.id(stats);
+    const dx = this.makeOutput<T>(x.shape);
+    const dgamma = this.makeOutput<Tensor>([width]);
+    const dbeta = this.makeOutput<Tensor>([width]);
+    const rc = binding.layerNormBackprop(this.ctx, did, xid, gid, sid, this.outId(dx), this.outId(dgamma),
+                                         this.outId(dbeta), util.sizeFromShape(x.shape.slice(0, -1)), width);
+    this.enqueued(rc, [dx, dgamma, dbeta], [td, tx, tg, ts]);
+    return [dx, dgamma, dbeta];
+  }
+
+  /** scale * table[indices]; a row of zeros where the index lies outside the table (padding). */
+  embeddingLookup(table: Tensor, indices: Tensor, scale = 1, outputStorage?: 'float32'|'float16'): Tensor {
+    this.assertNumeric([table], 'embeddingLookup');
+    if (table.rank !== 2) throw new Error(`embeddingLookup needs a table of rank 2, got rank ${table.rank}`);
+    const [tid, tt] = this.activationId(table);
+    const [iid, ti] = this.id(indices, 'int32');
+    const out = this.makeActivation<Tensor>([...indices.shape, table.shape[1]], outputStorage);
+    const rc = binding.embeddingLookup(this.ctx, tid, iid, this.outId(out), indices.size, table.shape[0],
+                                       table.shape[1], scale);
+    this.enqueued(rc, [out], [tt, ti]);
+    return out;
+  }
+
+  /** The gradient of embeddingLookup's table, [vocab, width]. */
+  embeddingLookupBackprop(dy: Tensor, indices: Tensor, vocab: number, scale = 1): Tensor {
+    this.assertNumeric([dy], 'embeddingLookupBackprop');
+    if (dy.rank === 0 || !util.arraysEqual(dy.shape.slice(0, -1), indices.shape)) {
+      throw new Error(`embeddingLookupBackprop: dy's shape ${dy.shape} does not match indices ${indices.shape}`);
+    }
+    const width = dy.shape[dy.rank - 1];
+    const [did, td] = this.activationId(dy);
+    const [iid, ti] = this.id(indices, 'int32');
+    const out = this.makeOutput<Tensor>([vocab, width]);
+    const rc = binding.embeddingLookupBackprop(this.ctx, did, iid, this.outId(out), indices.size, vocab, width, scale);
+    this.enqueued(rc, [out], [td, ti]);
+    return out;
+  }
+
+  private static distillationExtent(logits: Tensor, teacherLogits: Tensor, teacherIndices: Tensor): [number, number, number] {
+    if (logits.rank === 0 || !util.arraysEqual(logits.shape.slice(0, -1), teacherLogits.shape.slice(0, -1)) ||
+        !util.arraysEqual(teacherLogits.shape, teacherIndices.shape)) {
+      throw new Error(`distillationLoss: logits ${logits.shape}, teacherLogits ${teacherLogits.shape} and ` +
+                      `teacherIndices ${teacherIndices.shape} must be [..., classes], [..., top] and [..., top]`);
+    }
+    return [util.sizeFromShape(logits.shape.slice(0, -1)), logits.shape[logits.rank - 1],
+            teacherLogits.shape[logits.rank - 1]];
+  }
+
+  /** T^2 * KL(p || q) of each row over the teacher's listed classes, and the statistics [..., 2] that
+   * the gradient reads (null unless `withStats`). */
+  distillationLoss(logits: Tensor, teacherLogits: Tensor, teacherIndices: Tensor, temperature = 1,
+                   withStats = true): [Tensor, Tensor|null] {
+    this.assertNumeric([logits, teacherLogits], 'distillationLoss');
+    const [rows, classes, top] = BackendCuda.distillationExtent(logits, teacherLogits, teacherIndices);
+    const [zid, tz] = this.activationId(logits);
+    const [uid, tu] = this.activationId(teacherLogits);
+    const [iid, ti] = this.id(teacherIndices, 'int32');
+    const outer = logits.shape.slice(0, -1);
+    const loss = this.makeOutput<Tensor>(outer);
+    const stats = withStats ? this.makeOutput<Tensor>([...outer, 2]) : null;
+    const rc = binding.distillationLoss(this.ctx, zid, uid, iid, this.outId(loss), stats == null ? 0 : this.outId(stats),
+                                        rows, classes, top, temperature);
+    this.enqueued(rc, [loss, stats], [tz, tu, ti]);
+    return [loss, stats];
+  }
+
+  /** The gradient of distillationLoss's logits, from the statistics of its forward pass. */
+  distillationLossBackprop(dloss: Tensor, logits: Tensor, teacherLogits: Tensor, teacherIndices: Tensor,
+                           stats: Tensor, temperature = 1): Tensor {
+    this.assertNumeric([dloss, logits, teacherLogits, stats], 'distillationLossBackprop');
+    const [rows, classes, top] = BackendCuda.distillationExtent(logits, teacherLogits, teacherIndices);
+    const [did, td] = this.id(dloss);
+    const [zid, tz] = this.activationId(logits);
+    const [uid, tu] = this.activationId(teacherLogits);
+    const [iid, ti] = this.id(teacherIndices, 'int32');
+    const [sid, ts] = this.id(stats);
+    const out = this.makeOutput<Tensor>(logits.shape);
+    const rc = binding.distillationLossBackprop(this.ctx, did, zid, uid, iid, sid, this.outId(out), rows, classes, top,
+                                                temperature);
+    this.enqueued(rc, [out], [td, tz, tu, ti, ts]);
     return out;
   }
 

@@ -815,6 +815,104 @@ napi_value SoftmaxLast(napi_env env, napi_callback_info cbinfo) {
   return status_value(env, (int64_t)tfjs_cuda_softmax_last(ctx, x, out, outer, inner));
 }
 
+// tfjs_cuda_layer_norm
+napi_value LayerNorm(napi_env env, napi_callback_info cbinfo) {
+  Args argz(env, cbinfo);
+  tfjs_cuda_ctx* ctx = (tfjs_cuda_ctx*)argz.handle(0);
+  const tfjs_tensor_id x = (tfjs_tensor_id)argz.integer(1);
+  const tfjs_tensor_id gamma = (tfjs_tensor_id)argz.integer(2);
+  const tfjs_tensor_id beta = (tfjs_tensor_id)argz.integer(3);
+  const tfjs_tensor_id y = (tfjs_tensor_id)argz.integer(4);
+  const tfjs_tensor_id stats = (tfjs_tensor_id)argz.integer(5);
+  const int64_t rows = (int64_t)argz.integer(6);
+  const int64_t width = (int64_t)argz.integer(7);
+  const float epsilon = (float)argz.number(8);
+  if (!argz.ok) return nullptr;
+  return status_value(env, (int64_t)tfjs_cuda_layer_norm(ctx, x, gamma, beta, y, stats, rows, width, epsilon));
+}
+
+// tfjs_cuda_layer_norm_backprop
+napi_value LayerNormBackprop(napi_env env, napi_callback_info cbinfo) {
+  Args argz(env, cbinfo);
+  tfjs_cuda_ctx* ctx = (tfjs_cuda_ctx*)argz.handle(0);
+  const tfjs_tensor_id dy = (tfjs_tensor_id)argz.integer(1);
+  const tfjs_tensor_id x = (tfjs_tensor_id)argz.integer(2);
+  const tfjs_tensor_id gamma = (tfjs_tensor_id)argz.integer(3);
+  const tfjs_tensor_id stats = (tfjs_tensor_id)argz.integer(4);
+  const tfjs_tensor_id dx = (tfjs_tensor_id)argz.integer(5);
+  const tfjs_tensor_id dgamma = (tfjs_tensor_id)argz.integer(6);
+  const tfjs_tensor_id dbeta = (tfjs_tensor_id)argz.integer(7);
+  const int64_t rows = (int64_t)argz.integer(8);
+  const int64_t width = (int64_t)argz.integer(9);
+  if (!argz.ok) return nullptr;
+  return status_value(env, (int64_t)tfjs_cuda_layer_norm_backprop(ctx, dy, x, gamma, stats, dx, dgamma, dbeta, rows, width));
+}
+
+// tfjs_cuda_embedding_lookup
+napi_value EmbeddingLookup(napi_env env, napi_callback_info cbinfo) {
+  Args argz(env, cbinfo);
+  tfjs_cuda_ctx* ctx = (tfjs_cuda_ctx*)argz.handle(0);
+  const tfjs_tensor_id table = (tfjs_tensor_id)argz.integer(1);
+  const tfjs_tensor_id indices = (tfjs_tensor_id)argz.integer(2);
+  const tfjs_tensor_id out = (tfjs_tensor_id)argz.integer(3);
+  const int64_t tokens = (int64_t)argz.integer(4);
+  const int64_t vocab = (int64_t)argz.integer(5);
+  const int64_t width = (int64_t)argz.integer(6);
+  const float scale = (float)argz.number(7);
+  if (!argz.ok) return nullptr;
+  return status_value(env, (int64_t)tfjs_cuda_embedding_lookup(ctx, table, indices, out, tokens, vocab, width, scale));
+}
+
+// tfjs_cuda_embedding_lookup_backprop
+napi_value EmbeddingLookupBackprop(napi_env env, napi_callback_info cbinfo) {
+  Args argz(env, cbinfo);
+  tfjs_cuda_ctx* ctx = (tfjs_cuda_ctx*)argz.handle(0);
+  const tfjs_tensor_id dy = (tfjs_tensor_id)argz.integer(1);
+  const tfjs_tensor_id indices = (tfjs_tensor_id)argz.integer(2);
+  const tfjs_tensor_id dtable = (tfjs_tensor_id)argz.integer(3);
+  const int64_t tokens = (int64_t)argz.integer(4);
+  const int64_t vocab = (int64_t)argz.integer(5);
+  const int64_t width = (int64_t)argz.integer(6);
+  const float scale = (float)argz.number(7);
+  if (!argz.ok) return nullptr;
+  return status_value(env, (int64_t)tfjs_cuda_embedding_lookup_backprop(ctx, dy, indices, dtable, tokens, vocab, width, scale));
+}
+
+// tfjs_cuda_distillation_loss
+napi_value DistillationLoss(napi_env env, napi_callback_info cbinfo) {
+  Args argz(env, cbinfo);
+  tfjs_cuda_ctx* ctx = (tfjs_cuda_ctx*)argz.handle(0);
+  const tfjs_tensor_id logits = (tfjs_tensor_id)argz.integer(1);
+  const tfjs_tensor_id teacher_logits = (tfjs_tensor_id)argz.integer(2);
+  const tfjs_tensor_id teacher_indices = (tfjs_tensor_id)argz.integer(3);
+  const tfjs_tensor_id loss = (tfjs_tensor_id)argz.integer(4);
+  const tfjs_tensor_id stats = (tfjs_tensor_id)argz.integer(5);
+  const int64_t rows = (int64_t)argz.integer(6);
+  const int64_t classes = (int64_t)argz.integer(7);
+  const int64_t top = (int64_t)argz.integer(8);
+  const float temperature = (float)argz.number(9);
+  if (!argz.ok) return nullptr;
+  return status_value(env, (int64_t)tfjs_cuda_distillation_loss(ctx, logits, teacher_logits, teacher_indices, loss, stats, rows, classes, top, temperature));
+}
+
+// tfjs_cuda_distillation_loss_backprop
+napi_value DistillationLossBackprop(napi_env env, napi_callback_info cbinfo) {
+  Args argz(env, cbinfo);
+  tfjs_cuda_ctx* ctx = (tfjs_cuda_ctx*)argz.handle(0);
+  const tfjs_tensor_id dloss = (tfjs_tensor_id)argz.integer(1);
+  const tfjs_tensor_id logits = (tfjs_tensor_id)argz.integer(2);
+  const tfjs_tensor_id teacher_logits = (tfjs_tensor_id)argz.integer(3);
+  const tfjs_tensor_id teacher_indices = (tfjs_tensor_id)argz.integer(4);
+  const tfjs_tensor_id stats = (tfjs_tensor_id)argz.integer(5);
+  const tfjs_tensor_id dlogits = (tfjs_tensor_id)argz.integer(6);
+  const int64_t rows = (int64_t)argz.integer(7);
+  const int64_t classes = (int64_t)argz.integer(8);
+  const int64_t top = (int64_t)argz.integer(9);
+  const float temperature = (float)argz.number(10);
+  if (!argz.ok) return nullptr;
+  return status_value(env, (int64_t)tfjs_cuda_distillation_loss_backprop(ctx, dloss, logits, teacher_logits, teacher_indices, stats, dlogits, rows, classes, top, temperature));
+}
+
 // tfjs_cuda_cast
 napi_value Cast(napi_env env, napi_callback_info cbinfo) {
   Args argz(env, cbinfo);
@@ -935,6 +1033,12 @@ static napi_value Init(napi_env env, napi_value exports) {
   EXPORT("unary", Unary);
   EXPORT("reduceLast", ReduceLast);
   EXPORT("softmaxLast", SoftmaxLast);
+  EXPORT("layerNorm", LayerNorm);
+  EXPORT("layerNormBackprop", LayerNormBackprop);
+  EXPORT("embeddingLookup", EmbeddingLookup);
+  EXPORT("embeddingLookupBackprop", EmbeddingLookupBackprop);
+  EXPORT("distillationLoss", DistillationLoss);
+  EXPORT("distillationLossBackprop", DistillationLossBackprop);
   EXPORT("cast", Cast);
   EXPORT("matmulStaticScratch", MatmulStaticScratch);
   EXPORT("graphBegin", GraphBegin);

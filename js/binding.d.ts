@@ -58,6 +58,12 @@ export function binary(ctx: Handle, op: number, a: number, a_rank: number, a_sha
 export function unary(ctx: Handle, op: number, x: number, out: number, p0: number, p1: number): number;  // tfjs_cuda_unary
 export function reduceLast(ctx: Handle, op: number, x: number, out: number, outer: number, inner: number): number;  // tfjs_cuda_reduce_last
 export function softmaxLast(ctx: Handle, x: number, out: number, outer: number, inner: number): number;  // tfjs_cuda_softmax_last
+export function layerNorm(ctx: Handle, x: number, gamma: number, beta: number, y: number, stats: number, rows: number, width: number, epsilon: number): number;  // tfjs_cuda_layer_norm
+export function layerNormBackprop(ctx: Handle, dy: number, x: number, gamma: number, stats: number, dx: number, dgamma: number, dbeta: number, rows: number, width: number): number;  // tfjs_cuda_layer_norm_backprop
+export function embeddingLookup(ctx: Handle, table: number, indices: number, out: number, tokens: number, vocab: number, width: number, scale: number): number;  // tfjs_cuda_embedding_lookup
+export function embeddingLookupBackprop(ctx: Handle, dy: number, indices: number, dtable: number, tokens: number, vocab: number, width: number, scale: number): number;  // tfjs_cuda_embedding_lookup_backprop
+export function distillationLoss(ctx: Handle, logits: number, teacher_logits: number, teacher_indices: number, loss: number, stats: number, rows: number, classes: number, top: number, temperature: number): number;  // tfjs_cuda_distillation_loss
+export function distillationLossBackprop(ctx: Handle, dloss: number, logits: number, teacher_logits: number, teacher_indices: number, stats: number, dlogits: number, rows: number, classes: number, top: number, temperature: number): number;  // tfjs_cuda_distillation_loss_backprop
 export function cast(ctx: Handle, x: number, out: number): number;  // tfjs_cuda_cast
 export function matmulStaticScratch(ctx: Handle, a: bigint|null, b: bigint|null, bias: bigint|null, out: bigint|null, m: number, k: number, n: number, activation: number, clip_lo: number, clip_hi: number): number;  // tfjs_cuda_matmul_static_scratch
 export function graphBegin(ctx: Handle): number;  // tfjs_cuda_graph_begin

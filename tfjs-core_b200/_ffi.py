@@ -106,6 +106,12 @@ SIGNATURES = {
     "tfjs_cuda_unary": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_float, C.c_float]),
     "tfjs_cuda_reduce_last": (C.c_int, [_P, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int64]),
     "tfjs_cuda_softmax_last": (C.c_int, [_P, C.c_int64, C.c_int64, C.c_int64, C.c_int64]),
+    "tfjs_cuda_layer_norm": (C.c_int, [_P] + [C.c_int64] * 7 + [C.c_float]),
+    "tfjs_cuda_layer_norm_backprop": (C.c_int, [_P] + [C.c_int64] * 9),
+    "tfjs_cuda_embedding_lookup": (C.c_int, [_P] + [C.c_int64] * 6 + [C.c_float]),
+    "tfjs_cuda_embedding_lookup_backprop": (C.c_int, [_P] + [C.c_int64] * 6 + [C.c_float]),
+    "tfjs_cuda_distillation_loss": (C.c_int, [_P] + [C.c_int64] * 8 + [C.c_float]),
+    "tfjs_cuda_distillation_loss_backprop": (C.c_int, [_P] + [C.c_int64] * 9 + [C.c_float]),
     "tfjs_cuda_cast": (C.c_int, [_P, C.c_int64, C.c_int64]),
     "tfjs_cuda_matmul_static_scratch": (C.c_int, [_P, _P, _P, _P, _P, C.c_int64, C.c_int64, C.c_int64,
                                                   C.c_int, C.c_float, C.c_float]),

@@ -7,8 +7,9 @@ that only enqueues device work.  Tensor data lives in device memory owned by the
 moves to the host only in readSync()/read().
 
 Methods outside the reference's surface are extensions and are named in their docstrings:
-a clip/relu6 activation for the fused ops, fusedDepthwiseConv2D, softmax, quantised weight
-registration and CUDA-graph capture.  Each has an unfused equivalent through the plain
+a clip/relu6 activation for the fused ops, fusedDepthwiseConv2D, softmax, layerNorm,
+embeddingLookup and distillationLoss with their gradients, quantised weight registration, device
+arrays and CUDA-graph capture.  The fused ones have an unfused equivalent through the plain
 methods, which is what unmodified tf.* code reaches.
 """
 import ctypes as C
@@ -25,6 +26,7 @@ EPSILON_FLOAT16 = 1e-4  # backends/backend.ts:24
 _DTYPE_CODE = {"float32": _ffi.F32, "int32": _ffi.I32, "bool": _ffi.BOOL, "float16": _ffi.F16}
 # host-side element type per STORAGE dtype: half-stored tensors travel as float32 (the library converts)
 _HOST_DTYPE = dict(NP_DTYPE, float16=np.float32)
+_TYPESTR = {"float32": "<f4", "int32": "<i4", "bool": "|b1", "float16": "<f2"}
 
 
 class CudaError(RuntimeError):
@@ -52,6 +54,15 @@ class _ReadHandle:
             self._b._lib.tfjs_cuda_event_destroy(self._ev)
             self._b._lib.tfjs_cuda_host_free(self._ptr)
         return self._value
+
+
+class DeviceArray:
+    """A tensor's storage as other CUDA libraries take it (`__cuda_array_interface__`, version 3):
+    `torch.as_tensor(array, device="cuda")` is a view of it, not a copy.  See BackendCuda.deviceArray."""
+    __slots__ = ("__cuda_array_interface__",)
+
+    def __init__(self, interface):
+        self.__cuda_array_interface__ = interface
 
 
 class BackendCuda:
@@ -293,6 +304,35 @@ class BackendCuda:
         self._data[t.dataId] = {"id": out.value, "dtype": "float32", "shape": list(t.shape),
                                 "quantized": True}
         return t
+
+    def registerStored(self, shape, storage, values=None):
+        """Extension: a tensor with the named storage, 'float32', 'int32' or 'float16' (a float32 tensor
+        stored as IEEE half, as the convolutions leave it under setActivationStorage('float16')).
+        Without `values` its contents are undefined until write() or a deviceArray() fills them."""
+        if storage not in ("float32", "int32", "float16"):
+            raise ValueError(f"storage must be 'float32', 'int32' or 'float16', got {storage!r}")
+        self._pending_storage = storage
+        try:
+            t = Tensor.make(shape, {}, "int32" if storage == "int32" else "float32", self)
+        finally:
+            self._pending_storage = None
+        if values is not None:
+            ENGINE.write(self, t.dataId, values)
+        return t
+
+    def deviceArray(self, t):
+        """Extension: `t`'s storage in place, for another library on the same device (half-stored tensors
+        appear as float16, quantised ones as their bytes).  The array is valid until `t`'s data is
+        disposed.  Work that another stream does on it is ordered by the caller: after sync(), or on
+        stream(); a tensor whose contents are written through it must not have been a contraction's or
+        convolution's weights before, whose repacked form is kept."""
+        t._throw_if_disposed()
+        rec = self._rec(t.dataId)
+        ptr = C.c_void_p()
+        self._check(self._lib.tfjs_cuda_tensor_device_ptr(self._ctx, rec["id"], C.byref(ptr), None))
+        typestr = "|u1" if rec.get("quantized") else _TYPESTR[rec["dtype"]]
+        return DeviceArray({"shape": tuple(t.shape), "typestr": typestr, "data": (ptr.value or 0, False),
+                            "version": 3, "stream": self.stream()})
 
     # ---- fused epilogue marshalling ------------------------------------------------------
     @staticmethod
@@ -633,6 +673,123 @@ class BackendCuda:
         self._check(self._lib.tfjs_cuda_softmax_last(self._ctx, xid, self._rec(out.dataId)["id"],
                                                      outer, inner))
         self._free_tmp(tx)
+        return out
+
+    # ---- normalisation, lookup and loss of token and feature models (extensions) -----------
+    def _enqueue(self, rc, outputs, temporaries):
+        """Ends a kernel method: frees the converted operands and, if the call failed, its outputs."""
+        self._free_tmp(*temporaries)
+        if rc != 0:
+            for t in outputs:
+                if t is not None:
+                    t.dispose()
+            self._check(rc)
+
+    def _oid(self, t):
+        return 0 if t is None else self._data[t.dataId]["id"]
+
+    def layerNorm(self, x, gamma, beta, epsilon, withStats=False, outputStorage=None):
+        """Extension: (x - mean) * rstd * gamma + beta over the inner-most axis; gamma and beta are
+        [width] or None.  Returns (y, stats): stats is [..., 2] (mean and rstd of each row), which the
+        gradient reads, or None unless `withStats`.  `outputStorage` overrides the activation-storage
+        mode for y."""
+        self._assert_numeric([x, gamma, beta], "layerNorm")
+        if not x.shape:
+            raise ValueError("layerNorm needs a tensor of rank 1 or more")
+        width = x.shape[-1]
+        xid, tx = self._activation_id(x)
+        gid, tg = self._id(gamma) if gamma is not None else (0, None)
+        bid, tb = self._id(beta) if beta is not None else (0, None)
+        y = self._out_activation(x.shape, outputStorage)
+        stats = self._out(x.shape[:-1] + [2]) if withStats else None
+        rc = self._lib.tfjs_cuda_layer_norm(self._ctx, xid, gid, bid, self._oid(y), self._oid(stats),
+                                            size_from_shape(x.shape[:-1]), width, float(epsilon))
+        self._enqueue(rc, (y, stats), (tx, tg, tb))
+        return y, stats
+
+    def layerNormBackprop(self, dy, x, gamma, stats):
+        """Extension: (dx, dgamma, dbeta) of layerNorm, from the stats of its forward pass."""
+        self._assert_numeric([dy, x, gamma, stats], "layerNormBackprop")
+        if not x.shape:
+            raise ValueError("layerNorm needs a tensor of rank 1 or more")
+        width = x.shape[-1]
+        did, td = self._activation_id(dy)
+        xid, tx = self._activation_id(x)
+        gid, tg = self._id(gamma) if gamma is not None else (0, None)
+        sid, ts = self._id(stats)
+        dx, dgamma, dbeta = outputs = (self._out(x.shape), self._out([width]), self._out([width]))
+        rc = self._lib.tfjs_cuda_layer_norm_backprop(self._ctx, did, xid, gid, sid, self._oid(dx), self._oid(dgamma),
+                                                     self._oid(dbeta), size_from_shape(x.shape[:-1]), width)
+        self._enqueue(rc, outputs, (td, tx, tg, ts))
+        return outputs
+
+    def embeddingLookup(self, table, indices, scale=1.0, outputStorage=None):
+        """Extension: scale * table[indices], [..., width]; a row of zeros where the index lies outside
+        the table (padding).  The table may be half-stored or quantised.  `outputStorage` overrides the
+        activation-storage mode for the result."""
+        self._assert_numeric(table, "embeddingLookup")
+        if len(table.shape) != 2:
+            raise ValueError(f"embeddingLookup needs a table of rank 2, got rank {len(table.shape)}")
+        tid, tt = self._activation_id(table)
+        iid, ti = self._id(indices, "int32")
+        out = self._out_activation(indices.shape + [table.shape[1]], outputStorage)
+        rc = self._lib.tfjs_cuda_embedding_lookup(self._ctx, tid, iid, self._oid(out), indices.size, table.shape[0],
+                                                  table.shape[1], float(scale))
+        self._enqueue(rc, (out,), (tt, ti))
+        return out
+
+    def embeddingLookupBackprop(self, dy, indices, vocab, scale=1.0):
+        """Extension: the gradient of embeddingLookup's table, [vocab, width]: scale times the sum of the
+        rows of dy that name each table row, in the order of the tokens."""
+        self._assert_numeric(dy, "embeddingLookupBackprop")
+        if dy.shape[:-1] != indices.shape or not dy.shape:
+            raise ValueError(f"embeddingLookupBackprop: dy's shape {dy.shape} does not match indices {indices.shape}")
+        did, td = self._activation_id(dy)
+        iid, ti = self._id(indices, "int32")
+        out = self._out([int(vocab), dy.shape[-1]])
+        rc = self._lib.tfjs_cuda_embedding_lookup_backprop(self._ctx, did, iid, self._oid(out), indices.size,
+                                                           int(vocab), dy.shape[-1], float(scale))
+        self._enqueue(rc, (out,), (td, ti))
+        return out
+
+    @staticmethod
+    def _distillation_extent(logits, teacherLogits, teacherIndices):
+        if not logits.shape or logits.shape[:-1] != teacherLogits.shape[:-1] or \
+                teacherLogits.shape != teacherIndices.shape:
+            raise ValueError(f"distillationLoss: logits {logits.shape}, teacherLogits {teacherLogits.shape} and "
+                             f"teacherIndices {teacherIndices.shape} must be [..., classes], [..., top] and [..., top]")
+        return size_from_shape(logits.shape[:-1]), logits.shape[-1], teacherLogits.shape[-1]
+
+    def distillationLoss(self, logits, teacherLogits, teacherIndices, temperature=1.0, withStats=True):
+        """Extension: T^2 * KL(p || q) of each row, q = softmax(logits / T) over all classes and
+        p = softmax(teacherLogits / T) over the teacher's listed classes (an index outside the classes
+        does not count; a row without any gives 0).  Returns (loss, stats): stats, [..., 2], is what the
+        gradient reads, or None unless `withStats`."""
+        self._assert_numeric([logits, teacherLogits], "distillationLoss")
+        rows, classes, top = self._distillation_extent(logits, teacherLogits, teacherIndices)
+        zid, tz = self._activation_id(logits)
+        uid, tu = self._activation_id(teacherLogits)
+        iid, ti = self._id(teacherIndices, "int32")
+        loss = self._out(logits.shape[:-1])
+        stats = self._out(logits.shape[:-1] + [2]) if withStats else None
+        rc = self._lib.tfjs_cuda_distillation_loss(self._ctx, zid, uid, iid, self._oid(loss), self._oid(stats), rows,
+                                                   classes, top, float(temperature))
+        self._enqueue(rc, (loss, stats), (tz, tu, ti))
+        return loss, stats
+
+    def distillationLossBackprop(self, dloss, logits, teacherLogits, teacherIndices, stats, temperature=1.0):
+        """Extension: the gradient of distillationLoss's logits, from the stats of its forward pass."""
+        self._assert_numeric([dloss, logits, teacherLogits, stats], "distillationLossBackprop")
+        rows, classes, top = self._distillation_extent(logits, teacherLogits, teacherIndices)
+        did, td = self._id(dloss)
+        zid, tz = self._activation_id(logits)
+        uid, tu = self._activation_id(teacherLogits)
+        iid, ti = self._id(teacherIndices, "int32")
+        sid, ts = self._id(stats)
+        out = self._out(logits.shape)
+        rc = self._lib.tfjs_cuda_distillation_loss_backprop(self._ctx, did, zid, uid, iid, sid, self._oid(out), rows,
+                                                            classes, top, float(temperature))
+        self._enqueue(rc, (out,), (td, tz, tu, ti, ts))
         return out
 
     # ---- metadata ops (backend.ts:480-486; backend_util.ts:36-76) ------------------------

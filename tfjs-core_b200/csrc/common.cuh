@@ -190,6 +190,8 @@ int get_f32(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, int64_t min_elems, const char
 // An activation operand: float32 or half-precision storage.
 int get_activation(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, int64_t min_elems, const char* what,
                    TensorEntry** out);
+// An int32 operand of exactly `elems` elements (token ids, class lists).
+int get_i32(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, int64_t elems, const char* what, TensorEntry** out);
 // elementwise.cu: dst[i] = convert(src[i]) between the storage dtypes (float32, int32, bool, float16)
 int launch_convert(tfjs_cuda_ctx* ctx, const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n);
 

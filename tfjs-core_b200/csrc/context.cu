@@ -744,6 +744,16 @@ int get_activation(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, int64_t min_elems, con
   return wait_for_upload(ctx, t);
 }
 
+int get_i32(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, int64_t elems, const char* what, TensorEntry** out) {
+  TensorEntry* t = find_tensor(ctx, id);
+  if (!t) return set_error(ctx, TFJS_CUDA_ERR_NOT_FOUND, "%s: unknown tensor id %lld", what, (long long)id);
+  TFJS_REQUIRE(ctx, t->dtype == TFJS_I32, "%s must be stored as int32", what);
+  TFJS_REQUIRE(ctx, t->size == elems, "%s holds %lld elements, %lld expected", what, (long long)t->size,
+               (long long)elems);
+  *out = t;
+  return wait_for_upload(ctx, t);
+}
+
 int resolve_epilogue(tfjs_cuda_ctx* ctx, const tfjs_epilogue* epi, int64_t channels,
                      EpilogueArgs* out) {
   *out = EpilogueArgs();

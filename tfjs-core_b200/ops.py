@@ -658,6 +658,98 @@ def fused_softmax(logits):
     return ENGINE.runKernel(forward, "softmax", {"logits": logits}, _softmax_grad(logits.rank - 1))
 
 
+# ---- normalisation, lookup and loss of token and feature models (extensions) ---------------------
+def layer_norm(x, gamma=None, beta=None, axis=-1, epsilon=1e-5):
+    """Extension: (x - mean) / sqrt(var + epsilon) * gamma + beta over the inner-most axes `axis`;
+    gamma and beta have the shape of those axes.  Differentiable in x, gamma and beta."""
+    x = _convert(x, "x", "layerNorm")
+    axes = sorted(_parse_axes(axis, x.rank))
+    _assert(x.rank > 0 and axes and axes == list(range(x.rank - len(axes), x.rank)),
+            f"Error in layerNorm: axes must be inner-most, got axes {axes} and rank-{x.rank} input")
+    _assert(epsilon >= 0, f"Error in layerNorm: epsilon must not be negative, got {epsilon}.")
+    shape = x.shape[axes[0]:]
+    width = size_from_shape(shape)
+    weights = {}
+    for name, w in (("gamma", gamma), ("beta", beta)):
+        if w is not None:
+            w = _convert(w, name, "layerNorm")
+            _assert(w.shape == shape, f"Error in layerNorm: {name} must have shape {shape}, got {w.shape}.")
+            weights[name] = reshape(w, [width])
+    x2 = reshape(x, [size_from_shape(x.shape[:axes[0]]), width])
+    g1, b1 = weights.get("gamma"), weights.get("beta")
+
+    def forward(b, save):
+        y, stats = b.layerNorm(x2, g1, b1, epsilon, ENGINE.gradientDepth > 0)
+        if stats is not None:
+            save([x2, stats] + ([g1] if g1 is not None else []))
+            stats.dispose()
+        return y
+
+    def backward(dy, saved):
+        state = []
+
+        def gradients():
+            if not state:   # one kernel call gives all three
+                state.append(ENGINE.runKernel(
+                    lambda b: b.layerNormBackprop(dy, saved[0], saved[2] if g1 is not None else None, saved[1]),
+                    "layerNormBackprop"))
+            return state[0]
+        return {"x": lambda: gradients()[0], "gamma": lambda: gradients()[1], "beta": lambda: gradients()[2]}
+    res = ENGINE.runKernel(forward, "layerNorm", dict(weights, x=x2), backward)
+    out = reshape(res, x.shape)
+    for t in [x2, res] + list(weights.values()):
+        t.dispose()
+    return out
+
+
+def embedding_lookup(table, indices, scale=1.0):
+    """Extension: scale * table[indices] (tf.gather over axis 0, scaled); a row of zeros where an index
+    lies outside the table, which is how batches are padded.  Differentiable in the table."""
+    table = _convert(table, "table", "embeddingLookup")
+    indices = indices if isinstance(indices, Tensor) else tensor(indices, dtype="int32")
+    _assert(table.rank == 2, f"Error in embeddingLookup: table must be rank 2, but got rank {table.rank}.")
+    _assert(indices.dtype == "int32",
+            f"Argument 'indices' passed to 'embeddingLookup' must be int32 tensor, but got {indices.dtype} tensor")
+
+    def forward(b, save):
+        save([indices])
+        return b.embeddingLookup(table, indices, scale)
+
+    def backward(dy, saved):
+        return {"table": lambda: ENGINE.runKernel(
+            lambda b: b.embeddingLookupBackprop(dy, saved[0], table.shape[0], scale), "embeddingLookupBackprop")}
+    return ENGINE.runKernel(forward, "embeddingLookup", {"table": table}, backward)
+
+
+def distillation_loss(logits, teacherLogits, teacherIndices, temperature=1.0):
+    """Extension: the distillation loss T^2 * KL(p || q) of each row of `logits` [..., classes] against a
+    teacher's top logits [..., top] and their classes (int32; -1 ends a shorter list, and a row without
+    a teacher gives 0).  Differentiable in the logits; the teacher is a constant."""
+    logits = _convert(logits, "logits", "distillationLoss")
+    teacherLogits = _convert(teacherLogits, "teacherLogits", "distillationLoss")
+    teacherIndices = teacherIndices if isinstance(teacherIndices, Tensor) else tensor(teacherIndices, dtype="int32")
+    _assert(logits.rank > 0 and teacherLogits.shape[:-1] == logits.shape[:-1]
+            and teacherLogits.shape == teacherIndices.shape,
+            f"Error in distillationLoss: logits {logits.shape}, teacherLogits {teacherLogits.shape} and teacherIndices "
+            f"{teacherIndices.shape} must be [..., classes], [..., top] and [..., top].")
+    _assert(teacherIndices.dtype == "int32",
+            "Argument 'teacherIndices' passed to 'distillationLoss' must be int32 tensor, but got "
+            f"{teacherIndices.dtype} tensor")
+    _assert(temperature > 0, f"Error in distillationLoss: the temperature must be positive, got {temperature}.")
+
+    def forward(b, save):
+        loss, stats = b.distillationLoss(logits, teacherLogits, teacherIndices, temperature, ENGINE.gradientDepth > 0)
+        if stats is not None:
+            save([logits, teacherLogits, teacherIndices, stats])
+            stats.dispose()
+        return loss
+
+    def backward(dy, saved):
+        return {"logits": lambda: ENGINE.runKernel(
+            lambda b: b.distillationLossBackprop(dy, *saved, temperature), "distillationLossBackprop")}
+    return ENGINE.runKernel(forward, "distillationLoss", {"logits": logits}, backward)
+
+
 # ---- gradients (ops/gradients.ts) ----------------------------------------------------------------
 def grad(f):
     """tf.grad(f)(x, dy?) -> df/dx."""
