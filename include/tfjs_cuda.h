@@ -300,8 +300,8 @@ int tfjs_cuda_embedding_lookup_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id dy, t
  * q = softmax(logits[r] / T) over all classes, p = softmax(teacher_logits[r] / T) over the entries
  * whose index lies in [0, classes) and whose logit is above -inf (so -1 ends a shorter list; a class
  * named twice counts twice).  A row without such an entry has loss 0 and gradient 0.  top <= 1024.
- * stats, [rows, 2] (log-sum-exp of the student's and of the teacher's scaled logits) or 0, is what the
- * gradient reads. */
+ * stats, [rows, 4] (the largest logit and log2 of the sum beside it, of the student and of the teacher)
+ * or 0, is what the gradient reads. */
 int tfjs_cuda_distillation_loss(tfjs_cuda_ctx* ctx, tfjs_tensor_id logits, tfjs_tensor_id teacher_logits,
                                 tfjs_tensor_id teacher_indices, tfjs_tensor_id loss, tfjs_tensor_id stats,
                                 int64_t rows, int64_t classes, int64_t top, float temperature);

@@ -812,7 +812,7 @@ export class BackendCuda extends KernelBackend {
             teacherLogits.shape[logits.rank - 1]];
   }
 
-  /** T^2 * KL(p || q) of each row over the teacher's listed classes, and the statistics [..., 2] that
+  /** T^2 * KL(p || q) of each row over the teacher's listed classes, and the statistics [..., 4] that
    * the gradient reads (null unless `withStats`). */
   distillationLoss(logits: Tensor, teacherLogits: Tensor, teacherIndices: Tensor, temperature = 1,
                    withStats = true): [Tensor, Tensor|null] {
@@ -823,7 +823,7 @@ export class BackendCuda extends KernelBackend {
     const [iid, ti] = this.id(teacherIndices, 'int32');
     const outer = logits.shape.slice(0, -1);
     const loss = this.makeOutput<Tensor>(outer);
-    const stats = withStats ? this.makeOutput<Tensor>([...outer, 2]) : null;
+    const stats = withStats ? this.makeOutput<Tensor>([...outer, 4]) : null;
     const rc = binding.distillationLoss(this.ctx, zid, uid, iid, this.outId(loss), stats == null ? 0 : this.outId(stats),
                                         rows, classes, top, temperature);
     this.enqueued(rc, [loss, stats], [tz, tu, ti]);

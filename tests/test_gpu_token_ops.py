@@ -576,7 +576,7 @@ def test_refusals_leave_the_context_usable(tf):
         lambda: bk.distillationLoss(z(2, 8), z(2, 2), i(2, 2), 0.0),
         lambda: bk.distillationLoss(z(2, 8), z(2, 2), i(2, 2), float("inf")),
         lambda: bk.distillationLoss(z(2, 8), z(2, 2), i(2, 2), 1e-45),
-        lambda: bk.distillationLossBackprop(z(3), z(2, 8), z(2, 2), i(2, 2), z(2, 2)),
+        lambda: bk.distillationLossBackprop(z(3), z(2, 8), z(2, 2), i(2, 2), z(2, 4)),
         lambda: bk.distillationLossBackprop(z(2), z(2, 8), z(2, 2), i(2, 2), z(2, 3)),
         lambda: bk.layerNorm(bk.registerQuantized([2, 8], np.zeros(16), 1, 0), None, None, EPS),
     ]

@@ -763,7 +763,7 @@ class BackendCuda:
     def distillationLoss(self, logits, teacherLogits, teacherIndices, temperature=1.0, withStats=True):
         """Extension: T^2 * KL(p || q) of each row, q = softmax(logits / T) over all classes and
         p = softmax(teacherLogits / T) over the teacher's listed classes (an index outside the classes
-        does not count; a row without any gives 0).  Returns (loss, stats): stats, [..., 2], is what the
+        does not count; a row without any gives 0).  Returns (loss, stats): stats, [..., 4], is what the
         gradient reads, or None unless `withStats`."""
         self._assert_numeric([logits, teacherLogits], "distillationLoss")
         rows, classes, top = self._distillation_extent(logits, teacherLogits, teacherIndices)
@@ -771,7 +771,7 @@ class BackendCuda:
         uid, tu = self._activation_id(teacherLogits)
         iid, ti = self._id(teacherIndices, "int32")
         loss = self._out(logits.shape[:-1])
-        stats = self._out(logits.shape[:-1] + [2]) if withStats else None
+        stats = self._out(logits.shape[:-1] + [4]) if withStats else None
         rc = self._lib.tfjs_cuda_distillation_loss(self._ctx, zid, uid, iid, self._oid(loss), self._oid(stats), rows,
                                                    classes, top, float(temperature))
         self._enqueue(rc, (loss, stats), (tz, tu, ti))

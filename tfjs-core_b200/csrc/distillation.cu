@@ -7,125 +7,275 @@
 //   loss = T^2 sum_k p_k (log p_k - log q_{i_k})              (T^2 keeps the gradient's size)
 //   dz_v = dloss T (q_v - sum of p_k over the entries with i_k == v)
 //
-// A row without a counting entry has loss 0 and gradient 0.  The forward pass leaves the two
-// log-sum-exps (of z / T and of u / T; -inf for an empty list) for the backward pass.
-#include <cuda_fp16.h>
+// A row without a counting entry has loss 0 and gradient 0.
+//
+// Both softmaxes are taken relative to their largest logit, in raw units: exp2((z - max) * k) with
+// k = log2(e) / T, so that a row of the type's lowest values is still a uniform row.  The forward
+// pass leaves (max z, log2 of z's sum, max u, log2 of u's sum) of each row for the backward pass,
+// apart, because the logarithm would be lost beside a large maximum.  max u is -inf for an empty list.
+//
+// Both passes stream the logits once and are bound by memory.  A row starts anywhere, so its elements
+// before the first 16-byte boundary and behind the last one are taken one by one and all others in
+// 16-byte loads; the float32 gradient has the same element offsets, so its stores are aligned too.
+#include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "vec.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr int kMaxTop = 1024;
+constexpr int kThreads = 512;      // of a block of the loss
+constexpr int kGradThreads = 256;  // of a block of the gradient
+constexpr int kBatch = 4;          // 16-byte loads in flight a thread
+constexpr float kLn2 = 0.693147180559945f;
+constexpr float kLog2e = 1.44269504088896f;
 
-__device__ __forceinline__ float load_f32(const float* p) { return *p; }
-__device__ __forceinline__ float load_f32(const __half* p) { return __half2float(*p); }
-
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) v += scratch[w];
-  return v;
+// 2^v by the hardware's approximation (2 ulp); below 2^-126 it gives 0
+__device__ __forceinline__ float exp2_approx(float v) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
 }
-__device__ __forceinline__ float block_max(float v, float* scratch) {
+__device__ __forceinline__ float load_one(const float* p) { return *p; }
+__device__ __forceinline__ float load_one(const __half* p) { return __half2float(*p); }
+
+// Sum and NaN-keeping maximum over G threads: a warp, or the whole block.  `scratch`: G / 32 floats.
+template <int G>
+__device__ __forceinline__ float group_max(float v, float* scratch) {
+#pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = -INFINITY;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) v = max_nan(v, scratch[w]);
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = scratch[threadIdx.x & (G / 32 - 1)];
+#pragma unroll
+    for (int o = G / 64; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+  }
+  return v;
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float* scratch) {
+  v = lanes_sum<32>(v);
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = lanes_sum<G / 32>(scratch[threadIdx.x & (G / 32 - 1)]);
+  }
   return v;
 }
 
-// u / T of a counting entry, -inf of any other.
-template <typename TU>
-__device__ __forceinline__ float teacher_entry(const TU* u, int32_t i, int64_t classes, float inv_t) {
-  return i >= 0 && i < classes ? load_f32(u) * inv_t : -INFINITY;
-}
+// Where a row's 16-byte units lie: `head` elements before them, `vecs` units, `tail` elements behind.
+template <int V>
+struct RowSplit {
+  int head, vecs, tail;
+  __device__ RowSplit(int64_t first, int classes) {
+    head = (int)(-first & (V - 1));
+    if (head > classes) head = classes;
+    vecs = (classes - head) / V;
+    tail = classes - head - vecs * V;
+  }
+  // element of the i-th of the head + tail ones
+  __device__ int loose(int i) const { return i < head ? i : i + vecs * V; }
+};
 
-template <typename TZ, typename TU>
-__global__ void __launch_bounds__(kThreads) distillation_kernel(const TZ* __restrict__ z, const TU* __restrict__ u,
-                                                               const int32_t* __restrict__ indices,
-                                                               float* __restrict__ loss, float* __restrict__ stats,
-                                                               int64_t rows, int64_t classes, int top, float temperature) {
-  __shared__ float scratch[kThreads / 32];
-  const float inv_t = 1.f / temperature;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const TZ* zr = z + row * classes;
-    const TU* ur = u + row * top;
-    const int32_t* ir = indices + row * top;
-    float m = -INFINITY;
-    for (int64_t j = threadIdx.x; j < classes; j += kThreads) m = max_nan(m, load_f32(zr + j) * inv_t);
-    m = block_max(m, scratch);
-    float s = 0.f;
-    for (int64_t j = threadIdx.x; j < classes; j += kThreads) s += expf(load_f32(zr + j) * inv_t - m);
-    const float lse = m + logf(block_sum(s, scratch));
-    float um = -INFINITY;
-    for (int k = threadIdx.x; k < top; k += kThreads) um = max_nan(um, teacher_entry(ur + k, ir[k], classes, inv_t));
-    um = block_max(um, scratch);
-    float ulse = -INFINITY, l = 0.f;
-    if (um != -INFINITY) {  // the same for the whole block
-      s = 0.f;
-      for (int k = threadIdx.x; k < top; k += kThreads) s += expf(teacher_entry(ur + k, ir[k], classes, inv_t) - um);
-      ulse = um + logf(block_sum(s, scratch));
-      for (int k = threadIdx.x; k < top; k += kThreads) {
-        const float lp = teacher_entry(ur + k, ir[k], classes, inv_t) - ulse, p = expf(lp);
-        if (p != 0.f) l += p * (lp - (load_f32(zr + ir[k]) * inv_t - lse));
-      }
-      l = block_sum(l, scratch);
-    }
-    if (threadIdx.x == 0) {
-      loss[row] = temperature * temperature * l;
-      if (stats) {
-        stats[2 * row] = lse;
-        stats[2 * row + 1] = ulse;
+// max m and s = sum of 2^((z - m) k), joined with another pair
+__device__ __forceinline__ float shifted(float z, float m, float k) { return exp2_approx((z - (m == -INFINITY ? 0.f : m)) * k); }
+
+// G threads a row (a warp, or a block), C blocks a row (only with whole blocks).  NK: teacher entries a
+// thread, G * NK >= top.
+template <typename TZ, typename TU, int G, int NK>
+__global__ void __launch_bounds__(G > 32 ? kThreads : 256) distillation_kernel(
+    const TZ* __restrict__ z, const TU* __restrict__ u, const int32_t* __restrict__ indices, float* __restrict__ loss,
+    float* __restrict__ stats, int64_t rows, int classes, int top, float temperature, int C) {
+  constexpr int V = 16 / (int)sizeof(TZ);
+  __shared__ float scratch[5][32];
+  __shared__ float2 slot;
+  const int t = threadIdx.x & (G - 1);
+  const int rank = G > 32 ? (int)(blockIdx.x % C) : 0;
+  const int64_t row = G > 32 ? blockIdx.x / C : (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  if (G == 32 && row >= rows) return;  // whole warps
+  const float inv_t = 1.f / temperature, k2 = kLog2e * inv_t;
+  const int64_t first = row * classes;
+  const TZ* zr = z + first;
+  const RowSplit<V> split(first, classes);
+
+  // the teacher's entries, fetched ahead of the row (by the row's first block)
+  float tu[NK], tz[NK];
+  if (rank == 0) {
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      const int e = t + i * G;
+      tu[i] = -INFINITY;
+      tz[i] = 0.f;
+      if (e < top) {
+        const int32_t at = indices[row * top + e];
+        if (at >= 0 && at < classes) {
+          tu[i] = load_one(u + row * top + e);
+          tz[i] = load_one(zr + at);
+        }
       }
     }
   }
+
+  // ---- one pass over the row: running maximum and sum
+  float m = -INFINITY, s = 0.f;
+  if (rank == 0 && t < split.head + split.tail) {
+    m = load_one(zr + split.loose(t));
+    s = shifted(m, m, k2);
+  }
+  {
+    const TZ* body = zr + split.head;
+    const int lo = (int)((int64_t)split.vecs * rank / C), hi = (int)((int64_t)split.vecs * (rank + 1) / C);
+    for (int j = lo + t; j < hi; j += G * kBatch) {
+      float v[kBatch][V];
+#pragma unroll
+      for (int i = 0; i < kBatch; i++) {
+        if (j + i * G < hi) {
+          load_vec<V>(body + (int64_t)(j + i * G) * V, v[i]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; k++) v[i][k] = -INFINITY;
+        }
+      }
+      float b = m;
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+#pragma unroll
+        for (int k = 0; k < V; k++) b = max_nan(b, v[i][k]);
+      const float at = b == -INFINITY ? 0.f : b;
+      s *= exp2_approx((m - at) * k2);  // m = -inf: 0 * s = 0
+#pragma unroll
+      for (int i = 0; i < kBatch; i++)
+#pragma unroll
+        for (int k = 0; k < V; k++) s += exp2_approx((v[i][k] - at) * k2);
+      m = b;
+    }
+  }
+  float all = group_max<G>(m, scratch[0]);
+  s = group_sum<G>(s * shifted(m, all, k2), scratch[1]);
+  if (G > 32 && C > 1) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (threadIdx.x == 0) slot = make_float2(all, s);
+    cluster.sync();
+    if (rank == 0) {
+      float big = -INFINITY, sum = 0.f;
+      for (int i = 0; i < C; i++) big = max_nan(big, cluster.map_shared_rank(&slot, i)->x);
+      for (int i = 0; i < C; i++) {
+        const float2 o = *cluster.map_shared_rank(&slot, i);
+        sum += o.y * shifted(o.x, big, k2);
+      }
+      all = big;
+      s = sum;
+    }
+    cluster.sync();  // the other blocks' slots have been read
+    if (rank != 0) return;
+  }
+  // ---- the teacher's list, and the loss
+  float um = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NK; i++) um = max_nan(um, tu[i]);
+  um = group_max<G>(um, scratch[2]);
+  const float ls = log2f(s);
+  float uls = 0.f, l = 0.f;
+  if (um != -INFINITY) {  // the same for all threads of the row
+    float e = 0.f;
+#pragma unroll
+    for (int i = 0; i < NK; i++) e += exp2_approx((tu[i] - um) * k2);
+    uls = log2f(group_sum<G>(e, scratch[3]));
+#pragma unroll
+    for (int i = 0; i < NK; i++) {
+      const float lp = (tu[i] - um) * k2 - uls, p = exp2_approx(lp);
+      if (p != 0.f) l += p * (lp - ((tz[i] - all) * k2 - ls));
+    }
+    l = group_sum<G>(l, scratch[4]) * kLn2;
+  }
+  if (t == 0) {
+    loss[row] = temperature * temperature * l;
+    if (stats) *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(all, ls, um, uls);
+  }
 }
 
-template <typename TZ, typename TU>
-__global__ void __launch_bounds__(kThreads) distillation_backprop_kernel(
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if (G > 32) __syncthreads();
+  else __syncwarp();
+}
+
+// G threads take a tile of G * kBatch units of a row (the first tile also the loose elements): all
+// classes get c q_v, then the tile's listed classes are written again with their p taken off, by the
+// first entry that names the class.  `room`: entries of shared memory a group.
+template <typename TZ, typename TU, int G>
+__global__ void __launch_bounds__(kGradThreads) distillation_backprop_kernel(
     const float* __restrict__ dloss, const TZ* __restrict__ z, const TU* __restrict__ u,
     const int32_t* __restrict__ indices, const float* __restrict__ stats, float* __restrict__ dz, int64_t rows,
-    int64_t classes, int top, float temperature) {
-  __shared__ int32_t s_i[kMaxTop];
-  __shared__ float s_p[kMaxTop];
-  const float inv_t = 1.f / temperature;
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const TZ* zr = z + row * classes;
-    float* dr = dz + row * classes;
-    const float lse = stats[2 * row], ulse = stats[2 * row + 1], c = dloss[row] * temperature;
-    const bool empty = ulse == -INFINITY;
-    __syncthreads();
-    for (int k = threadIdx.x; k < top; k += kThreads) {
-      const int32_t i = indices[row * top + k];
-      const bool there = i >= 0 && i < classes && !empty;
-      s_i[k] = there ? i : -1;
-      s_p[k] = there ? expf(load_f32(u + row * top + k) * inv_t - ulse) : 0.f;
+    int classes, int top, float temperature, int tiles, int room) {
+  constexpr int V = 16 / (int)sizeof(TZ);
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int t = threadIdx.x & (G - 1), group = threadIdx.x / G;
+  const int64_t item = (int64_t)blockIdx.x * (kGradThreads / G) + group;
+  const int64_t row = item / tiles;
+  if (row >= rows) return;  // whole groups
+  const int tile = (int)(item - row * tiles);
+  int32_t* s_i = reinterpret_cast<int32_t*>(smem) + group * 2 * room;
+  float* s_p = reinterpret_cast<float*>(s_i) + room;
+  const float k2 = kLog2e * (1.f / temperature);
+  const int64_t first = row * classes;
+  const TZ* zr = z + first;
+  float* dr = dz + first;
+  const RowSplit<V> split(first, classes);
+  const int v0 = tile * G * kBatch;
+
+  float v[kBatch][V];
+#pragma unroll
+  for (int i = 0; i < kBatch; i++)
+    if (v0 + i * G + t < split.vecs) load_vec<V>(zr + split.head + (int64_t)(v0 + i * G + t) * V, v[i]);
+  const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
+  const float c = dloss[row] * temperature;
+  const bool empty = st.z == -INFINITY;
+  for (int e = t; e < room; e += G) {
+    int32_t at = -1;
+    float p = 0.f;
+    if (e < top && !empty) {
+      at = indices[row * top + e];
+      if (at >= 0 && at < classes) p = exp2_approx((load_one(u + row * top + e) - st.z) * k2 - st.w);
+      else at = -1;
     }
-    for (int64_t j = threadIdx.x; j < classes; j += kThreads)
-      dr[j] = empty ? 0.f : c * expf(load_f32(zr + j) * inv_t - lse);
-    __syncthreads();
-    // the entries' own classes: the first entry of a class writes q - (all its entries' p)
-    for (int k = threadIdx.x; k < top; k += kThreads) {
-      const int32_t i = s_i[k];
-      if (i < 0) continue;
-      float p = 0.f;
-      bool first = true;
-      for (int j = 0; j < top; j++) {
-        if (s_i[j] != i) continue;
-        if (j < k) {
-          first = false;
-          break;
-        }
-        p += s_p[j];
-      }
-      if (first) dr[i] = c * (expf(load_f32(zr + i) * inv_t - lse) - p);
+    s_i[e] = at;
+    s_p[e] = p;
+  }
+#pragma unroll
+  for (int i = 0; i < kBatch; i++) {
+    if (v0 + i * G + t < split.vecs) {
+#pragma unroll
+      for (int k = 0; k < V; k++) v[i][k] = empty ? 0.f : c * exp2_approx((v[i][k] - st.x) * k2 - st.y);
+      store_vec<V>(dr + split.head + (int64_t)(v0 + i * G + t) * V, v[i]);
     }
+  }
+  if (tile == 0 && t < split.head + split.tail) {
+    const int at = split.loose(t);
+    dr[at] = empty ? 0.f : c * exp2_approx((load_one(zr + at) - st.x) * k2 - st.y);
+  }
+  if (empty) return;  // the whole group
+  group_sync<G>();    // the list is there, and the classes are written before they are written again
+  const int lo = split.head + v0 * V, hi = split.head + min(v0 + G * kBatch, split.vecs) * V;
+  for (int e = t; e < top; e += G) {
+    const int32_t at = s_i[e];
+    if (at < 0) continue;
+    const bool loose = at < split.head || at >= split.head + split.vecs * V;
+    if (loose ? tile != 0 : (at < lo || at >= hi)) continue;
+    float p = 0.f;
+    bool is_first = true;
+    for (int j = 0; j < top; j += 4) {  // room is a multiple of 4; the entries behind top hold -1
+      const int4 q = *reinterpret_cast<const int4*>(s_i + j);
+      if (q.x == at) is_first &= j >= e, p += s_p[j];
+      if (q.y == at) is_first &= j + 1 >= e, p += s_p[j + 1];
+      if (q.z == at) is_first &= j + 2 >= e, p += s_p[j + 2];
+      if (q.w == at) is_first &= j + 3 >= e, p += s_p[j + 3];
+    }
+    if (is_first) dr[at] = c * (exp2_approx((load_one(zr + at) - st.x) * k2 - st.y) - p);
   }
 }
 
@@ -136,7 +286,7 @@ struct Operands {
 int get_operands(tfjs_cuda_ctx* ctx, tfjs_tensor_id z, tfjs_tensor_id u, tfjs_tensor_id indices, int64_t rows,
                  int64_t classes, int64_t top, float temperature, Operands* o) {
   TFJS_REQUIRE(ctx, rows >= 0 && classes >= 0 && top >= 0, "negative extent");
-  TFJS_REQUIRE(ctx, classes < (1ll << 31) && rows <= (1ll << 60) / (classes > kMaxTop ? classes : kMaxTop),
+  TFJS_REQUIRE(ctx, classes < (1ll << 31) - 65536 && rows < (1ll << 27) && rows <= (1ll << 60) / (classes > kMaxTop ? classes : kMaxTop),
                "distillationLoss: too many rows or classes");
   TFJS_REQUIRE(ctx, top <= kMaxTop, "distillationLoss: a teacher's list holds at most %d entries, got %lld", kMaxTop,
                (long long)top);
@@ -160,21 +310,49 @@ int get_rows(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, int64_t elems, const char* w
 }
 
 template <typename TZ, typename TU>
-void launch_forward(tfjs_cuda_ctx* ctx, const Operands& o, float* loss, float* stats, int64_t rows, int64_t classes,
-                    int top, float temperature) {
-  const int64_t cap = (int64_t)ctx->sm_count * 8;
-  distillation_kernel<TZ, TU><<<(unsigned)(rows < cap ? rows : cap), kThreads, 0, ctx->stream>>>(
-      (const TZ*)o.z->ptr, (const TU*)o.u->ptr, (const int32_t*)o.indices->ptr, loss, stats, rows, classes, top,
-      temperature);
+int launch_forward(tfjs_cuda_ctx* ctx, const Operands& o, float* loss, float* stats, int64_t rows, int64_t classes,
+                   int top, float temperature) {
+  const TZ* z = (const TZ*)o.z->ptr;
+  const TU* u = (const TU*)o.u->ptr;
+  const int32_t* indices = (const int32_t*)o.indices->ptr;
+  if (classes <= 1024 && top <= 128) {
+    distillation_kernel<TZ, TU, 32, 4><<<(unsigned)ceil_div64(rows, 8), 256, 0, ctx->stream>>>(
+        z, u, indices, loss, stats, rows, (int)classes, top, temperature, 1);
+    return post_launch(ctx, "distillationLoss (warps)");
+  }
+  // few rows: up to 8 blocks share one, while each still has 8192 classes or more
+  int C = 1;
+  while (C < 8 && rows * C * 2 <= 2 * ctx->sm_count && classes / (2 * C) >= 8192) C *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * C));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = C;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  TFJS_CHECK_CUDA(ctx, cudaLaunchKernelEx(&cfg, distillation_kernel<TZ, TU, kThreads, 2>, z, u, indices, loss, stats, rows,
+                                          (int)classes, top, temperature, C));
+  return post_launch(ctx, "distillationLoss");
 }
 
 template <typename TZ, typename TU>
-void launch_backward(tfjs_cuda_ctx* ctx, const float* dloss, const Operands& o, const float* stats, float* dz,
-                     int64_t rows, int64_t classes, int top, float temperature) {
-  const int64_t cap = (int64_t)ctx->sm_count * 8;
-  distillation_backprop_kernel<TZ, TU><<<(unsigned)(rows < cap ? rows : cap), kThreads, 0, ctx->stream>>>(
-      dloss, (const TZ*)o.z->ptr, (const TU*)o.u->ptr, (const int32_t*)o.indices->ptr, stats, dz, rows, classes, top,
-      temperature);
+int launch_backward(tfjs_cuda_ctx* ctx, const float* dloss, const Operands& o, const float* stats, float* dz,
+                    int64_t rows, int64_t classes, int top, float temperature) {
+  constexpr int V = 16 / (int)sizeof(TZ);
+  const bool warps = classes <= 32 * kBatch * V * 2 && top <= 128;
+  const int G = warps ? 32 : kGradThreads, groups = kGradThreads / G;
+  const int64_t tiles = classes <= G * kBatch * V ? 1 : ceil_div64(classes, (int64_t)G * kBatch * V);
+  const int64_t blocks = ceil_div64(rows * tiles, groups);
+  TFJS_REQUIRE(ctx, blocks < (1ll << 31), "distillationLossBackprop: too many rows times classes");
+  const int room = (top + 3) / 4 * 4;
+  auto kernel = warps ? distillation_backprop_kernel<TZ, TU, 32> : distillation_backprop_kernel<TZ, TU, kGradThreads>;
+  kernel<<<(unsigned)blocks, kGradThreads, (size_t)groups * room * 8, ctx->stream>>>(
+      dloss, (const TZ*)o.z->ptr, (const TU*)o.u->ptr, (const int32_t*)o.indices->ptr, stats, dz, rows, (int)classes, top,
+      temperature, (int)tiles, room);
+  return post_launch(ctx, "distillationLossBackprop");
 }
 
 }  // namespace
@@ -188,7 +366,7 @@ extern "C" int tfjs_cuda_distillation_loss(tfjs_cuda_ctx* ctx, tfjs_tensor_id lo
   TensorEntry *loss, *stats = nullptr;
   int rc = get_operands(ctx, logits_id, teacher_logits_id, teacher_indices_id, rows, classes, top, temperature, &o);
   if (!rc) rc = get_rows(ctx, loss_id, rows, "distillationLoss output", &loss);
-  if (!rc && stats_id) rc = get_rows(ctx, stats_id, 2 * rows, "distillationLoss statistics", &stats);
+  if (!rc && stats_id) rc = get_rows(ctx, stats_id, 4 * rows, "distillationLoss statistics", &stats);
   if (rc) return rc;
   TFJS_REQUIRE(ctx, loss != o.z && loss != o.u && loss != stats && (!stats || (stats != o.z && stats != o.u)),
                "distillationLoss: an output cannot be one of the inputs or another output");
@@ -199,8 +377,7 @@ extern "C" int tfjs_cuda_distillation_loss(tfjs_cuda_ctx* ctx, tfjs_tensor_id lo
   const bool hz = o.z->dtype == TFJS_F16, hu = o.u->dtype == TFJS_F16;
   auto launch = hz ? (hu ? launch_forward<__half, __half> : launch_forward<__half, float>)
                    : (hu ? launch_forward<float, __half> : launch_forward<float, float>);
-  launch(ctx, o, (float*)loss->ptr, stats ? (float*)stats->ptr : nullptr, rows, classes, (int)top, temperature);
-  return post_launch(ctx, "distillationLoss");
+  return launch(ctx, o, (float*)loss->ptr, stats ? (float*)stats->ptr : nullptr, rows, classes, (int)top, temperature);
 }
 
 extern "C" int tfjs_cuda_distillation_loss_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id dloss_id, tfjs_tensor_id logits_id,
@@ -212,7 +389,7 @@ extern "C" int tfjs_cuda_distillation_loss_backprop(tfjs_cuda_ctx* ctx, tfjs_ten
   TensorEntry *dloss, *stats, *dz;
   int rc = get_operands(ctx, logits_id, teacher_logits_id, teacher_indices_id, rows, classes, top, temperature, &o);
   if (!rc) rc = get_rows(ctx, dloss_id, rows, "dloss", &dloss);
-  if (!rc) rc = get_rows(ctx, stats_id, 2 * rows, "distillationLoss statistics", &stats);
+  if (!rc) rc = get_rows(ctx, stats_id, 4 * rows, "distillationLoss statistics", &stats);
   if (!rc) rc = get_rows(ctx, dlogits_id, rows * classes, "dlogits", &dz);
   if (rc) return rc;
   TFJS_REQUIRE(ctx, dz != o.z && dz != o.u && dz != dloss && dz != stats,
@@ -223,6 +400,6 @@ extern "C" int tfjs_cuda_distillation_loss_backprop(tfjs_cuda_ctx* ctx, tfjs_ten
   const bool hz = o.z->dtype == TFJS_F16, hu = o.u->dtype == TFJS_F16;
   auto launch = hz ? (hu ? launch_backward<__half, __half> : launch_backward<__half, float>)
                    : (hu ? launch_backward<float, __half> : launch_backward<float, float>);
-  launch(ctx, (const float*)dloss->ptr, o, (const float*)stats->ptr, (float*)dz->ptr, rows, classes, (int)top, temperature);
-  return post_launch(ctx, "distillationLossBackprop");
+  return launch(ctx, (const float*)dloss->ptr, o, (const float*)stats->ptr, (float*)dz->ptr, rows, classes, (int)top,
+                temperature);
 }

@@ -4,129 +4,684 @@
 //   with n = (x - m) r and a = dy g:
 //   dx = r (a - mean(a) - n mean(a n)),   dg = sum over rows of dy n,   db = sum over rows of dy
 //
-// All sums are float32 or wider; a half-stored x is widened on load and y rounded once on store.
-#include <cuda_fp16.h>
+// All sums are float32; a half-stored x or dy is widened on load, a half-stored y rounded once on
+// store.  Every sum has a fixed order, so equal inputs give equal bits.
+//
+// Forward.  A row is read once and stays on chip: the mean and then the centred square sum (which
+// does not cancel, unlike E[x^2] - m^2) come from the same registers.  Three forms by width:
+//   up to 1024     L lanes a row (4 .. 32), no shared memory
+//   up to 16384    one block a row
+//   above          a cluster of 8 blocks a row, the row in their shared memory, sums joined over DSMEM
+// Gradient.  One pass over dy and x gives dx and, per block, the weights' gradients:
+//   up to 8192     persistent blocks; a ring of stages (several rows each) filled by cp.async.  First
+//                  the lanes of a row sum a and a n, then every thread takes the same columns of every
+//                  row: it writes dx and keeps its columns' dg, db in registers.
+//   above          a cluster of 8 blocks a row; dg, db accumulate in a buffer of the cluster's own
+// and a second kernel adds the blocks' partial dg, db in order.
+#include <cooperative_groups.h>
 
 #include "common.cuh"
+#include "vec.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 256;
+// y = (x - mean) * rstd * gamma + beta for V columns from `col`
+template <int V, typename TY>
+__device__ __forceinline__ void finish_vec(const float (&x)[V], float mean, float rstd, const float* __restrict__ gamma,
+                                           const float* __restrict__ beta, int64_t col, TY* y) {
+  float o[V], w[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) o[i] = (x[i] - mean) * rstd;
+  if (gamma) {
+    load_vec<V>(gamma + col, w);
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] *= w[i];
+  }
+  if (beta) {
+    load_vec<V>(beta + col, w);
+#pragma unroll
+    for (int i = 0; i < V; i++) o[i] += w[i];
+  }
+  store_vec<V>(y, o);
+}
 
-__device__ __forceinline__ float load_f32(const float* p) { return *p; }
-__device__ __forceinline__ float load_f32(const __half* p) { return __half2float(*p); }
-__device__ __forceinline__ void store_f32(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_f32(__half* p, float v) { *p = __float2half_rn(v); }
-
-// Sum over the block; every thread gets it.  The order is fixed, so equal inputs give equal bits.
+// Sum over a block of NT threads; every thread gets it.  `scratch` holds NT / 32 floats of its own.
+template <int NT>
 __device__ __forceinline__ float block_sum(float v, float* scratch) {
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  __syncthreads();
+  v = lanes_sum<32>(v);
   if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
   __syncthreads();
-  v = 0.f;
-  for (int w = 0; w < (int)(blockDim.x >> 5); w++) v += scratch[w];
-  return v;
+  return lanes_sum<NT / 32>(scratch[threadIdx.x & (NT / 32 - 1)]);
 }
 
-template <typename TX, typename TY>
-__global__ void __launch_bounds__(kThreads) layer_norm_kernel(const TX* __restrict__ x, const float* __restrict__ gamma,
+// ---- forward -------------------------------------------------------------------------------------
+// L lanes a row, NV vectors of V values a lane: width <= L * NV * V, a multiple of V.
+template <typename TX, typename TY, int V, int NV, int L>
+__global__ void __launch_bounds__(256) layer_norm_lanes_kernel(const TX* __restrict__ x, const float* __restrict__ gamma,
+                                                              const float* __restrict__ beta, TY* __restrict__ y,
+                                                              float* __restrict__ stats, int64_t rows, int width,
+                                                              float epsilon) {
+  const int lane = threadIdx.x & (L - 1);
+  const int64_t step = (int64_t)gridDim.x * (256 / L);
+  // all lanes of a warp go round the loop together, so that the shuffles see every lane
+  for (int64_t base = (int64_t)blockIdx.x * (256 / L); base < rows; base += step) {
+    const int64_t row = base + threadIdx.x / L;
+    const bool there = row < rows;
+    const TX* r = x + row * width;
+    float v[NV][V];
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int col = (i * L + lane) * V;
+      if (there && col < width) {
+        load_vec<V>(r + col, v[i]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; k++) v[i][k] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int k = 0; k < V; k++) s += v[i][k];
+    const float mean = lanes_sum<L>(s) / (float)width;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      if ((i * L + lane) * V < width) {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+          const float d = v[i][k] - mean;
+          s = fmaf(d, d, s);
+        }
+      }
+    const float rstd = 1.f / sqrtf(lanes_sum<L>(s) / (float)width + epsilon);
+    if (!there) continue;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int col = (i * L + lane) * V;
+      if (col < width) finish_vec<V>(v[i], mean, rstd, gamma, beta, col, y + row * width + col);
+    }
+    if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
+  }
+}
+
+// One block of NT threads a row: width <= NT * NV * V, a multiple of V.
+template <typename TX, typename TY, int V, int NV, int NT>
+__global__ void __launch_bounds__(NT) layer_norm_block_kernel(const TX* __restrict__ x, const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, TY* __restrict__ y,
-                                                             float* __restrict__ stats, int64_t rows, int64_t width,
+                                                             float* __restrict__ stats, int64_t rows, int width,
                                                              float epsilon) {
-  __shared__ float scratch[kThreads / 32];
+  __shared__ float scratch[2][32];  // one for each sum of a row: its readers are done before its next writers start
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
     const TX* r = x + row * width;
+    float v[NV][V];
     float s = 0.f;
-    for (int64_t j = threadIdx.x; j < width; j += kThreads) s += load_f32(r + j);
-    const float mean = block_sum(s, scratch) / (float)width;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int col = (i * NT + threadIdx.x) * V;
+      if (col < width) {
+        load_vec<V>(r + col, v[i]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; k++) v[i][k] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int k = 0; k < V; k++) s += v[i][k];
+    const float mean = block_sum<NT>(s, scratch[0]) / (float)width;
     s = 0.f;
-    for (int64_t j = threadIdx.x; j < width; j += kThreads) {
-      const float d = load_f32(r + j) - mean;
-      s += d * d;
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+      if ((i * NT + (int)threadIdx.x) * V < width) {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+          const float d = v[i][k] - mean;
+          s = fmaf(d, d, s);
+        }
+      }
+    const float rstd = 1.f / sqrtf(block_sum<NT>(s, scratch[1]) / (float)width + epsilon);
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int col = (i * NT + threadIdx.x) * V;
+      if (col < width) finish_vec<V>(v[i], mean, rstd, gamma, beta, col, y + row * width + col);
     }
-    const float rstd = 1.f / sqrtf(block_sum(s, scratch) / (float)width + epsilon);
-    for (int64_t j = threadIdx.x; j < width; j += kThreads) {
-      float v = (load_f32(r + j) - mean) * rstd;
-      if (gamma) v *= gamma[j];
-      if (beta) v += beta[j];
-      store_f32(y + row * width + j, v);
+    if (stats && threadIdx.x == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
+  }
+}
+
+constexpr int kClusterBlocks = 8;
+constexpr int kClusterThreads = 512;
+
+// Sum over the cluster in the order of its blocks.  `mine` is this block's slot in its own shared
+// memory; two uses of the same slot must have another cluster-wide sum between them.
+__device__ __forceinline__ float2 cluster_sum(float a, float b, float2* slot, float* scratch) {
+  cg::cluster_group cluster = cg::this_cluster();
+  a = lanes_sum<32>(a);
+  b = lanes_sum<32>(b);
+  if ((threadIdx.x & 31) == 0) {
+    scratch[2 * (threadIdx.x >> 5)] = a;
+    scratch[2 * (threadIdx.x >> 5) + 1] = b;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int w = threadIdx.x & (kClusterThreads / 32 - 1);
+    a = lanes_sum<kClusterThreads / 32>(scratch[2 * w]);
+    b = lanes_sum<kClusterThreads / 32>(scratch[2 * w + 1]);
+    if (threadIdx.x == 0) *slot = make_float2(a, b);
+  }
+  cluster.sync();
+  float2 t = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < kClusterBlocks; i++) {
+    const float2 o = *cluster.map_shared_rank(slot, i);
+    t.x += o.x;
+    t.y += o.y;
+  }
+  return t;
+}
+
+// A cluster of 8 blocks a row.  `cached`: the block's share of the row fits into its dynamic shared
+// memory and is read from there the second and third time, else from global memory (L2).
+template <typename TX, typename TY, int V>
+__global__ void __launch_bounds__(kClusterThreads) layer_norm_cluster_kernel(
+    const TX* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, TY* __restrict__ y,
+    float* __restrict__ stats, int64_t rows, int64_t width, float epsilon, int cached) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float scratch[2][2 * kClusterThreads / 32];
+  __shared__ float2 slot[2];
+  TX* kept = reinterpret_cast<TX*>(smem);
+  const int64_t vecs = width / V, clusters = gridDim.x / kClusterBlocks;
+  const int64_t rank = blockIdx.x % kClusterBlocks;
+  const int64_t lo = vecs * rank / kClusterBlocks, n = vecs * (rank + 1) / kClusterBlocks - lo;
+  for (int64_t row = blockIdx.x / kClusterBlocks; row < rows; row += clusters) {
+    const TX* r = x + row * width + lo * V;
+    float s = 0.f;
+#pragma unroll 4
+    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+      float v[V];
+      load_vec<V>(r + j * V, v);
+      if (cached) store_vec<V>(kept + j * V, v);  // exact: the values came from this type
+#pragma unroll
+      for (int k = 0; k < V; k++) s += v[k];
     }
-    if (stats && threadIdx.x == 0) {
-      stats[2 * row] = mean;
-      stats[2 * row + 1] = rstd;
+    const float mean = cluster_sum(s, 0.f, &slot[0], scratch[0]).x / (float)width;
+    s = 0.f;
+    const TX* from = cached ? kept : r;  // a thread reads back only what it wrote
+#pragma unroll 4
+    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+      float v[V];
+      load_vec<V>(from + j * V, v);
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float d = v[k] - mean;
+        s = fmaf(d, d, s);
+      }
+    }
+    const float rstd = 1.f / sqrtf(cluster_sum(s, 0.f, &slot[1], scratch[1]).x / (float)width + epsilon);
+#pragma unroll 2
+    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+      float v[V];
+      load_vec<V>(from + j * V, v);
+      finish_vec<V>(v, mean, rstd, gamma, beta, (lo + j) * V, y + row * width + (lo + j) * V);
+    }
+    if (stats && rank == 0 && threadIdx.x == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
+  }
+  cg::this_cluster().sync();  // no block leaves while another may still read its slot
+}
+
+// ---- gradient, width <= kStagedWidth -----------------------------------------------------------------
+constexpr int kStagedWidth = 8192;
+constexpr int kStagedThreads = 512;
+constexpr int kMaxStageRows = 512;
+
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+struct StagedParams {
+  const float* gamma;
+  const float* stats;
+  float* dx;
+  float* partial;  // [gridDim.x][2][width] or null
+  int64_t rows, items;
+  int width, stage_rows;        // stage_rows: a power of two
+  int x_bytes, stage_bytes;     // of the dy and the whole stage area
+};
+
+// The whole 16-byte units that [first, first + bytes) touches, into shared memory.  The units lie
+// within the tensor's buffer: its start is 16-byte aligned and its size class a multiple of 16.
+__device__ __forceinline__ void stage_copy(uint8_t* dst, const uint8_t* base, int64_t first, int bytes) {
+  const int64_t lo = first & ~15ll;
+  const int units = (int)((first + bytes - lo + 15) >> 4);
+  for (int i = threadIdx.x; i < units; i += kStagedThreads) copy_async16(dst + i * 16, base + lo + (int64_t)i * 16);
+}
+
+constexpr int kStages = 3;
+
+template <typename TD, typename TX, int V, int MC, int MINB>
+__global__ void __launch_bounds__(kStagedThreads, MINB) layer_norm_staged_kernel(const TD* __restrict__ dy,
+                                                                                 const TX* __restrict__ x,
+                                                                                 StagedParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int width = p.width, R = p.stage_rows, nc = width / V;
+  const int tid = threadIdx.x, lane = tid & 31;
+  uint8_t* ring = smem;
+  float* s_gamma = reinterpret_cast<float*>(smem + kStages * p.stage_bytes);
+  const int LR = R >= kStagedThreads ? 1 : kStagedThreads / R;   // lanes that sum a row
+  const int parts = LR > 32 ? LR / 32 : 1;                       // their warps' partial sums
+  float2* s_part = reinterpret_cast<float2*>(s_gamma + (width + 3) / 4 * 4);
+
+  for (int j = tid; j < width; j += kStagedThreads) s_gamma[j] = p.gamma ? p.gamma[j] : 1.f;
+
+  // phase 2: thread -> columns; several row groups share the block where a row has few columns
+  const int RG = nc < kStagedThreads ? kStagedThreads / nc : 1;
+  const int rg = nc < kStagedThreads ? tid / nc : 0;
+  const int c0 = nc < kStagedThreads ? tid - rg * nc : tid;
+  const bool owner = rg < RG;
+  float dg[MC][V], db[MC][V];
+#pragma unroll
+  for (int i = 0; i < MC; i++)
+#pragma unroll
+    for (int k = 0; k < V; k++) dg[i][k] = db[i][k] = 0.f;
+
+  const int64_t first = blockIdx.x, step = gridDim.x;
+  auto fill = [&](int64_t item, int slot) {
+    if (item < p.items) {
+      const int64_t row = item * R;
+      const int n = (int)(p.rows - row < R ? p.rows - row : R);
+      uint8_t* dst = ring + slot * p.stage_bytes;
+      stage_copy(dst, (const uint8_t*)dy, row * width * (int64_t)sizeof(TD), n * width * (int)sizeof(TD));
+      stage_copy(dst + p.x_bytes, (const uint8_t*)x, row * width * (int64_t)sizeof(TX), n * width * (int)sizeof(TX));
+      float2* st = reinterpret_cast<float2*>(dst + p.stage_bytes) - R;
+      for (int i = tid; i < n; i += kStagedThreads) copy_async8(st + i, p.stats + 2 * (row + i));
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < kStages - 1; s++) fill(first + s * step, s);
+
+  int slot = 0;
+  for (int64_t item = first; item < p.items; item += step) {
+    copy_wait<kStages - 2>();
+    __syncthreads();  // this stage has arrived for all; the stage before it has been read by all
+    fill(item + (kStages - 1) * step, slot == 0 ? kStages - 1 : slot - 1);
+    const int64_t row0 = item * R;
+    const int n = (int)(p.rows - row0 < R ? p.rows - row0 : R);
+    const uint8_t* st = ring + slot * p.stage_bytes;
+    const TD* sd = reinterpret_cast<const TD*>(st + ((row0 * width * (int64_t)sizeof(TD)) & 15));
+    const TX* sx = reinterpret_cast<const TX*>(st + p.x_bytes + ((row0 * width * (int64_t)sizeof(TX)) & 15));
+    const float2* ss = reinterpret_cast<const float2*>(st + p.stage_bytes) - R;
+    // ---- phase 1: sum a and a n of each row
+    {
+      const int l = tid & (LR - 1);
+      const int row = tid / LR;   // groups of LR threads, one row each (R * LR >= the block)
+      float sa = 0.f, sn = 0.f;
+      if (row < n) {
+        const float2 mr = ss[row];
+        for (int j = l; j < nc; j += LR) {
+          float d[V], v[V], g[V];
+          load_vec<V>(sd + row * width + j * V, d);
+          load_vec<V>(sx + row * width + j * V, v);
+          load_vec<V>(s_gamma + j * V, g);
+#pragma unroll
+          for (int k = 0; k < V; k++) {
+            const float a = d[k] * g[k];
+            sa += a;
+            sn = fmaf(a, (v[k] - mr.x) * mr.y, sn);
+          }
+        }
+      }
+      const int w = LR < 32 ? LR : 32;
+      for (int o = w >> 1; o > 0; o >>= 1) {
+        sa += __shfl_xor_sync(0xffffffffu, sa, o);
+        sn += __shfl_xor_sync(0xffffffffu, sn, o);
+      }
+      if ((l & 31) == 0 && row < R) s_part[row * parts + (l >> 5)] = make_float2(sa, sn);
+    }
+    __syncthreads();
+    // ---- phase 2: dx, and the owned columns' dg and db
+    if (owner) {
+      for (int row = rg; row < n; row += RG) {
+        float2 t = make_float2(0.f, 0.f);
+        for (int i = 0; i < parts; i++) {
+          const float2 o = s_part[row * parts + i];
+          t.x += o.x;
+          t.y += o.y;
+        }
+        const float ma = t.x / (float)width, man = t.y / (float)width;
+        const float2 mr = ss[row];
+#pragma unroll
+        for (int i = 0; i < MC; i++) {
+          const int c = c0 + i * kStagedThreads;
+          if (c >= nc) break;
+          float d[V], v[V], g[V], o[V];
+          load_vec<V>(sd + row * width + c * V, d);
+          load_vec<V>(sx + row * width + c * V, v);
+          load_vec<V>(s_gamma + c * V, g);
+#pragma unroll
+          for (int k = 0; k < V; k++) {
+            const float nn = (v[k] - mr.x) * mr.y;
+            o[k] = mr.y * (d[k] * g[k] - ma - nn * man);
+            dg[i][k] = fmaf(d[k], nn, dg[i][k]);
+            db[i][k] += d[k];
+          }
+          if (p.dx) store_vec<V>(p.dx + (row0 + row) * width + c * V, o);
+        }
+      }
+    }
+    if (++slot == kStages) slot = 0;
+  }
+  if (!p.partial) return;
+  // ---- the row groups' sums, in order; then this block's partial sums
+  float* mine = p.partial + (int64_t)blockIdx.x * 2 * width;
+  if (RG > 1) {
+    copy_wait<0>();
+    __syncthreads();
+    float* join = reinterpret_cast<float*>(ring);  // [RG][2][width]
+    if (owner) {
+      store_vec<V>(join + (rg * 2) * width + c0 * V, dg[0]);
+      store_vec<V>(join + (rg * 2 + 1) * width + c0 * V, db[0]);
+    }
+    __syncthreads();
+    for (int j = tid; j < 2 * width; j += kStagedThreads) {
+      float s = 0.f;
+      for (int g = 0; g < RG; g++) s += join[g * 2 * width + j];
+      mine[j] = s;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < MC; i++) {
+      const int c = c0 + i * kStagedThreads;
+      if (owner && c < nc) {
+        store_vec<V>(mine + c * V, dg[i]);
+        store_vec<V>(mine + width + c * V, db[i]);
+      }
     }
   }
 }
 
-template <typename TD, typename TX>
-__global__ void __launch_bounds__(kThreads) layer_norm_dx_kernel(const TD* __restrict__ dy, const TX* __restrict__ x,
-                                                                const float* __restrict__ gamma,
-                                                                const float* __restrict__ stats, float* __restrict__ dx,
-                                                                int64_t rows, int64_t width) {
-  __shared__ float scratch[kThreads / 32];
-  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const int64_t at = row * width;
-    const float mean = stats[2 * row], rstd = stats[2 * row + 1];
-    float sa = 0.f, san = 0.f;
-    for (int64_t j = threadIdx.x; j < width; j += kThreads) {
-      const float a = load_f32(dy + at + j) * (gamma ? gamma[j] : 1.f);
-      sa += a;
-      san += a * ((load_f32(x + at + j) - mean) * rstd);
+// ---- gradient, longer rows: a cluster of 8 blocks a row --------------------------------------------
+// The row is read twice (the second time from L2).  partial [clusters][2][width]: each thread adds
+// its own columns there, the first row of the cluster stores.
+template <typename TD, typename TX, int V>
+__global__ void __launch_bounds__(kClusterThreads) layer_norm_backprop_cluster_kernel(
+    const TD* __restrict__ dy, const TX* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ stats,
+    float* __restrict__ dx, float* __restrict__ partial, int64_t rows, int64_t width) {
+  __shared__ float scratch[2][2 * kClusterThreads / 32];
+  __shared__ float2 slot[2];
+  const int64_t vecs = width / V, clusters = gridDim.x / kClusterBlocks, cluster = blockIdx.x / kClusterBlocks;
+  const int64_t rank = blockIdx.x % kClusterBlocks;
+  const int64_t lo = vecs * rank / kClusterBlocks * V, n = vecs * (rank + 1) / kClusterBlocks - vecs * rank / kClusterBlocks;
+  float* pg = partial ? partial + cluster * 2 * width + lo : nullptr;
+  int turn = 0;
+  for (int64_t row = cluster; row < rows; row += clusters, turn ^= 1) {
+    const TD* d0 = dy + row * width + lo;
+    const TX* x0 = x + row * width + lo;
+    const float2 mr = *reinterpret_cast<const float2*>(stats + 2 * row);
+    float sa = 0.f, sn = 0.f;
+#pragma unroll 4
+    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+      float d[V], v[V], g[V];
+      load_vec<V>(d0 + j * V, d);
+      load_vec<V>(x0 + j * V, v);
+      if (gamma) load_vec<V>(gamma + lo + j * V, g);
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float a = gamma ? d[k] * g[k] : d[k];
+        sa += a;
+        sn = fmaf(a, (v[k] - mr.x) * mr.y, sn);
+      }
     }
-    const float ma = block_sum(sa, scratch) / (float)width;
-    const float man = block_sum(san, scratch) / (float)width;
-    for (int64_t j = threadIdx.x; j < width; j += kThreads) {
-      const float a = load_f32(dy + at + j) * (gamma ? gamma[j] : 1.f);
-      const float n = (load_f32(x + at + j) - mean) * rstd;
-      dx[at + j] = rstd * (a - ma - n * man);
+    const float2 t = cluster_sum(sa, sn, &slot[turn], scratch[turn]);
+    const float ma = t.x / (float)width, man = t.y / (float)width;
+#pragma unroll 2
+    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+      float d[V], v[V], g[V], o[V], wg[V], wb[V];
+      load_vec<V>(d0 + j * V, d);
+      load_vec<V>(x0 + j * V, v);
+      if (gamma) load_vec<V>(gamma + lo + j * V, g);
+      if (pg && row != cluster) {
+        load_vec<V>(pg + j * V, wg);
+        load_vec<V>(pg + width + j * V, wb);
+      } else {
+#pragma unroll
+        for (int k = 0; k < V; k++) wg[k] = wb[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float nn = (v[k] - mr.x) * mr.y;
+        o[k] = mr.y * ((gamma ? d[k] * g[k] : d[k]) - ma - nn * man);
+        wg[k] = fmaf(d[k], nn, wg[k]);
+        wb[k] += d[k];
+      }
+      if (dx) store_vec<V>(dx + row * width + lo + j * V, o);
+      if (pg) {
+        store_vec<V>(pg + j * V, wg);
+        store_vec<V>(pg + width + j * V, wb);
+      }
     }
+  }
+  cg::this_cluster().sync();
+}
+
+// out[j] = sum over the blocks, in order, of partial[block][j]: 32 columns a block, 8 threads a column
+// take every eighth block's row and join theirs in order.  j runs over dg and then db.
+__global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __restrict__ partial, float* __restrict__ dgamma,
+                                                             float* __restrict__ dbeta, int blocks, int64_t width) {
+  __shared__ float part[8][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int64_t j0 = (int64_t)blockIdx.x * 32; j0 < 2 * width; j0 += (int64_t)gridDim.x * 32) {
+    const int64_t j = j0 + lane;
+    float s = 0.f;
+    if (j < 2 * width) {
+#pragma unroll 8
+      for (int b = w; b < blocks; b += 8) s += partial[(int64_t)b * 2 * width + j];
+    }
+    part[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && j < 2 * width) {
+#pragma unroll
+      for (int i = 1; i < 8; i++) s += part[i][lane];
+      float* out = j < width ? dgamma : dbeta;
+      if (out) out[j < width ? j : j - width] = s;
+    }
+    __syncthreads();
   }
 }
 
-// One thread a column, rows in order.
-template <typename TD, typename TX>
-__global__ void __launch_bounds__(32) layer_norm_dweights_kernel(const TD* __restrict__ dy, const TX* __restrict__ x,
-                                                                const float* __restrict__ stats,
-                                                                float* __restrict__ dgamma, float* __restrict__ dbeta,
-                                                                int64_t rows, int64_t width) {
-  for (int64_t j = blockIdx.x * 32 + threadIdx.x; j < width; j += gridDim.x * 32) {
-    double sg = 0.0, sb = 0.0;
-    for (int64_t row = 0; row < rows; row++) {
-      const float d = load_f32(dy + row * width + j);
-      sb += d;
-      sg += d * ((load_f32(x + row * width + j) - stats[2 * row]) * stats[2 * row + 1]);
-    }
-    if (dgamma) dgamma[j] = (float)sg;
-    if (dbeta) dbeta[j] = (float)sb;
+// ---- launchers -----------------------------------------------------------------------------------
+struct ForwardArgs {
+  const void* x;
+  const float *gamma, *beta;
+  void* y;
+  float* stats;
+  int64_t rows, width;
+  float epsilon;
+};
+
+unsigned grid_rows(const tfjs_cuda_ctx* ctx, int64_t blocks, int per_sm) {
+  const int64_t cap = (int64_t)ctx->sm_count * per_sm;
+  return (unsigned)(blocks < 1 ? 1 : blocks < cap ? blocks : cap);
+}
+
+template <typename TX, typename TY, int V, int NV, int L>
+void lanes_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+  layer_norm_lanes_kernel<TX, TY, V, NV, L><<<grid_rows(ctx, ceil_div64(a.rows, 256 / L), 8), 256, 0, ctx->stream>>>(
+      (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon);
+}
+template <typename TX, typename TY, int V, int NV, int NT>
+void block_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+  layer_norm_block_kernel<TX, TY, V, NV, NT><<<grid_rows(ctx, a.rows, 8), NT, 0, ctx->stream>>>(
+      (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon);
+}
+
+// A launch of clusters of 8 blocks; `smem` bytes of dynamic shared memory a block.
+template <typename... Params, typename... Args>
+cudaError_t launch_clusters(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), int64_t clusters, size_t smem, Args... args) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
   }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(clusters * kClusterBlocks));
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kClusterBlocks;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
+template <typename TX, typename TY, int V>
+int cluster_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+  const int64_t share = (ceil_div64(a.width / V, kClusterBlocks) * V * (int64_t)sizeof(TX) + 15) / 16 * 16;
+  const bool cached = share <= 200 * 1024;
+  const int64_t cap = (int64_t)ctx->sm_count * 2 / kClusterBlocks;
+  TFJS_CHECK_CUDA(ctx, launch_clusters(ctx, layer_norm_cluster_kernel<TX, TY, V>, a.rows < cap ? a.rows : cap,
+                                       cached ? (size_t)share : 0, (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats,
+                                       a.rows, a.width, a.epsilon, cached ? 1 : 0));
+  return post_launch(ctx, "layerNorm (clusters)");
+}
+
+// V values a load: 16 bytes where every row starts on a 16-byte boundary, else 2 values, else 1.
+template <typename TX, typename TY, int V>
+int forward_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+  const int64_t w = a.width;
+  if (w > 16384) return cluster_form<TX, TY, V>(ctx, a);
+  if (w <= 1024) {
+    if (w <= 4 * V) lanes_form<TX, TY, V, 1, 4>(ctx, a);
+    else if (w <= 16 * V) lanes_form<TX, TY, V, 1, 16>(ctx, a);
+    else if (w <= 64 * V) lanes_form<TX, TY, V, 2, 32>(ctx, a);
+    else if (w <= 128 * V) lanes_form<TX, TY, V, 4, 32>(ctx, a);
+    else if constexpr (V <= 4) {
+      if (w <= 256 * V) lanes_form<TX, TY, V, 8, 32>(ctx, a);
+      else if constexpr (V <= 2) {
+        if (w <= 512 * V) lanes_form<TX, TY, V, 16, 32>(ctx, a);
+        else if constexpr (V == 1) lanes_form<TX, TY, V, 32, 32>(ctx, a);
+      }
+    }
+    return post_launch(ctx, "layerNorm (lanes)");
+  }
+  constexpr int NV = 32 / V;  // 32 values a thread
+  if (w <= 256 * 8) block_form<TX, TY, V, NV / 4, 256>(ctx, a);
+  else if (w <= 256 * 16) block_form<TX, TY, V, NV / 2, 256>(ctx, a);
+  else if (w <= 256 * 32) block_form<TX, TY, V, NV, 256>(ctx, a);
+  else block_form<TX, TY, V, NV, 512>(ctx, a);
+  return post_launch(ctx, "layerNorm (blocks)");
 }
 
 template <typename TX, typename TY>
-void launch_forward(tfjs_cuda_ctx* ctx, const void* x, const float* gamma, const float* beta, void* y, float* stats,
-                    int64_t rows, int64_t width, float epsilon) {
-  const int64_t cap = (int64_t)ctx->sm_count * 8;
-  layer_norm_kernel<TX, TY><<<(unsigned)(rows < cap ? rows : cap), kThreads, 0, ctx->stream>>>(
-      (const TX*)x, gamma, beta, (TY*)y, stats, rows, width, epsilon);
+int launch_forward(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+  constexpr int W = 16 / (int)sizeof(TX);
+  if (a.width % W == 0) return forward_form<TX, TY, W>(ctx, a);
+  if (a.width % 2 == 0) return forward_form<TX, TY, 2>(ctx, a);
+  return forward_form<TX, TY, 1>(ctx, a);
+}
+
+struct BackwardArgs {
+  const void *dy, *x;
+  const float *gamma, *stats;
+  float *dx, *dgamma, *dbeta;
+  int64_t rows, width;
+};
+
+int join(tfjs_cuda_ctx* ctx, const BackwardArgs& a, const float* partial, int blocks) {
+  layer_norm_join_kernel<<<grid_rows(ctx, ceil_div64(2 * a.width, 32), 16), 256, 0, ctx->stream>>>(
+      partial, a.dgamma, a.dbeta, blocks, a.width);
+  return post_launch(ctx, "layerNormBackprop (join)");
+}
+
+template <typename TD, typename TX, int V, int MC, int MINB>
+int staged_launch(tfjs_cuda_ctx* ctx, const BackwardArgs& a, StagedParams& p, int blocks, size_t smem) {
+  auto kernel = layer_norm_staged_kernel<TD, TX, V, MC, MINB>;
+  TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  kernel<<<blocks, kStagedThreads, smem, ctx->stream>>>((const TD*)a.dy, (const TX*)a.x, p);
+  return post_launch(ctx, "layerNormBackprop");
+}
+
+template <typename TD, typename TX, int V>
+int staged_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
+  const int width = (int)a.width, row_bytes = width * (int)(sizeof(TD) + sizeof(TX));
+  // rows a stage: about 24 KB, so that two blocks with three stages each share an SM, but not so many
+  // that the blocks have fewer than four stages each
+  int R = 1;
+  while (R < kMaxStageRows && 2 * R * row_bytes <= 24 * 1024 && ceil_div64(a.rows, 2 * R) >= 8 * ctx->sm_count) R *= 2;
+  StagedParams p = {};
+  p.gamma = a.gamma;
+  p.stats = a.stats;
+  p.dx = a.dx;
+  p.rows = a.rows;
+  p.items = ceil_div64(a.rows, R);
+  p.width = width;
+  p.stage_rows = R;
+  p.x_bytes = (R * width * (int)sizeof(TD) + 31) / 16 * 16;  // one 16-byte unit more for the rows' own offset
+  p.stage_bytes = p.x_bytes + (R * width * (int)sizeof(TX) + 31) / 16 * 16 + (R + 1) / 2 * 16;
+  const int LR = R >= kStagedThreads ? 1 : kStagedThreads / R;
+  size_t smem = (size_t)kStages * p.stage_bytes;
+  const size_t join_bytes = (size_t)2 * kStagedThreads * V * 4;  // the row groups' sums reuse the ring
+  if (smem < join_bytes) {
+    p.stage_bytes = ((int)(join_bytes / kStages) + 16) / 16 * 16;
+    smem = (size_t)kStages * p.stage_bytes;
+  }
+  smem += (size_t)(width + 3) / 4 * 16 + (size_t)R * (LR > 32 ? LR / 32 : 1) * 8;
+  const int per_sm = smem <= 113 * 1024 && width <= 1024 * V ? 2 : 1;
+  const int64_t cap = (int64_t)ctx->sm_count * per_sm;
+  const int blocks = (int)(p.items < cap ? p.items : cap);
+  void* partial = nullptr;
+  size_t partial_cap = 0;
+  int rc;
+  if (a.dgamma || a.dbeta) {
+    if ((rc = ctx_alloc(ctx, (size_t)blocks * 2 * width * 4, &partial, &partial_cap))) return rc;
+    p.partial = (float*)partial;
+  }
+  // columns a thread: width / V / 512, rounded up to 1, 2, 4, 8 or 16 vectors
+  const int mc = (width / V + kStagedThreads - 1) / kStagedThreads;
+  if (mc <= 1) rc = staged_launch<TD, TX, V, 1, 2>(ctx, a, p, blocks, smem);
+  else if (mc <= 2) rc = staged_launch<TD, TX, V, 2, 2>(ctx, a, p, blocks, smem);
+  else if (mc <= 4) rc = staged_launch<TD, TX, V, 4, 1>(ctx, a, p, blocks, smem);
+  else if constexpr (V == 1) rc = staged_launch<TD, TX, V, 16, 1>(ctx, a, p, blocks, smem);
+  if (!rc && partial) rc = join(ctx, a, (const float*)partial, blocks);
+  ctx_free(ctx, partial, partial_cap);
+  return rc;
+}
+
+template <typename TD, typename TX, int V>
+int backward_cluster_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
+  const int64_t cap = (int64_t)ctx->sm_count * 2 / kClusterBlocks, clusters = a.rows < cap ? a.rows : cap;
+  void* partial = nullptr;
+  size_t partial_cap = 0;
+  int rc = TFJS_CUDA_OK;
+  if ((a.dgamma || a.dbeta) && (rc = ctx_alloc(ctx, (size_t)clusters * 2 * a.width * 4, &partial, &partial_cap))) return rc;
+  const cudaError_t e = launch_clusters(ctx, layer_norm_backprop_cluster_kernel<TD, TX, V>, clusters, 0, (const TD*)a.dy,
+                                        (const TX*)a.x, a.gamma, a.stats, a.dx, (float*)partial, a.rows, a.width);
+  if (e != cudaSuccess) rc = set_error(ctx, TFJS_CUDA_ERR_CUDA, "layerNormBackprop failed: %s", cudaGetErrorString(e));
+  if (!rc) rc = post_launch(ctx, "layerNormBackprop (clusters)");
+  if (!rc && partial) rc = join(ctx, a, (const float*)partial, (int)clusters);
+  ctx_free(ctx, partial, partial_cap);
+  return rc;
 }
 
 template <typename TD, typename TX>
-int launch_backward(tfjs_cuda_ctx* ctx, const void* dy, const void* x, const float* gamma, const float* stats, float* dx,
-                    float* dgamma, float* dbeta, int64_t rows, int64_t width) {
-  const int64_t cap = (int64_t)ctx->sm_count * 8;
-  if (dx && rows) {
-    layer_norm_dx_kernel<TD, TX><<<(unsigned)(rows < cap ? rows : cap), kThreads, 0, ctx->stream>>>(
-        (const TD*)dy, (const TX*)x, gamma, stats, dx, rows, width);
-    const int rc = post_launch(ctx, "layerNormBackprop (dx)");
-    if (rc) return rc;
-  }
-  if (dgamma || dbeta) {
-    const int64_t blocks = ceil_div64(width, 32);
-    layer_norm_dweights_kernel<TD, TX><<<(unsigned)(blocks < 65535 ? blocks : 65535), 32, 0, ctx->stream>>>(
-        (const TD*)dy, (const TX*)x, stats, dgamma, dbeta, rows, width);
-    return post_launch(ctx, "layerNormBackprop (weights)");
-  }
-  return TFJS_CUDA_OK;
+int launch_backward(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
+  if (a.width <= kStagedWidth) return a.width % 4 == 0 ? staged_form<TD, TX, 4>(ctx, a) : staged_form<TD, TX, 1>(ctx, a);
+  return a.width % 4 == 0 ? backward_cluster_form<TD, TX, 4>(ctx, a) : backward_cluster_form<TD, TX, 1>(ctx, a);
 }
 
 // A float32 operand of exactly `elems` values, not quantised; null for id 0.
@@ -183,8 +738,7 @@ extern "C" int tfjs_cuda_layer_norm(tfjs_cuda_ctx* ctx, tfjs_tensor_id x_id, tfj
   const bool hx = x->dtype == TFJS_F16, hy = y->dtype == TFJS_F16;
   auto launch = hx ? (hy ? launch_forward<__half, __half> : launch_forward<__half, float>)
                    : (hy ? launch_forward<float, __half> : launch_forward<float, float>);
-  launch(ctx, x->ptr, f32_ptr(gamma), f32_ptr(beta), y->ptr, f32_out(stats), rows, width, epsilon);
-  return post_launch(ctx, "layerNorm");
+  return launch(ctx, {x->ptr, f32_ptr(gamma), f32_ptr(beta), y->ptr, f32_out(stats), rows, width, epsilon});
 }
 
 extern "C" int tfjs_cuda_layer_norm_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id dy_id, tfjs_tensor_id x_id,
@@ -211,9 +765,15 @@ extern "C" int tfjs_cuda_layer_norm_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id 
   }
   if (width == 0) return TFJS_CUDA_OK;
   cudaSetDevice(ctx->device);
+  if (rows == 0) {  // the sum of no rows
+    for (int i = 1; i < 3; i++)
+      if (out[i]) TFJS_CHECK_CUDA(ctx, cudaMemsetAsync(out[i]->ptr, 0, (size_t)width * 4, ctx->stream));
+    return TFJS_CUDA_OK;
+  }
+  if (!out[0] && !out[1] && !out[2]) return TFJS_CUDA_OK;
   const bool hd = dy->dtype == TFJS_F16, hx = x->dtype == TFJS_F16;
   auto launch = hd ? (hx ? launch_backward<__half, __half> : launch_backward<__half, float>)
                    : (hx ? launch_backward<float, __half> : launch_backward<float, float>);
-  return launch(ctx, dy->ptr, x->ptr, f32_ptr(gamma), f32_ptr(stats), f32_out(out[0]), f32_out(out[1]), f32_out(out[2]),
-                rows, width);
+  return launch(ctx, {dy->ptr, x->ptr, f32_ptr(gamma), f32_ptr(stats), f32_out(out[0]), f32_out(out[1]), f32_out(out[2]),
+                      rows, width});
 }
