@@ -142,5 +142,9 @@ def load():
     return _lib
 
 
+_SHAPE = [C.c_int64 * max(rank, 1) for rank in range(9)]   # the library takes ranks up to 8
+
+
 def shape_array(shape):
-    return (C.c_int64 * max(len(shape), 1))(*[int(s) for s in shape])
+    rank = len(shape)
+    return (_SHAPE[rank] if rank < 9 else C.c_int64 * rank)(*map(int, shape))

@@ -14,7 +14,6 @@ methods, which is what unmodified tf.* code reaches.
 """
 import ctypes as C
 import time as _time
-import weakref
 
 import numpy as np
 
@@ -78,7 +77,12 @@ class BackendCuda:
             raise CudaError(f"cuda backend initialisation failed ({rc}): {msg}")
         self._ctx = ctx
         self.device = int(device)
-        self._data = weakref.WeakKeyDictionary()  # DataStorage (backend.ts:47-70): dataId -> record
+        # DataStorage (backend.ts:47-70): dataId -> record; the engine disposes every dataId it registers
+        self._data = {}
+        # out-parameters of the calls that every operator makes (one host thread a context)
+        self._out_id, self._out_ptr = C.c_int64(), C.c_void_p()
+        self._out_id_ref, self._out_ptr_ref = C.byref(self._out_id), C.byref(self._out_ptr)
+        self._stream = self._lib.tfjs_cuda_ctx_stream(ctx)
         self.activation_storage = "float32"
         self._pending_storage = None
         self.setMathMode(math_mode)
@@ -111,10 +115,11 @@ class BackendCuda:
         return tmp, tmp
 
     def _new_id(self, shape, dtype):
-        out = C.c_int64()
-        self._check(self._lib.tfjs_cuda_tensor_register(self._ctx, C.byref(out), len(shape),
-                                                        _ffi.shape_array(shape), _DTYPE_CODE[dtype]))
-        return out.value
+        rc = self._lib.tfjs_cuda_tensor_register(self._ctx, self._out_id_ref, len(shape), _ffi.shape_array(shape),
+                                                 _DTYPE_CODE[dtype])
+        if rc != 0:
+            self._check(rc)
+        return self._out_id.value
 
     def _free_tmp(self, *ids):
         for i in ids:
@@ -156,8 +161,7 @@ class BackendCuda:
         storage = dtype
         if self._pending_storage == "float16" and dtype == "float32":
             storage = "float16"   # a float32 tensor stored as IEEE half (16-bit activation storage)
-        self._data[dataId] = {"id": self._new_id(shape, storage), "dtype": storage,
-                              "shape": list(shape)}
+        self._data[dataId] = {"id": self._new_id(shape, storage), "dtype": storage, "shape": list(shape)}
 
     def write(self, dataId, values):
         if values is None:
@@ -232,7 +236,7 @@ class BackendCuda:
         if self._ctx:
             self._lib.tfjs_cuda_ctx_destroy(self._ctx)
             self._ctx = None
-            self._data = weakref.WeakKeyDictionary()
+            self._data = {}
 
     def fromPixels(self, pixels, numChannels):
         raise NotImplementedError("Not yet implemented.")
@@ -328,11 +332,10 @@ class BackendCuda:
         convolution's weights before, whose repacked form is kept."""
         t._throw_if_disposed()
         rec = self._rec(t.dataId)
-        ptr = C.c_void_p()
-        self._check(self._lib.tfjs_cuda_tensor_device_ptr(self._ctx, rec["id"], C.byref(ptr), None))
-        typestr = "|u1" if rec.get("quantized") else _TYPESTR[rec["dtype"]]
-        return DeviceArray({"shape": tuple(t.shape), "typestr": typestr, "data": (ptr.value or 0, False),
-                            "version": 3, "stream": self.stream()})
+        self._check(self._lib.tfjs_cuda_tensor_device_ptr(self._ctx, rec["id"], self._out_ptr_ref, None))
+        typestr = "|u1" if "quantized" in rec else _TYPESTR[rec["dtype"]]
+        return DeviceArray({"shape": tuple(t.shape), "typestr": typestr, "data": (self._out_ptr.value or 0, False),
+                            "version": 3, "stream": self._stream})
 
     # ---- fused epilogue marshalling ------------------------------------------------------
     @staticmethod
@@ -678,7 +681,9 @@ class BackendCuda:
     # ---- normalisation, lookup and loss of token and feature models (extensions) -----------
     def _enqueue(self, rc, outputs, temporaries):
         """Ends a kernel method: frees the converted operands and, if the call failed, its outputs."""
-        self._free_tmp(*temporaries)
+        for i in temporaries:
+            if i is not None:
+                self._lib.tfjs_cuda_tensor_dispose(self._ctx, i)
         if rc != 0:
             for t in outputs:
                 if t is not None:

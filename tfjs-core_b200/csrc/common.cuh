@@ -177,6 +177,23 @@ inline void launch_ex(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), dim3 grid, 
   cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// The same, always with the attribute: for a second kernel of one operator, whose blocks may be placed
+// while the first kernel (which calls pdl_launch_dependents()) runs out.  The kernel must call pdl_wait()
+// before touching global memory.
+template <typename... Params, typename... Args>
+inline void launch_dependent(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), dim3 grid, dim3 block, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = ctx->stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+}
+
 // Allocator (context.cu).
 int ctx_alloc(tfjs_cuda_ctx* ctx, size_t nbytes, void** ptr, size_t* capacity);
 void ctx_free(tfjs_cuda_ctx* ctx, void* ptr, size_t capacity);

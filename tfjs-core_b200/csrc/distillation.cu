@@ -27,9 +27,10 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kMaxTop = 1024;
-constexpr int kThreads = 512;      // of a block of the loss
+constexpr int kThreads = 256;      // of a block of the loss
 constexpr int kGradThreads = 256;  // of a block of the gradient
-constexpr int kBatch = 4;          // 16-byte loads in flight a thread
+constexpr int kBatch = 4;          // 16-byte loads in flight a thread of the loss
+constexpr int kGradBatch = 4;      // and of the gradient
 constexpr float kLn2 = 0.693147180559945f;
 constexpr float kLog2e = 1.44269504088896f;
 
@@ -42,29 +43,122 @@ __device__ __forceinline__ float exp2_approx(float v) {
 __device__ __forceinline__ float load_one(const float* p) { return *p; }
 __device__ __forceinline__ float load_one(const __half* p) { return __half2float(*p); }
 
-// Sum and NaN-keeping maximum over G threads: a warp, or the whole block.  `scratch`: G / 32 floats.
-template <int G>
-__device__ __forceinline__ float group_max(float v, float* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (G > 32) {
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[threadIdx.x & (G / 32 - 1)];
-#pragma unroll
-    for (int o = G / 64; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
-  }
-  return v;
+// Two float32 values in one register pair, for the packed instructions (one issue slot for two values).
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
-template <int G>
-__device__ __forceinline__ float group_sum(float v, float* scratch) {
-  v = lanes_sum<32>(v);
-  if (G > 32) {
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = lanes_sum<G / 32>(scratch[threadIdx.x & (G / 32 - 1)]);
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 16 bytes of logits as they are stored: P pairs.
+template <typename T>
+struct Unit {
+  static constexpr int P = 8 / (int)sizeof(T);
+  uint4 q;
+  __device__ void load(const T* p) { q = *reinterpret_cast<const uint4*>(p); }
+  __device__ void fill_low() {  // -inf
+    const uint32_t w = sizeof(T) == 4 ? 0xff800000u : 0xfc00fc00u;
+    q = make_uint4(w, w, w, w);
   }
-  return v;
+  __device__ float2 get(int i) const {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+  }
+};
+// Four of them.
+template <typename T>
+struct alignas(4 * sizeof(T)) Raw4 {
+  T v[4];
+  __device__ float2 get(int i) const { return make_float2(load_one(&v[2 * i]), load_one(&v[2 * i + 1])); }
+};
+// Largest value of N units, NaN if there is one (halves are compared two at a time, as halves).
+template <int N>
+__device__ __forceinline__ float units_max(const Unit<float> (&u)[N]) {
+  float m = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < N; i++)
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const float2 f = u[i].get(j);
+      m = max_nan(m, max_nan(f.x, f.y));
+    }
+  return m;
+}
+template <int N>
+__device__ __forceinline__ float units_max(const Unit<__half> (&u)[N]) {
+  uint32_t low = 0xfc00fc00u;
+  __half2 m = *reinterpret_cast<__half2*>(&low);
+#pragma unroll
+  for (int i = 0; i < N; i++) {
+    const uint32_t w[4] = {u[i].q.x, u[i].q.y, u[i].q.z, u[i].q.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) m = __hmax2_nan(m, *reinterpret_cast<const __half2*>(&w[j]));
+  }
+  const float2 f = __half22float2(m);
+  return max_nan(f.x, f.y);
+}
+
+// The exponent (z - m) k - l of a value z is taken as fma(z, k, shift), shift = -(m k + l): one packed
+// instruction for two values.  What the rounding of `shift` loses is the same for all of them, so it
+// goes into a factor for the whole: 2^((z - m) k - l) = 2^fma(z, k, shift) * factor.  Where m k is too
+// large for that (a row of the type's lowest values), `exact` is set and the difference comes first.
+struct Shift {
+  float shift, factor;
+  bool exact;
+  __device__ Shift(float m, float k, float l) {
+    const float hi = m * k, lo = fmaf(m, k, -hi);
+    const float sum = hi + l, back = sum - hi;
+    const float lost = (hi - (sum - back)) + (l - back) + lo;
+    shift = -sum;
+    factor = 1.f - lost * kLn2;  // |lost| < 2^-20 |shift|: 2^-lost to float32's precision
+    exact = !(fabsf(sum) < 1e4f);
+  }
+};
+
+// NaN-keeping maximum, or sum, of two values over G threads: a warp, or the whole block of G (`scratch`:
+// G / 32 pairs that no other call uses).
+template <int G, bool MAX>
+__device__ __forceinline__ float2 group_reduce(float a, float b, float2* scratch) {
+  auto join = [](float p, float q) { return MAX ? max_nan(p, q) : p + q; };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
+    b = join(b, __shfl_xor_sync(0xffffffffu, b, o));
+  }
+  if (G > 32) {
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(a, b);
+    __syncthreads();
+    const float2 v = scratch[threadIdx.x & (G / 32 - 1)];
+    a = v.x;
+    b = v.y;
+#pragma unroll
+    for (int o = G / 64; o > 0; o >>= 1) {
+      a = join(a, __shfl_xor_sync(0xffffffffu, a, o));
+      b = join(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+  }
+  return make_float2(a, b);
 }
 
 // Where a row's 16-byte units lie: `head` elements before them, `vecs` units, `tail` elements behind.
@@ -91,7 +185,7 @@ __global__ void __launch_bounds__(G > 32 ? kThreads : 256) distillation_kernel(
     const TZ* __restrict__ z, const TU* __restrict__ u, const int32_t* __restrict__ indices, float* __restrict__ loss,
     float* __restrict__ stats, int64_t rows, int classes, int top, float temperature, int C) {
   constexpr int V = 16 / (int)sizeof(TZ);
-  __shared__ float scratch[5][32];
+  __shared__ float2 scratch[3][kThreads / 32];
   __shared__ float2 slot;
   const int t = threadIdx.x & (G - 1);
   const int rank = G > 32 ? (int)(blockIdx.x % C) : 0;
@@ -129,68 +223,82 @@ __global__ void __launch_bounds__(G > 32 ? kThreads : 256) distillation_kernel(
   {
     const TZ* body = zr + split.head;
     const int lo = (int)((int64_t)split.vecs * rank / C), hi = (int)((int64_t)split.vecs * (rank + 1) / C);
+    const uint64_t kk = pair(k2, k2);
     for (int j = lo + t; j < hi; j += G * kBatch) {
-      float v[kBatch][V];
+      Unit<TZ> q[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; i++) {
-        if (j + i * G < hi) {
-          load_vec<V>(body + (int64_t)(j + i * G) * V, v[i]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < V; k++) v[i][k] = -INFINITY;
-        }
+        if (j + i * G < hi) q[i].load(body + (int64_t)(j + i * G) * V);
+        else q[i].fill_low();
       }
-      float b = m;
-#pragma unroll
-      for (int i = 0; i < kBatch; i++)
-#pragma unroll
-        for (int k = 0; k < V; k++) b = max_nan(b, v[i][k]);
+      const float b = max_nan(m, units_max(q));
       const float at = b == -INFINITY ? 0.f : b;
+      const Shift sh(at, k2, 0.f);
       s *= exp2_approx((m - at) * k2);  // m = -inf: 0 * s = 0
+      if (!sh.exact) {
+        const uint64_t shift2 = pair(sh.shift, sh.shift);
+        uint64_t sum = 0;
 #pragma unroll
-      for (int i = 0; i < kBatch; i++)
+        for (int i = 0; i < kBatch; i++)
 #pragma unroll
-        for (int k = 0; k < V; k++) s += exp2_approx((v[i][k] - at) * k2);
+          for (int k = 0; k < Unit<TZ>::P; k++) {
+            const float2 f = q[i].get(k), e = unpair(fma_pair(pair(f.x, f.y), kk, shift2));
+            sum = add_pair(sum, pair(exp2_approx(e.x), exp2_approx(e.y)));
+          }
+        const float2 f = unpair(sum);
+        s = fmaf(f.x + f.y, sh.factor, s);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kBatch; i++)
+#pragma unroll
+          for (int k = 0; k < Unit<TZ>::P; k++) {
+            const float2 f = q[i].get(k);
+            s += exp2_approx((f.x - at) * k2) + exp2_approx((f.y - at) * k2);
+          }
+      }
       m = b;
     }
   }
-  float all = group_max<G>(m, scratch[0]);
-  s = group_sum<G>(s * shifted(m, all, k2), scratch[1]);
+  float um = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < NK; i++) um = max_nan(um, tu[i]);
+  const float2 big = group_reduce<G, true>(m, um, scratch[0]);
+  float all = big.x;
+  um = big.y;
+  const float ut = um == -INFINITY ? 0.f : um;
+  float e = 0.f;
+#pragma unroll
+  for (int i = 0; i < NK; i++) e += exp2_approx((tu[i] - ut) * k2);
+  const float2 sums = group_reduce<G, false>(s * shifted(m, all, k2), e, scratch[1]);
+  s = sums.x;
   if (G > 32 && C > 1) {
     cg::cluster_group cluster = cg::this_cluster();
     if (threadIdx.x == 0) slot = make_float2(all, s);
     cluster.sync();
     if (rank == 0) {
-      float big = -INFINITY, sum = 0.f;
-      for (int i = 0; i < C; i++) big = max_nan(big, cluster.map_shared_rank(&slot, i)->x);
+      float most = -INFINITY, sum = 0.f;
+      for (int i = 0; i < C; i++) most = max_nan(most, cluster.map_shared_rank(&slot, i)->x);
       for (int i = 0; i < C; i++) {
         const float2 o = *cluster.map_shared_rank(&slot, i);
-        sum += o.y * shifted(o.x, big, k2);
+        sum += o.y * shifted(o.x, most, k2);
       }
-      all = big;
+      all = most;
       s = sum;
     }
     cluster.sync();  // the other blocks' slots have been read
     if (rank != 0) return;
   }
-  // ---- the teacher's list, and the loss
-  float um = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NK; i++) um = max_nan(um, tu[i]);
-  um = group_max<G>(um, scratch[2]);
+  // ---- the loss
   const float ls = log2f(s);
   float uls = 0.f, l = 0.f;
   if (um != -INFINITY) {  // the same for all threads of the row
-    float e = 0.f;
-#pragma unroll
-    for (int i = 0; i < NK; i++) e += exp2_approx((tu[i] - um) * k2);
-    uls = log2f(group_sum<G>(e, scratch[3]));
+    uls = log2f(sums.y);
 #pragma unroll
     for (int i = 0; i < NK; i++) {
       const float lp = (tu[i] - um) * k2 - uls, p = exp2_approx(lp);
       if (p != 0.f) l += p * (lp - ((tz[i] - all) * k2 - ls));
     }
-    l = group_sum<G>(l, scratch[4]) * kLn2;
+    l = group_reduce<G, false>(l, 0.f, scratch[2]).x * kLn2;
   }
   if (t == 0) {
     loss[row] = temperature * temperature * l;
@@ -204,7 +312,7 @@ __device__ __forceinline__ void group_sync() {
   else __syncwarp();
 }
 
-// G threads take a tile of G * kBatch units of a row (the first tile also the loose elements): all
+// G threads take a tile of G * kGradBatch units of a row (the first tile also the loose elements): all
 // classes get c q_v, then the tile's listed classes are written again with their p taken off, by the
 // first entry that names the class.  `room`: entries of shared memory a group.
 template <typename TZ, typename TU, int G>
@@ -212,7 +320,7 @@ __global__ void __launch_bounds__(kGradThreads) distillation_backprop_kernel(
     const float* __restrict__ dloss, const TZ* __restrict__ z, const TU* __restrict__ u,
     const int32_t* __restrict__ indices, const float* __restrict__ stats, float* __restrict__ dz, int64_t rows,
     int classes, int top, float temperature, int tiles, int room) {
-  constexpr int V = 16 / (int)sizeof(TZ);
+  constexpr int V = 4;  // values a unit: their float32 gradient is one 16-byte store, side by side over the lanes
   extern __shared__ __align__(16) uint8_t smem[];
   const int t = threadIdx.x & (G - 1), group = threadIdx.x / G;
   const int64_t item = (int64_t)blockIdx.x * (kGradThreads / G) + group;
@@ -226,33 +334,47 @@ __global__ void __launch_bounds__(kGradThreads) distillation_backprop_kernel(
   const TZ* zr = z + first;
   float* dr = dz + first;
   const RowSplit<V> split(first, classes);
-  const int v0 = tile * G * kBatch;
+  const int v0 = tile * G * kGradBatch;
 
-  float v[kBatch][V];
+  Raw4<TZ> q[kGradBatch];
 #pragma unroll
-  for (int i = 0; i < kBatch; i++)
-    if (v0 + i * G + t < split.vecs) load_vec<V>(zr + split.head + (int64_t)(v0 + i * G + t) * V, v[i]);
+  for (int i = 0; i < kGradBatch; i++)
+    if (v0 + i * G + t < split.vecs) q[i] = *reinterpret_cast<const Raw4<TZ>*>(zr + split.head + (int64_t)(v0 + i * G + t) * V);
   const float4 st = *reinterpret_cast<const float4*>(stats + 4 * row);
   const float c = dloss[row] * temperature;
   const bool empty = st.z == -INFINITY;
   for (int e = t; e < room; e += G) {
     int32_t at = -1;
     float p = 0.f;
-    if (e < top && !empty) {
+    if (e < top) {
       at = indices[row * top + e];
-      if (at >= 0 && at < classes) p = exp2_approx((load_one(u + row * top + e) - st.z) * k2 - st.w);
-      else at = -1;
+      p = exp2_approx((load_one(u + row * top + e) - st.z) * k2 - st.w);
+      if (at < 0 || at >= classes) at = -1;
     }
     s_i[e] = at;
     s_p[e] = p;
   }
+  const Shift sh(st.x, k2, st.y);
+  const uint64_t kk = pair(k2, k2), shift2 = pair(sh.shift, sh.shift);
+  const uint64_t c2 = pair(c * sh.factor, c * sh.factor);
 #pragma unroll
-  for (int i = 0; i < kBatch; i++) {
-    if (v0 + i * G + t < split.vecs) {
+  for (int i = 0; i < kGradBatch; i++) {
+    if (v0 + i * G + t >= split.vecs) continue;
+    float o[V];
 #pragma unroll
-      for (int k = 0; k < V; k++) v[i][k] = empty ? 0.f : c * exp2_approx((v[i][k] - st.x) * k2 - st.y);
-      store_vec<V>(dr + split.head + (int64_t)(v0 + i * G + t) * V, v[i]);
+    for (int h = 0; h < 2; h++) {
+      const float2 f = q[i].get(h);
+      float2 e;
+      if (!sh.exact) {
+        e = unpair(fma_pair(pair(f.x, f.y), kk, shift2));
+        e = unpair(mul_pair(pair(exp2_approx(e.x), exp2_approx(e.y)), c2));
+      } else {
+        e = make_float2(c * exp2_approx((f.x - st.x) * k2 - st.y), c * exp2_approx((f.y - st.x) * k2 - st.y));
+      }
+      o[2 * h] = empty ? 0.f : e.x;
+      o[2 * h + 1] = empty ? 0.f : e.y;
     }
+    store_vec<V>(dr + split.head + (int64_t)(v0 + i * G + t) * V, o);
   }
   if (tile == 0 && t < split.head + split.tail) {
     const int at = split.loose(t);
@@ -260,7 +382,7 @@ __global__ void __launch_bounds__(kGradThreads) distillation_backprop_kernel(
   }
   if (empty) return;  // the whole group
   group_sync<G>();    // the list is there, and the classes are written before they are written again
-  const int lo = split.head + v0 * V, hi = split.head + min(v0 + G * kBatch, split.vecs) * V;
+  const int lo = split.head + v0 * V, hi = split.head + min(v0 + G * kGradBatch, split.vecs) * V;
   for (int e = t; e < top; e += G) {
     const int32_t at = s_i[e];
     if (at < 0) continue;
@@ -333,7 +455,7 @@ int launch_forward(tfjs_cuda_ctx* ctx, const Operands& o, float* loss, float* st
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  TFJS_CHECK_CUDA(ctx, cudaLaunchKernelEx(&cfg, distillation_kernel<TZ, TU, kThreads, 2>, z, u, indices, loss, stats, rows,
+  TFJS_CHECK_CUDA(ctx, cudaLaunchKernelEx(&cfg, distillation_kernel<TZ, TU, kThreads, kMaxTop / kThreads>, z, u, indices, loss, stats, rows,
                                           (int)classes, top, temperature, C));
   return post_launch(ctx, "distillationLoss");
 }
@@ -341,10 +463,10 @@ int launch_forward(tfjs_cuda_ctx* ctx, const Operands& o, float* loss, float* st
 template <typename TZ, typename TU>
 int launch_backward(tfjs_cuda_ctx* ctx, const float* dloss, const Operands& o, const float* stats, float* dz,
                     int64_t rows, int64_t classes, int top, float temperature) {
-  constexpr int V = 16 / (int)sizeof(TZ);
-  const bool warps = classes <= 32 * kBatch * V * 2 && top <= 128;
+  constexpr int V = 4;
+  const bool warps = classes <= 32 * kGradBatch * V && top <= 128;
   const int G = warps ? 32 : kGradThreads, groups = kGradThreads / G;
-  const int64_t tiles = classes <= G * kBatch * V ? 1 : ceil_div64(classes, (int64_t)G * kBatch * V);
+  const int64_t tiles = classes <= G * kGradBatch * V ? 1 : ceil_div64(classes, (int64_t)G * kGradBatch * V);
   const int64_t blocks = ceil_div64(rows * tiles, groups);
   TFJS_REQUIRE(ctx, blocks < (1ll << 31), "distillationLossBackprop: too many rows times classes");
   const int room = (top + 3) / 4 * 4;

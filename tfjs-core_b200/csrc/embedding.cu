@@ -14,50 +14,52 @@ namespace {
 constexpr int kThreads = 256;
 
 // ---- lookup ----------------------------------------------------------------------------------------
+// V values of a table row as they are stored.
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Raw {
+  T v[V];
+};
 // A quantised table's value is the float32 that decodeWeights gives (io_utils.ts:139): a float64
 // product and sum, rounded once.
 struct Decode {
   double scale, min;
 };
-template <int V>
-__device__ __forceinline__ void load_row(const uint8_t* p, Decode q, float (&v)[V]) {
-  uint32_t word = 0;
-  if constexpr (V == 4) word = *reinterpret_cast<const uint32_t*>(p);
-  else word = *p;
-#pragma unroll
-  for (int i = 0; i < V; i++)
-    v[i] = (float)__dadd_rn(__dmul_rn((double)((word >> (8 * i)) & 255u), q.scale), q.min);
-}
-template <int V, typename T>
-__device__ __forceinline__ void load_row(const T* p, Decode, float (&v)[V]) {
-  load_vec<V>(p, v);
-}
+__device__ __forceinline__ float widen(float v, Decode) { return v; }
+__device__ __forceinline__ float widen(__half v, Decode) { return __half2float(v); }
+__device__ __forceinline__ float widen(uint8_t v, Decode q) { return (float)__dadd_rn(__dmul_rn((double)v, q.scale), q.min); }
 
-// L lanes a token, V columns a lane and step.
-template <typename TT, typename TO, int V, int L>
+// L lanes a token; blockIdx.y takes U * L * V columns.  Bound by the bytes written; the U loads of a lane
+// are issued before its first store, and a block ends with its tokens (blocks that go on to further ones
+// measured 8 % slower: 32768 x 1024 from bytes 28.9 us, this form 26.7; a decoded-value table in shared
+// memory instead of the float64 arithmetic changes nothing).  `stream`: the result exceeds L2 by far, so
+// its lines may leave first (24.7 us).
+template <typename TT, typename TO, int V, int L, int U>
 __global__ void __launch_bounds__(kThreads) embedding_kernel(const TT* __restrict__ table,
                                                             const int32_t* __restrict__ indices, TO* __restrict__ out,
                                                             int64_t tokens, int64_t vocab, int width, float scale,
-                                                            Decode q) {
+                                                            Decode q, bool stream) {
   const int lane = threadIdx.x & (L - 1), vecs = width / V;
-  const int64_t step = (int64_t)gridDim.x * (kThreads / L);
-  for (int64_t t = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L; t < tokens; t += step) {
-    const int64_t v = indices[t];
-    const bool there = v >= 0 && v < vocab;
-    const TT* row = table + (there ? v : 0) * width;
-    TO* o = out + t * width;
-#pragma unroll 4
-    for (int j = lane; j < vecs; j += L) {
-      float r[V];
-      if (there) {
-        load_row<V>(row + j * V, q, r);
+  const int64_t t = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L;
+  if (t >= tokens) return;
+  const int32_t v = indices[t];
+  const bool there = v >= 0 && v < vocab;
+  const Raw<TT, V>* row = reinterpret_cast<const Raw<TT, V>*>(table + (int64_t)(there ? v : 0) * width);
+  for (int j = blockIdx.y * U * L + lane; j < vecs; j += gridDim.y * U * L) {
+    Raw<TT, V> r[U];
+    if (there) {
 #pragma unroll
-        for (int i = 0; i < V; i++) r[i] *= scale;
-      } else {
+      for (int i = 0; i < U; i++)
+        if (j + i * L < vecs) r[i] = row[j + i * L];
+    }
 #pragma unroll
-        for (int i = 0; i < V; i++) r[i] = 0.f;
-      }
-      store_vec<V>(o + j * V, r);
+    for (int i = 0; i < U; i++) {
+      if (j + i * L >= vecs) break;
+      float f[V];
+#pragma unroll
+      for (int k = 0; k < V; k++) f[k] = there ? widen(r[i].v[k], q) * scale : 0.f;
+      TO* o = out + t * width + (int64_t)(j + i * L) * V;
+      if (stream) store_vec_stream<V>(o, f);
+      else store_vec<V>(o, f);
     }
   }
 }
@@ -65,7 +67,7 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const TT* __restric
 // ---- gradient: tokens sorted by table row --------------------------------------------------------------
 // Stable least-significant-digit radix sort of (table row, token) pairs; a token outside the table
 // gets the key `vocab`, behind all others.  Within a block each warp owns a run of keys: it counts
-// their digits into its own counters (the lanes of equal digits agree through match_any, one of them
+// their digits into its own counters (the lanes of equal digits find each other by votes, one of them
 // adds), the counters are summed over the warps and blocks, and the same walk then gives each key its
 // place.  No atomics: equal inputs give the same order, ascending tokens within each table row.
 constexpr int kSortThreads = 1024, kSortWarps = 32;
@@ -82,39 +84,52 @@ Digits digits_of(int64_t vocab) {
   return {passes, (total + passes - 1) / passes};
 }
 
-// One walk over the block's keys.  PLACE false: counts[warp][digit]; true: place(key, token, place within
-// the block's own keys of that digit), from the exclusive prefix over the warps that counts then holds.
-template <bool PLACE, typename F>
-__device__ __forceinline__ void walk_keys(const uint32_t* keys, const uint32_t* tokens, int n, int per_warp, int shift,
-                                          int bins, uint16_t* counts, F place) {
+// Each thread's keys (at most 8): their digits, and their places among the keys of that digit that the
+// warp owns; counts[warp][digit] is the number of them.  A place beyond the block's n keys has digit ~0.
+constexpr int kKeysPerThread = kSortKeys / kSortThreads;
+__device__ __forceinline__ void rank_keys(const uint32_t* keys, int n, int per_warp, int shift, int bins, uint16_t* counts,
+                                          uint32_t (&digit)[kKeysPerThread], uint32_t (&place)[kKeysPerThread]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint16_t* mine = counts + warp * bins;
-  for (int i = 0; i < per_warp; i += 32) {
-    const int at = warp * per_warp + i + lane;
-    const bool there = at < n;
-    if (!__any_sync(0xffffffffu, there)) break;
-    const uint32_t key = there ? keys[at] : 0;
-    const uint32_t digit = there ? (key >> shift) & (uint32_t)(bins - 1) : 0xffffffffu;
-    const uint32_t peers = __match_any_sync(0xffffffffu, digit);
+#pragma unroll
+  for (int i = 0; i < kKeysPerThread; i++) {
+    digit[i] = ~0u;
+    place[i] = 0;
+    const int at = warp * per_warp + i * 32 + lane;
+    const bool there = i * 32 < per_warp && at < n;
+    if (!__any_sync(0xffffffffu, there)) continue;
+    if (there) digit[i] = (keys[at] >> shift) & (uint32_t)(bins - 1);
+    // the lanes of the same digit, by a vote on each of its bits (match.any took twice as long: a sort of
+    // 65536 keys 37 us with it)
+    uint32_t peers = __ballot_sync(0xffffffffu, there);
+    for (int bit = 0; (bins >> bit) > 1; bit++) {
+      const bool set = digit[i] >> bit & 1;
+      const uint32_t votes = __ballot_sync(0xffffffffu, set);
+      peers &= set ? votes : ~votes;
+    }
     const int before = __popc(peers & ((1u << lane) - 1));
     uint32_t base = 0;
-    if (there) base = mine[digit];
+    if (there) base = mine[digit[i]];
     __syncwarp();
-    if (there && before == 0) mine[digit] = (uint16_t)(base + __popc(peers));
+    if (there && before == 0) mine[digit[i]] = (uint16_t)(base + __popc(peers));
     __syncwarp();
-    if (PLACE && there) place(key, tokens[at], digit, base + before);
+    place[i] = base + before;
   }
 }
 
 // counts[warp][digit] -> exclusive prefix over the warps; returns the block's total of digit threadIdx.x.
 __device__ __forceinline__ uint32_t prefix_over_warps(uint16_t* counts, int bins) {
   uint32_t sum = 0;
-  if ((int)threadIdx.x < bins)
+  if ((int)threadIdx.x < bins) {
+    uint32_t c[kSortWarps];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; w++) c[w] = counts[w * bins + threadIdx.x];
+#pragma unroll
     for (int w = 0; w < kSortWarps; w++) {
-      const uint32_t c = counts[w * bins + threadIdx.x];
       counts[w * bins + threadIdx.x] = (uint16_t)sum;
-      sum += c;
+      sum += c[w];
     }
+  }
   return sum;
 }
 
@@ -151,6 +166,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(
     uint32_t* __restrict__ sorted_tokens, float* __restrict__ dtable, int64_t values) {
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks();
+  pdl_launch_dependents();  // the sums wait for this kernel's end before they read
   if ((int)blockIdx.x >= blocks) {
     const int64_t stride = (int64_t)(gridDim.x - blocks) * kSortThreads;
     const int64_t first = (int64_t)(blockIdx.x - blocks) * kSortThreads + threadIdx.x;
@@ -170,41 +186,52 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(
     s.keys[0][i] = (uint32_t)v < vocab ? (uint32_t)v : vocab;
     s.tokens[0][i] = (uint32_t)(rank * share + i);
   }
+  const int per_warp = share / kSortWarps, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int pass = 0; pass < passes; pass++) {
     const int from = pass & 1, shift = pass * bits;
     for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(s.counts)[i] = 0;
     __syncthreads();
-    walk_keys<false>(s.keys[from], s.tokens[from], n, share / kSortWarps, shift, bins, s.counts,
-                     [](uint32_t, uint32_t, uint32_t, uint32_t) {});
+    uint32_t digit[kKeysPerThread], place[kKeysPerThread];
+    rank_keys(s.keys[from], n, per_warp, shift, bins, s.counts, digit, place);
     __syncthreads();
     const uint32_t total = prefix_over_warps(s.counts, bins);
     if ((int)threadIdx.x < bins) s.totals[threadIdx.x] = total;
     cluster.sync();
     uint32_t all = 0, before = 0;
-    if ((int)threadIdx.x < bins)
-      for (int r = 0; r < blocks; r++) {
-        const uint32_t c = cluster.map_shared_rank(s.totals, r)[threadIdx.x];
+    if ((int)threadIdx.x < bins) {
+#pragma unroll
+      for (int r = 0; r < 8; r++) {
+        const uint32_t c = r < blocks ? cluster.map_shared_rank(s.totals, r)[threadIdx.x] : 0;
         all += c;
         if (r < rank) before += c;
       }
+    }
+    const bool last = pass + 1 == passes;
+    // The last pass writes to global memory only: its barrier, which keeps the blocks until their totals
+    // have been read, is entered here, so that it does not wait for those writes (they queue behind the
+    // other blocks' zeros).
+    if (last) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const uint32_t smaller = block_exclusive(all, s.warps);
     if ((int)threadIdx.x < bins) s.base[threadIdx.x] = smaller + before;
     __syncthreads();
-    const bool last = pass + 1 == passes;
-    walk_keys<true>(s.keys[from], s.tokens[from], n, share / kSortWarps, shift, bins, s.counts,
-                    [&](uint32_t key, uint32_t token, uint32_t digit, uint32_t place) {
-                      const int g = (int)(s.base[digit] + place);
-                      if (last) {
-                        sorted_keys[g] = key;
-                        sorted_tokens[g] = token;
-                      } else {
-                        const int to = g / share, slot = g - to * share;
-                        cluster.map_shared_rank(s.keys[from ^ 1], to)[slot] = key;
-                        cluster.map_shared_rank(s.tokens[from ^ 1], to)[slot] = token;
-                      }
-                    });
-    cluster.sync();  // the pass's writes have arrived; nobody reads this block's totals any more
+#pragma unroll
+    for (int i = 0; i < kKeysPerThread; i++) {
+      if (digit[i] == ~0u) continue;
+      const int at = warp * per_warp + i * 32 + lane;
+      const uint32_t key = s.keys[from][at], token = s.tokens[from][at];
+      const int g = (int)(s.base[digit[i]] + s.counts[warp * bins + digit[i]] + place[i]);
+      if (last) {
+        sorted_keys[g] = key;
+        sorted_tokens[g] = token;
+      } else {
+        const int to = g / share, slot = g - to * share;
+        cluster.map_shared_rank(s.keys[from ^ 1], to)[slot] = key;
+        cluster.map_shared_rank(s.tokens[from ^ 1], to)[slot] = token;
+      }
+    }
+    if (!last) cluster.sync();  // the pass's writes have arrived; nobody reads this block's totals any more
   }
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // More tokens: three launches a pass, over tiles of 8192 keys.
@@ -235,8 +262,8 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_count_kernel(const 
   for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(s.counts)[i] = 0;
   const int n = load_tile(indices, keys_in, tokens_in, tokens, vocab, s);
   __syncthreads();
-  walk_keys<false>(s.keys[0], s.tokens[0], n, kSortKeys / kSortWarps, shift, bins, s.counts,
-                   [](uint32_t, uint32_t, uint32_t, uint32_t) {});
+  uint32_t digit[kKeysPerThread], place[kKeysPerThread];
+  rank_keys(s.keys[0], n, kSortKeys / kSortWarps, shift, bins, s.counts, digit, place);
   __syncthreads();
   const uint32_t total = prefix_over_warps(s.counts, bins);
   if ((int)threadIdx.x < bins) counts[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = total;
@@ -266,51 +293,57 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_scatter_kernel(
   for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(s.counts)[i] = 0;
   const int n = load_tile(indices, keys_in, tokens_in, tokens, vocab, s);
   __syncthreads();
-  walk_keys<false>(s.keys[0], s.tokens[0], n, kSortKeys / kSortWarps, shift, bins, s.counts,
-                   [](uint32_t, uint32_t, uint32_t, uint32_t) {});
+  uint32_t digit[kKeysPerThread], place[kKeysPerThread];
+  rank_keys(s.keys[0], n, kSortKeys / kSortWarps, shift, bins, s.counts, digit, place);
   __syncthreads();
   prefix_over_warps(s.counts, bins);
   if ((int)threadIdx.x < bins) s.base[threadIdx.x] = counts[(int64_t)threadIdx.x * gridDim.x + blockIdx.x];
   __syncthreads();
-  walk_keys<true>(s.keys[0], s.tokens[0], n, kSortKeys / kSortWarps, shift, bins, s.counts,
-                  [&](uint32_t key, uint32_t token, uint32_t digit, uint32_t place) {
-                    const uint32_t g = s.base[digit] + place;
-                    keys_out[g] = key;
-                    tokens_out[g] = token;
-                  });
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int i = 0; i < kKeysPerThread; i++) {
+    if (digit[i] == ~0u) continue;
+    const int at = warp * (kSortKeys / kSortWarps) + i * 32 + lane;
+    const uint32_t g = s.base[digit[i]] + s.counts[warp * bins + digit[i]] + place[i];
+    keys_out[g] = s.keys[0][at];
+    tokens_out[g] = s.tokens[0][at];
+  }
 }
 
 // ---- gradient: sums over the sorted tokens -----------------------------------------------------------------
-// A warp takes 32 sorted tokens and 32 V columns.  A table row whose tokens all lie in this chunk is
+// A warp takes 16 sorted tokens and 32 V columns.  A table row whose tokens all lie in this chunk is
 // finished here.  One that began in an earlier chunk leaves this chunk's share in partial[chunk][0], one
 // that begins here and goes on in partial[chunk][1].
-constexpr int kChunk = 32;
-constexpr int kBatch = 8;  // rows of dy in flight a warp
+constexpr int kChunk = 16;
+constexpr int kBatch = 4;  // rows of dy in flight a warp
+constexpr int kSumThreads = 128;
 
 template <typename TD, int V>
-__global__ void __launch_bounds__(kThreads) embedding_sum_kernel(const TD* __restrict__ dy,
+__global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const TD* __restrict__ dy,
                                                                 const uint32_t* __restrict__ keys,
                                                                 const uint32_t* __restrict__ order,
                                                                 float* __restrict__ dtable, float* __restrict__ partial,
                                                                 int64_t tokens, uint32_t vocab, int64_t width, float scale,
                                                                 int64_t tiles, int64_t items) {
   const int lane = threadIdx.x & 31;
-  const int64_t item = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const int64_t item = (int64_t)blockIdx.x * (kSumThreads / 32) + (threadIdx.x >> 5);
+  pdl_launch_dependents();  // the join waits for this kernel's end
+  pdl_wait();
   if (item >= items) return;
   const int64_t chunk = item / tiles, col = ((item - chunk * tiles) * 32 + lane) * V;
   const int64_t p0 = chunk * kChunk;
-  const uint32_t key = p0 + lane < tokens ? keys[p0 + lane] : vocab;
-  const uint32_t token = p0 + lane < tokens ? order[p0 + lane] : 0;
+  const bool held = lane < kChunk && p0 + lane < tokens;
+  const uint32_t key = held ? keys[p0 + lane] : vocab;
+  const uint32_t token = held ? order[p0 + lane] : 0;
   uint32_t edge = vocab;  // lane 0: the key before the chunk, lane 1: the key behind it
   if (lane == 0 && p0 > 0) edge = keys[p0 - 1];
   if (lane == 1 && p0 + kChunk < tokens) edge = keys[p0 + kChunk];
   const uint32_t before = p0 > 0 ? __shfl_sync(0xffffffffu, edge, 0) : 0xffffffffu;
   const uint32_t behind = __shfl_sync(0xffffffffu, edge, 1);
-  const uint32_t below = __shfl_down_sync(0xffffffffu, key, 1);
-  const uint32_t next = lane == 31 ? behind : below;
+  const uint32_t next = __shfl_down_sync(0xffffffffu, key, 1);
   const uint32_t first_key = __shfl_sync(0xffffffffu, key, 0);
   const int n = __popc(__ballot_sync(0xffffffffu, key < vocab));  // keys ascend: the real ones come first
-  const uint32_t ends = __ballot_sync(0xffffffffu, key != next || lane == 31);
+  const uint32_t ends = __ballot_sync(0xffffffffu, key != next || lane == kChunk - 1);
   const bool column = col < width;
   float acc[V];
 #pragma unroll
@@ -336,7 +369,7 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(const TD* __res
       if (!(ends >> at & 1)) continue;
       const uint32_t row = __shfl_sync(0xffffffffu, key, at);
       const bool came = row == first_key && row == before;
-      const bool goes = at == 31 && row == behind;
+      const bool goes = at == kChunk - 1 && row == behind;
       if (column) {
         if (came || goes) {
           store_vec<V>(partial + (chunk * 2 + (came ? 0 : 1)) * width + col, acc);
@@ -352,60 +385,91 @@ __global__ void __launch_bounds__(kThreads) embedding_sum_kernel(const TD* __res
   }
 }
 
-// The table rows that begin in chunk blockIdx.x and go on: the sum of the chunks' shares.  Each of the 8
-// warps adds a run of chunks, then the runs are added in order.
+// The table rows that begin in one chunk and go on in others: the sum of the chunks' shares.  A warp takes a
+// chunk and 32 V columns, and up to 31 further chunks by itself; the longer runs (a token of hundreds of
+// places) the block's 8 warps then share out one after the other, each adding a run of chunks, in order.
+constexpr int kJoinWarps = kThreads / 32;
+template <int V>
+__device__ __forceinline__ void add_shares(const float* partial, int64_t lo, int64_t hi, int64_t width, int64_t col,
+                                           float (&acc)[V]) {
+#pragma unroll 8
+  for (int64_t c = lo; c < hi; c++) {
+    float v[V];
+    load_vec<V>(partial + c * 2 * width + col, v);
+#pragma unroll
+    for (int k = 0; k < V; k++) acc[k] += v[k];
+  }
+}
 template <int V>
 __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t* __restrict__ keys,
                                                                  const float* __restrict__ partial,
                                                                  float* __restrict__ dtable, int64_t tokens,
-                                                                 uint32_t vocab, int64_t width, float scale) {
-  __shared__ __align__(16) float join[kThreads / 32][32 * V];
+                                                                 uint32_t vocab, int64_t width, float scale,
+                                                                 int64_t chunks) {
+  __shared__ __align__(16) float join[kJoinWarps][32 * V];
+  __shared__ uint32_t long_row[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t chunk = blockIdx.x, end = (chunk + 1) * kChunk;
-  if (end >= tokens) return;
-  const uint32_t row = keys[end - 1];
-  if (row >= vocab || keys[end] != row || (chunk > 0 && keys[end - kChunk - 1] == row)) return;
-  // chunks that go on with this row: those whose first key it is
-  const int64_t chunks = (tokens + kChunk - 1) / kChunk;
-  int64_t more = 0;
-  for (;;) {
-    const int64_t c = chunk + 1 + more + threadIdx.x;
-    const int hit = __syncthreads_count(c < chunks && keys[c * kChunk] == row);
-    more += hit;
-    if (hit < kThreads) break;
+  const int64_t first = (int64_t)blockIdx.x * kJoinWarps, chunk = first + warp, end = (chunk + 1) * kChunk;
+  pdl_wait();
+  uint32_t row = vocab, behind = vocab, before = vocab, head = vocab;
+  if (end < tokens) {
+    row = keys[end - 1];
+    behind = keys[end];
+    if (chunk > 0) before = keys[end - kChunk - 1];
+    if (chunk + 1 + lane < chunks) head = keys[(chunk + 1 + lane) * kChunk];
   }
-  const int64_t per = (more + kThreads / 32 - 1) / (kThreads / 32);
-  const int64_t lo = chunk + 1 + warp * per, hi = min(lo + per, chunk + 1 + more);
+  const bool mine = row < vocab && behind == row && before != row;
+  const int more = mine ? __popc(__ballot_sync(0xffffffffu, head == row)) : 0;  // heads ascend: a run of ones
+  if (lane == 0) long_row[warp] = more == 32 ? row : vocab;
   for (int64_t j0 = (int64_t)blockIdx.y * 32 * V; j0 < width; j0 += (int64_t)gridDim.y * 32 * V) {
     const int64_t col = j0 + lane * V;
-    float acc[V];
-#pragma unroll
-    for (int k = 0; k < V; k++) acc[k] = 0.f;
-    if (col < width) {
-      if (warp == 0) load_vec<V>(partial + (chunk * 2 + 1) * width + col, acc);
-#pragma unroll 4
-      for (int64_t c = lo; c < hi; c++) {
-        float v[V];
-        load_vec<V>(partial + c * 2 * width + col, v);
-#pragma unroll
-        for (int k = 0; k < V; k++) acc[k] += v[k];
-      }
-    }
-    store_vec<V>(&join[warp][lane * V], acc);
-    __syncthreads();
-    if (warp == 0 && col < width) {
-#pragma unroll
-      for (int w = 1; w < kThreads / 32; w++) {
-        float v[V];
-        load_vec<V>(&join[w][lane * V], v);
-#pragma unroll
-        for (int k = 0; k < V; k++) acc[k] += v[k];
-      }
+    if (more > 0 && more < 32 && col < width) {
+      float acc[V];
+      load_vec<V>(partial + (chunk * 2 + 1) * width + col, acc);
+      add_shares<V>(partial, chunk + 1, chunk + 1 + more, width, col, acc);
 #pragma unroll
       for (int k = 0; k < V; k++) acc[k] *= scale;
       store_vec<V>(dtable + (int64_t)row * width + col, acc);
     }
-    __syncthreads();
+  }
+  __syncthreads();
+  for (int w = 0; w < kJoinWarps; w++) {
+    const uint32_t long_key = long_row[w];
+    if (long_key >= vocab) continue;  // the same for the whole block
+    int64_t run = 0;
+    for (;;) {
+      const int64_t c = first + w + 1 + run + threadIdx.x;
+      const int hit = __syncthreads_count(c < chunks && keys[c * kChunk] == long_key);
+      run += hit;
+      if (hit < kThreads) break;
+    }
+    const int64_t per = (run + kJoinWarps - 1) / kJoinWarps;
+    const int64_t lo = first + w + 1 + warp * per, hi = min(lo + per, first + w + 1 + run);
+    for (int64_t j0 = (int64_t)blockIdx.y * 32 * V; j0 < width; j0 += (int64_t)gridDim.y * 32 * V) {
+      const int64_t col = j0 + lane * V;
+      float acc[V];
+#pragma unroll
+      for (int k = 0; k < V; k++) acc[k] = 0.f;
+      if (col < width) {
+        if (warp == 0) load_vec<V>(partial + ((first + w) * 2 + 1) * width + col, acc);
+        add_shares<V>(partial, lo, hi, width, col, acc);
+      }
+      store_vec<V>(&join[warp][lane * V], acc);
+      __syncthreads();
+      if (warp == 0 && col < width) {
+#pragma unroll
+        for (int o = 1; o < kJoinWarps; o++) {
+          float v[V];
+          load_vec<V>(&join[o][lane * V], v);
+#pragma unroll
+          for (int k = 0; k < V; k++) acc[k] += v[k];
+        }
+#pragma unroll
+        for (int k = 0; k < V; k++) acc[k] *= scale;
+        store_vec<V>(dtable + (int64_t)long_key * width + col, acc);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -420,16 +484,20 @@ struct LookupArgs {
   Decode q;
 };
 
-template <typename TT, typename TO, int V, int L>
+template <typename TT, typename TO, int V, int L, int U>
 void lookup_lanes(tfjs_cuda_ctx* ctx, const LookupArgs& a) {
-  const int64_t blocks = ceil_div64(a.tokens, kThreads / L);
-  embedding_kernel<TT, TO, V, L><<<(unsigned)(blocks < (1 << 30) ? blocks : (1 << 30)), kThreads, 0, ctx->stream>>>(
-      (const TT*)a.table, a.indices, (TO*)a.out, a.tokens, a.vocab, a.width, a.scale, a.q);
+  const int64_t parts = ceil_div64(a.width / V, U * L);
+  const bool stream = a.tokens * a.width * (int64_t)sizeof(TO) > kStreamBytes;
+  embedding_kernel<TT, TO, V, L, U><<<dim3((unsigned)ceil_div64(a.tokens, kThreads / L), (unsigned)(parts < 64 ? parts : 64)),
+                                      kThreads, 0, ctx->stream>>>((const TT*)a.table, a.indices, (TO*)a.out, a.tokens, a.vocab,
+                                                                  a.width, a.scale, a.q, stream);
 }
 template <typename TT, typename TO, int V>
 void lookup_width(tfjs_cuda_ctx* ctx, const LookupArgs& a) {
-  if (a.width <= 8 * V) lookup_lanes<TT, TO, V, 8>(ctx, a);
-  else lookup_lanes<TT, TO, V, 32>(ctx, a);
+  constexpr int U = sizeof(TT) == 1 ? 8 : 4;
+  if (a.width <= 8 * V) lookup_lanes<TT, TO, V, 8, 1>(ctx, a);
+  else if (a.width <= 64 * V) lookup_lanes<TT, TO, V, 32, 2>(ctx, a);
+  else lookup_lanes<TT, TO, V, 32, U>(ctx, a);
 }
 // 16 bytes of the result a lane where the width allows it (bytes: 4, which are 16 of the result)
 template <typename TT, typename TO>
@@ -509,12 +577,13 @@ template <typename TD, int V>
 int sum_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, const uint32_t* keys, const uint32_t* order, float* partial) {
   const int64_t chunks = ceil_div64(a.tokens, kChunk), tiles = ceil_div64(a.width, 32 * V), items = chunks * tiles;
   TFJS_REQUIRE(ctx, items < (1ll << 33), "embeddingLookupBackprop: too many tokens times columns");
-  embedding_sum_kernel<TD, V><<<(unsigned)ceil_div64(items, kThreads / 32), kThreads, 0, ctx->stream>>>(
-      (const TD*)a.dy, keys, order, a.dtable, partial, a.tokens, (uint32_t)a.vocab, a.width, a.scale, tiles, items);
+  launch_dependent(ctx, embedding_sum_kernel<TD, V>, dim3((unsigned)ceil_div64(items, kSumThreads / 32)), dim3(kSumThreads),
+                   (const TD*)a.dy, keys, order, a.dtable, partial, a.tokens, (uint32_t)a.vocab, a.width, a.scale, tiles,
+                   items);
   const int rc = post_launch(ctx, "embeddingLookupBackprop (sum)");
   if (rc || chunks < 2) return rc;
-  embedding_join_kernel<V><<<dim3((unsigned)(chunks - 1), (unsigned)(tiles < 64 ? tiles : 64)), kThreads, 0, ctx->stream>>>(
-      keys, partial, a.dtable, a.tokens, (uint32_t)a.vocab, a.width, a.scale);
+  launch_dependent(ctx, embedding_join_kernel<V>, dim3((unsigned)ceil_div64(chunks - 1, kJoinWarps), (unsigned)(tiles < 64 ? tiles : 64)),
+                   dim3(kThreads), keys, (const float*)partial, a.dtable, a.tokens, (uint32_t)a.vocab, a.width, a.scale, chunks);
   return post_launch(ctx, "embeddingLookupBackprop (join)");
 }
 

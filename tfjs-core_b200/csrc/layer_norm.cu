@@ -57,55 +57,74 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 }
 
 // ---- forward -------------------------------------------------------------------------------------
-// L lanes a row, NV vectors of V values a lane: width <= L * NV * V, a multiple of V.
+// L lanes a row, NV vectors of V values a lane: width <= L * NV * V, a multiple of V.  Up to 16 values a
+// lane, gamma and beta are fetched with the row; with more, the registers serve more rows at once instead.
 template <typename TX, typename TY, int V, int NV, int L>
 __global__ void __launch_bounds__(256) layer_norm_lanes_kernel(const TX* __restrict__ x, const float* __restrict__ gamma,
                                                               const float* __restrict__ beta, TY* __restrict__ y,
                                                               float* __restrict__ stats, int64_t rows, int width,
                                                               float epsilon) {
+  constexpr bool kAhead = NV * V <= 16;
   const int lane = threadIdx.x & (L - 1);
-  const int64_t step = (int64_t)gridDim.x * (256 / L);
-  // all lanes of a warp go round the loop together, so that the shuffles see every lane
-  for (int64_t base = (int64_t)blockIdx.x * (256 / L); base < rows; base += step) {
-    const int64_t row = base + threadIdx.x / L;
-    const bool there = row < rows;
-    const TX* r = x + row * width;
-    float v[NV][V];
-    float s = 0.f;
+  const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  const bool there = row < rows;  // lanes without a row go along, for the shuffles
+  const TX* r = x + row * width;
+  float v[NV][V], g[kAhead ? NV : 1][V], b[kAhead ? NV : 1][V];
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int col = (i * L + lane) * V;
-      if (there && col < width) {
-        load_vec<V>(r + col, v[i]);
-      } else {
+  for (int i = 0; i < NV; i++) {
+    const int col = (i * L + lane) * V;
+    if (there && col < width) {
+      load_vec<V>(r + col, v[i]);
+    } else {
 #pragma unroll
-        for (int k = 0; k < V; k++) v[i][k] = 0.f;
-      }
+      for (int k = 0; k < V; k++) v[i][k] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-      for (int k = 0; k < V; k++) s += v[i][k];
-    const float mean = lanes_sum<L>(s) / (float)width;
-    s = 0.f;
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-      if ((i * L + lane) * V < width) {
-#pragma unroll
-        for (int k = 0; k < V; k++) {
-          const float d = v[i][k] - mean;
-          s = fmaf(d, d, s);
-        }
-      }
-    const float rstd = 1.f / sqrtf(lanes_sum<L>(s) / (float)width + epsilon);
-    if (!there) continue;
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int col = (i * L + lane) * V;
-      if (col < width) finish_vec<V>(v[i], mean, rstd, gamma, beta, col, y + row * width + col);
-    }
-    if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
   }
+  if constexpr (kAhead) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int col = (i * L + lane) * V;
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        g[i][k] = 1.f;
+        b[i][k] = 0.f;
+      }
+      if (gamma && col < width) load_vec<V>(gamma + col, g[i]);
+      if (beta && col < width) load_vec<V>(beta + col, b[i]);
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; i++)
+#pragma unroll
+    for (int k = 0; k < V; k++) s += v[i][k];
+  const float mean = lanes_sum<L>(s) / (float)width;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; i++)
+    if ((i * L + lane) * V < width) {
+#pragma unroll
+      for (int k = 0; k < V; k++) {
+        const float d = v[i][k] - mean;
+        s = fmaf(d, d, s);
+      }
+    }
+  const float rstd = 1.f / sqrtf(lanes_sum<L>(s) / (float)width + epsilon);
+  if (!there) return;
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int col = (i * L + lane) * V;
+    if (col >= width) break;
+    if constexpr (kAhead) {
+      float o[V];
+#pragma unroll
+      for (int k = 0; k < V; k++) o[k] = (v[i][k] - mean) * rstd * g[i][k] + b[i][k];
+      store_vec<V>(y + row * width + col, o);
+    } else {
+      finish_vec<V>(v[i], mean, rstd, gamma, beta, col, y + row * width + col);
+    }
+  }
+  if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
 }
 
 // One block of NT threads a row: width <= NT * NV * V, a multiple of V.
@@ -236,8 +255,8 @@ __global__ void __launch_bounds__(kClusterThreads) layer_norm_cluster_kernel(
 
 // ---- gradient, width <= kStagedWidth -----------------------------------------------------------------
 constexpr int kStagedWidth = 8192;
-constexpr int kStagedThreads = 512;
-constexpr int kMaxStageRows = 512;
+constexpr int kStagedThreads = 256;
+constexpr int kMaxStageRows = 256;
 
 __device__ __forceinline__ void copy_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
@@ -264,40 +283,43 @@ struct StagedParams {
 // The whole 16-byte units that [first, first + bytes) touches, into shared memory.  The units lie
 // within the tensor's buffer: its start is 16-byte aligned and its size class a multiple of 16.
 __device__ __forceinline__ void stage_copy(uint8_t* dst, const uint8_t* base, int64_t first, int bytes) {
-  const int64_t lo = first & ~15ll;
-  const int units = (int)((first + bytes - lo + 15) >> 4);
-  for (int i = threadIdx.x; i < units; i += kStagedThreads) copy_async16(dst + i * 16, base + lo + (int64_t)i * 16);
+  const int off = (int)(first & 15), units = (off + bytes + 15) >> 4;
+  const uint8_t* src = base + (first - off);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < units; i += kStagedThreads) copy_async16(dst + i * 16, src + i * 16);
 }
 
 constexpr int kStages = 3;
 
-template <typename TD, typename TX, int V, int MC, int MINB>
-__global__ void __launch_bounds__(kStagedThreads, MINB) layer_norm_staged_kernel(const TD* __restrict__ dy,
-                                                                                 const TX* __restrict__ x,
-                                                                                 StagedParams p) {
+// MC vectors of V columns a thread: width <= 256 * MC * V, a multiple of V.
+template <typename TD, typename TX, int V, int MC>
+__global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(const TD* __restrict__ dy,
+                                                                              const TX* __restrict__ x,
+                                                                              StagedParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int width = p.width, R = p.stage_rows, nc = width / V;
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x;
+  const float inv = 1.f / (float)width;
   uint8_t* ring = smem;
   float* s_gamma = reinterpret_cast<float*>(smem + kStages * p.stage_bytes);
-  const int LR = R >= kStagedThreads ? 1 : kStagedThreads / R;   // lanes that sum a row
-  const int parts = LR > 32 ? LR / 32 : 1;                       // their warps' partial sums
+  const int LR = kStagedThreads / R;             // lanes that sum a row
+  const int parts = LR > 32 ? LR / 32 : 1;       // their warps' partial sums
   float2* s_part = reinterpret_cast<float2*>(s_gamma + (width + 3) / 4 * 4);
-
-  for (int j = tid; j < width; j += kStagedThreads) s_gamma[j] = p.gamma ? p.gamma[j] : 1.f;
 
   // phase 2: thread -> columns; several row groups share the block where a row has few columns
   const int RG = nc < kStagedThreads ? kStagedThreads / nc : 1;
   const int rg = nc < kStagedThreads ? tid / nc : 0;
   const int c0 = nc < kStagedThreads ? tid - rg * nc : tid;
   const bool owner = rg < RG;
+  // phase 1: LR threads a row
+  const int l = tid & (LR - 1), row1 = tid / LR;
   float dg[MC][V], db[MC][V];
 #pragma unroll
   for (int i = 0; i < MC; i++)
 #pragma unroll
     for (int k = 0; k < V; k++) dg[i][k] = db[i][k] = 0.f;
 
-  const int64_t first = blockIdx.x, step = gridDim.x;
+  const int64_t step = gridDim.x;
   auto fill = [&](int64_t item, int slot) {
     if (item < p.items) {
       const int64_t row = item * R;
@@ -306,15 +328,17 @@ __global__ void __launch_bounds__(kStagedThreads, MINB) layer_norm_staged_kernel
       stage_copy(dst, (const uint8_t*)dy, row * width * (int64_t)sizeof(TD), n * width * (int)sizeof(TD));
       stage_copy(dst + p.x_bytes, (const uint8_t*)x, row * width * (int64_t)sizeof(TX), n * width * (int)sizeof(TX));
       float2* st = reinterpret_cast<float2*>(dst + p.stage_bytes) - R;
-      for (int i = tid; i < n; i += kStagedThreads) copy_async8(st + i, p.stats + 2 * (row + i));
+      if (tid < n) copy_async8(st + tid, p.stats + 2 * (row + tid));
     }
     copy_commit();
   };
 #pragma unroll
-  for (int s = 0; s < kStages - 1; s++) fill(first + s * step, s);
+  for (int s = 0; s < kStages - 1; s++) fill(blockIdx.x + s * step, s);
+  for (int j = tid; j < width; j += kStagedThreads) s_gamma[j] = p.gamma ? p.gamma[j] : 1.f;
+  pdl_launch_dependents();  // the join kernel waits for this one's end before it reads
 
   int slot = 0;
-  for (int64_t item = first; item < p.items; item += step) {
+  for (int64_t item = blockIdx.x; item < p.items; item += step) {
     copy_wait<kStages - 2>();
     __syncthreads();  // this stage has arrived for all; the stage before it has been read by all
     fill(item + (kStages - 1) * step, slot == 0 ? kStages - 1 : slot - 1);
@@ -324,61 +348,65 @@ __global__ void __launch_bounds__(kStagedThreads, MINB) layer_norm_staged_kernel
     const TD* sd = reinterpret_cast<const TD*>(st + ((row0 * width * (int64_t)sizeof(TD)) & 15));
     const TX* sx = reinterpret_cast<const TX*>(st + p.x_bytes + ((row0 * width * (int64_t)sizeof(TX)) & 15));
     const float2* ss = reinterpret_cast<const float2*>(st + p.stage_bytes) - R;
-    // ---- phase 1: sum a and a n of each row
+    // ---- phase 1: sum a and a (x - m) of each row
     {
-      const int l = tid & (LR - 1);
-      const int row = tid / LR;   // groups of LR threads, one row each (R * LR >= the block)
       float sa = 0.f, sn = 0.f;
-      if (row < n) {
-        const float2 mr = ss[row];
+      if (row1 < n) {
+        const float m = ss[row1].x;
+        const TD* d1 = sd + row1 * width;
+        const TX* x1 = sx + row1 * width;
+#pragma unroll 4
         for (int j = l; j < nc; j += LR) {
           float d[V], v[V], g[V];
-          load_vec<V>(sd + row * width + j * V, d);
-          load_vec<V>(sx + row * width + j * V, v);
+          load_vec<V>(d1 + j * V, d);
+          load_vec<V>(x1 + j * V, v);
           load_vec<V>(s_gamma + j * V, g);
 #pragma unroll
           for (int k = 0; k < V; k++) {
             const float a = d[k] * g[k];
             sa += a;
-            sn = fmaf(a, (v[k] - mr.x) * mr.y, sn);
+            sn = fmaf(a, v[k] - m, sn);
           }
         }
       }
-      const int w = LR < 32 ? LR : 32;
-      for (int o = w >> 1; o > 0; o >>= 1) {
+      for (int o = (LR < 32 ? LR : 32) >> 1; o > 0; o >>= 1) {
         sa += __shfl_xor_sync(0xffffffffu, sa, o);
         sn += __shfl_xor_sync(0xffffffffu, sn, o);
       }
-      if ((l & 31) == 0 && row < R) s_part[row * parts + (l >> 5)] = make_float2(sa, sn);
+      if ((l & 31) == 0) s_part[row1 * parts + (l >> 5)] = make_float2(sa, sn);
     }
     __syncthreads();
     // ---- phase 2: dx, and the owned columns' dg and db
     if (owner) {
+#pragma unroll 2
       for (int row = rg; row < n; row += RG) {
-        float2 t = make_float2(0.f, 0.f);
-        for (int i = 0; i < parts; i++) {
+        const float2 mr = ss[row];
+        float2 t = s_part[row * parts];
+        for (int i = 1; i < parts; i++) {
           const float2 o = s_part[row * parts + i];
           t.x += o.x;
           t.y += o.y;
         }
-        const float ma = t.x / (float)width, man = t.y / (float)width;
-        const float2 mr = ss[row];
+        const float ma = t.x * inv, man = t.y * mr.y * inv;
+        const TD* d2 = sd + row * width;
+        const TX* x2 = sx + row * width;
+        float* out = p.dx + (row0 + row) * width;
 #pragma unroll
         for (int i = 0; i < MC; i++) {
           const int c = c0 + i * kStagedThreads;
-          if (c >= nc) break;
+          if (MC > 1 && c >= nc) break;
           float d[V], v[V], g[V], o[V];
-          load_vec<V>(sd + row * width + c * V, d);
-          load_vec<V>(sx + row * width + c * V, v);
+          load_vec<V>(d2 + c * V, d);
+          load_vec<V>(x2 + c * V, v);
           load_vec<V>(s_gamma + c * V, g);
 #pragma unroll
           for (int k = 0; k < V; k++) {
             const float nn = (v[k] - mr.x) * mr.y;
-            o[k] = mr.y * (d[k] * g[k] - ma - nn * man);
+            o[k] = mr.y * fmaf(-nn, man, fmaf(d[k], g[k], -ma));
             dg[i][k] = fmaf(d[k], nn, dg[i][k]);
             db[i][k] += d[k];
           }
-          if (p.dx) store_vec<V>(p.dx + (row0 + row) * width + c * V, o);
+          if (p.dx) store_vec<V>(out + c * V, o);
         }
       }
     }
@@ -426,6 +454,7 @@ __global__ void __launch_bounds__(kClusterThreads) layer_norm_backprop_cluster_k
   const int64_t rank = blockIdx.x % kClusterBlocks;
   const int64_t lo = vecs * rank / kClusterBlocks * V, n = vecs * (rank + 1) / kClusterBlocks - vecs * rank / kClusterBlocks;
   float* pg = partial ? partial + cluster * 2 * width + lo : nullptr;
+  pdl_launch_dependents();  // the join kernel waits for this one's end before it reads
   int turn = 0;
   for (int64_t row = cluster; row < rows; row += clusters, turn ^= 1) {
     const TD* d0 = dy + row * width + lo;
@@ -483,6 +512,7 @@ __global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __res
                                                              float* __restrict__ dbeta, int blocks, int64_t width) {
   __shared__ float part[8][32];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  pdl_wait();
   for (int64_t j0 = (int64_t)blockIdx.x * 32; j0 < 2 * width; j0 += (int64_t)gridDim.x * 32) {
     const int64_t j = j0 + lane;
     float s = 0.f;
@@ -519,7 +549,7 @@ unsigned grid_rows(const tfjs_cuda_ctx* ctx, int64_t blocks, int per_sm) {
 
 template <typename TX, typename TY, int V, int NV, int L>
 void lanes_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
-  layer_norm_lanes_kernel<TX, TY, V, NV, L><<<grid_rows(ctx, ceil_div64(a.rows, 256 / L), 8), 256, 0, ctx->stream>>>(
+  layer_norm_lanes_kernel<TX, TY, V, NV, L><<<(unsigned)ceil_div64(a.rows, 256 / L), 256, 0, ctx->stream>>>(
       (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon);
 }
 template <typename TX, typename TY, int V, int NV, int NT>
@@ -589,7 +619,7 @@ int forward_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
 
 template <typename TX, typename TY>
 int launch_forward(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
-  constexpr int W = 16 / (int)sizeof(TX);
+  constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;  // 16 bytes of the result
   if (a.width % W == 0) return forward_form<TX, TY, W>(ctx, a);
   if (a.width % 2 == 0) return forward_form<TX, TY, 2>(ctx, a);
   return forward_form<TX, TY, 1>(ctx, a);
@@ -603,15 +633,16 @@ struct BackwardArgs {
 };
 
 int join(tfjs_cuda_ctx* ctx, const BackwardArgs& a, const float* partial, int blocks) {
-  layer_norm_join_kernel<<<grid_rows(ctx, ceil_div64(2 * a.width, 32), 16), 256, 0, ctx->stream>>>(
-      partial, a.dgamma, a.dbeta, blocks, a.width);
+  launch_dependent(ctx, layer_norm_join_kernel, dim3(grid_rows(ctx, ceil_div64(2 * a.width, 32), 16)), dim3(256), partial,
+                   a.dgamma, a.dbeta, blocks, a.width);
   return post_launch(ctx, "layerNormBackprop (join)");
 }
 
-template <typename TD, typename TX, int V, int MC, int MINB>
+template <typename TD, typename TX, int V, int MC>
 int staged_launch(tfjs_cuda_ctx* ctx, const BackwardArgs& a, StagedParams& p, int blocks, size_t smem) {
-  auto kernel = layer_norm_staged_kernel<TD, TX, V, MC, MINB>;
-  TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  auto kernel = layer_norm_staged_kernel<TD, TX, V, MC>;
+  if (smem > 48 * 1024)
+    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   kernel<<<blocks, kStagedThreads, smem, ctx->stream>>>((const TD*)a.dy, (const TX*)a.x, p);
   return post_launch(ctx, "layerNormBackprop");
 }
@@ -619,10 +650,10 @@ int staged_launch(tfjs_cuda_ctx* ctx, const BackwardArgs& a, StagedParams& p, in
 template <typename TD, typename TX, int V>
 int staged_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
   const int width = (int)a.width, row_bytes = width * (int)(sizeof(TD) + sizeof(TX));
-  // rows a stage: about 24 KB, so that two blocks with three stages each share an SM, but not so many
-  // that the blocks have fewer than four stages each
+  // rows a stage: about 32 KB, so that two blocks with three stages each share an SM, but not so many
+  // that the blocks have fewer than two stages each
   int R = 1;
-  while (R < kMaxStageRows && 2 * R * row_bytes <= 24 * 1024 && ceil_div64(a.rows, 2 * R) >= 8 * ctx->sm_count) R *= 2;
+  while (R < kMaxStageRows && 2 * R * row_bytes <= 32 * 1024 && ceil_div64(a.rows, 2 * R) >= 4 * ctx->sm_count) R *= 2;
   StagedParams p = {};
   p.gamma = a.gamma;
   p.stats = a.stats;
@@ -633,16 +664,11 @@ int staged_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
   p.stage_rows = R;
   p.x_bytes = (R * width * (int)sizeof(TD) + 31) / 16 * 16;  // one 16-byte unit more for the rows' own offset
   p.stage_bytes = p.x_bytes + (R * width * (int)sizeof(TX) + 31) / 16 * 16 + (R + 1) / 2 * 16;
-  const int LR = R >= kStagedThreads ? 1 : kStagedThreads / R;
-  size_t smem = (size_t)kStages * p.stage_bytes;
-  const size_t join_bytes = (size_t)2 * kStagedThreads * V * 4;  // the row groups' sums reuse the ring
-  if (smem < join_bytes) {
-    p.stage_bytes = ((int)(join_bytes / kStages) + 16) / 16 * 16;
-    smem = (size_t)kStages * p.stage_bytes;
-  }
-  smem += (size_t)(width + 3) / 4 * 16 + (size_t)R * (LR > 32 ? LR / 32 : 1) * 8;
-  const int per_sm = smem <= 113 * 1024 && width <= 1024 * V ? 2 : 1;
-  const int64_t cap = (int64_t)ctx->sm_count * per_sm;
+  const int join_bytes = 2 * kStagedThreads * V * 4;  // the row groups' sums reuse the ring
+  if (kStages * p.stage_bytes < join_bytes) p.stage_bytes = (join_bytes / kStages + 16) / 16 * 16;
+  const int parts = kStagedThreads / R > 32 ? kStagedThreads / R / 32 : 1;
+  const size_t smem = (size_t)kStages * p.stage_bytes + (size_t)(width + 3) / 4 * 16 + (size_t)R * parts * 8;
+  const int64_t cap = (int64_t)ctx->sm_count * (smem <= 113 * 1024 ? 2 : 1);
   const int blocks = (int)(p.items < cap ? p.items : cap);
   void* partial = nullptr;
   size_t partial_cap = 0;
@@ -651,12 +677,12 @@ int staged_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
     if ((rc = ctx_alloc(ctx, (size_t)blocks * 2 * width * 4, &partial, &partial_cap))) return rc;
     p.partial = (float*)partial;
   }
-  // columns a thread: width / V / 512, rounded up to 1, 2, 4, 8 or 16 vectors
-  const int mc = (width / V + kStagedThreads - 1) / kStagedThreads;
-  if (mc <= 1) rc = staged_launch<TD, TX, V, 1, 2>(ctx, a, p, blocks, smem);
-  else if (mc <= 2) rc = staged_launch<TD, TX, V, 2, 2>(ctx, a, p, blocks, smem);
-  else if (mc <= 4) rc = staged_launch<TD, TX, V, 4, 1>(ctx, a, p, blocks, smem);
-  else if constexpr (V == 1) rc = staged_launch<TD, TX, V, 16, 1>(ctx, a, p, blocks, smem);
+  // 4, 8, 16 or 32 columns a thread
+  const int columns = (width + kStagedThreads - 1) / kStagedThreads;
+  if (columns <= 4) rc = staged_launch<TD, TX, V, 4 / V>(ctx, a, p, blocks, smem);
+  else if (columns <= 8) rc = staged_launch<TD, TX, V, 8 / V>(ctx, a, p, blocks, smem);
+  else if (columns <= 16) rc = staged_launch<TD, TX, V, 16 / V>(ctx, a, p, blocks, smem);
+  else rc = staged_launch<TD, TX, V, 32 / V>(ctx, a, p, blocks, smem);
   if (!rc && partial) rc = join(ctx, a, (const float*)partial, blocks);
   ctx_free(ctx, partial, partial_cap);
   return rc;

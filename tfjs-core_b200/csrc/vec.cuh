@@ -70,6 +70,33 @@ __device__ __forceinline__ void store_vec(__half* p, const float (&v)[V]) {
   }
 }
 
+// The same with an evict-first hint, for results so large (kStreamBytes and more, where L2 holds 126 MB) that
+// whoever reads them next finds little of them in L2 anyway.
+constexpr int64_t kStreamBytes = 96ll << 20;
+template <int V>
+__device__ __forceinline__ void store_vec_stream(float* p, const float (&v)[V]) {
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) __stcs(reinterpret_cast<float4*>(p + i), make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+  } else if constexpr (V == 2) {
+    __stcs(reinterpret_cast<float2*>(p), make_float2(v[0], v[1]));
+  } else {
+    __stcs(p, v[0]);
+  }
+}
+template <int V>
+__device__ __forceinline__ void store_vec_stream(__half* p, const float (&v)[V]) {
+  if constexpr (V == 8) {
+    __stcs(reinterpret_cast<uint4*>(p), make_uint4(narrow2(v[0], v[1]), narrow2(v[2], v[3]), narrow2(v[4], v[5]), narrow2(v[6], v[7])));
+  } else if constexpr (V == 4) {
+    __stcs(reinterpret_cast<uint2*>(p), make_uint2(narrow2(v[0], v[1]), narrow2(v[2], v[3])));
+  } else if constexpr (V == 2) {
+    __stcs(reinterpret_cast<uint32_t*>(p), narrow2(v[0], v[1]));
+  } else {
+    __stcs(reinterpret_cast<unsigned short*>(p), __half_as_ushort(__float2half_rn(v[0])));
+  }
+}
+
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
