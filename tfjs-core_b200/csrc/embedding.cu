@@ -71,8 +71,9 @@ __global__ void __launch_bounds__(kThreads) embedding_kernel(const TT* __restric
 // adds), the counters are summed over the warps and blocks, and the same walk then gives each key its
 // place.  No atomics: equal inputs give the same order, ascending tokens within each table row.
 constexpr int kSortThreads = 1024, kSortWarps = 32;
-constexpr int kSortKeys = 8192;  // of one block
+constexpr int kSortKeys = 8192;  // of one block, at most
 constexpr int kMaxBins = 512;
+constexpr int kZeroQuads = 8 * kSortThreads;  // 128 KB of zeros a block
 
 struct Digits {
   int passes, bits;
@@ -87,7 +88,7 @@ Digits digits_of(int64_t vocab) {
 // Each thread's keys (at most 8): their digits, and their places among the keys of that digit that the
 // warp owns; counts[warp][digit] is the number of them.  A place beyond the block's n keys has digit ~0.
 constexpr int kKeysPerThread = kSortKeys / kSortThreads;
-__device__ __forceinline__ void rank_keys(const uint32_t* keys, int n, int per_warp, int shift, int bins, uint16_t* counts,
+__device__ __forceinline__ void rank_keys(const uint2* pairs, int n, int per_warp, int shift, int bins, uint16_t* counts,
                                           uint32_t (&digit)[kKeysPerThread], uint32_t (&place)[kKeysPerThread]) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint16_t* mine = counts + warp * bins;
@@ -98,9 +99,8 @@ __device__ __forceinline__ void rank_keys(const uint32_t* keys, int n, int per_w
     const int at = warp * per_warp + i * 32 + lane;
     const bool there = i * 32 < per_warp && at < n;
     if (!__any_sync(0xffffffffu, there)) continue;
-    if (there) digit[i] = (keys[at] >> shift) & (uint32_t)(bins - 1);
-    // the lanes of the same digit, by a vote on each of its bits (match.any took twice as long: a sort of
-    // 65536 keys 37 us with it)
+    if (there) digit[i] = (pairs[at].x >> shift) & (uint32_t)(bins - 1);
+    // the lanes of the same digit, by a vote on each of its bits
     uint32_t peers = __ballot_sync(0xffffffffu, there);
     for (int bit = 0; (bins >> bit) > 1; bit++) {
       const bool set = digit[i] >> bit & 1;
@@ -153,38 +153,53 @@ __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* warps)
   return (threadIdx.x >> 5 ? before : 0u) + s - v;
 }
 
-struct SortShared {
-  uint32_t keys[2][kSortKeys], tokens[2][kSortKeys];
-  uint16_t counts[kSortWarps * kMaxBins];
-  uint32_t totals[kMaxBins], base[kMaxBins], warps[32];
+// A sorting block's dynamic shared memory, of a size that goes with its share of the keys: `buffers` arrays
+// of (key, token) pairs, the digits' totals and first places, and the warps' counters.
+struct SortView {
+  uint2* pairs[2];
+  uint32_t *totals, *base, *warps;
+  uint16_t* counts;
+  __device__ SortView(uint8_t* raw, int share, int buffers, int bins) {
+    pairs[0] = reinterpret_cast<uint2*>(raw);
+    pairs[1] = pairs[0] + (buffers - 1) * share;
+    totals = reinterpret_cast<uint32_t*>(pairs[1] + share);
+    base = totals + bins;
+    warps = base + bins;
+    counts = reinterpret_cast<uint16_t*>(warps + 32);
+  }
+  static size_t bytes(int share, int buffers, int bins) {
+    return (size_t)share * buffers * 8 + (size_t)bins * 8 + 32 * 4 + (size_t)kSortWarps * bins * 2;
+  }
 };
 
 // Up to 8 * 8192 tokens: the first cluster sorts them in its blocks' shared memory, the other blocks
-// write the table gradient's zeros meanwhile.
-__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(
-    const int32_t* __restrict__ indices, int tokens, uint32_t vocab, int passes, int bits, uint32_t* __restrict__ sorted_keys,
-    uint32_t* __restrict__ sorted_tokens, float* __restrict__ dtable, int64_t values) {
+// write the table gradient's zeros meanwhile.  `share`: keys a block, a multiple of 1024.
+__global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const int32_t* __restrict__ indices, int tokens,
+                                                                        int share, uint32_t vocab, int passes, int bits,
+                                                                        uint2* __restrict__ sorted,
+                                                                        float* __restrict__ dtable, int64_t values) {
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = (int)cluster.num_blocks();
   pdl_launch_dependents();  // the sums wait for this kernel's end before they read
   if ((int)blockIdx.x >= blocks) {
-    const int64_t stride = (int64_t)(gridDim.x - blocks) * kSortThreads;
-    const int64_t first = (int64_t)(blockIdx.x - blocks) * kSortThreads + threadIdx.x;
-    float4* quads = reinterpret_cast<float4*>(dtable);
-    for (int64_t i = first; i < values / 4; i += stride) quads[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    // a piece of kZeroQuads float4 each, and out: blocks that stayed for a fixed share of the table made the
+    // clusters that do not fit at first double the kernel's time (32000 x 768 with 16384 tokens: 26 us)
+    const int64_t first = (int64_t)(blockIdx.x - blocks) * kZeroQuads + threadIdx.x, quads = values / 4;
+    float4* table = reinterpret_cast<float4*>(dtable);
+#pragma unroll
+    for (int i = 0; i < kZeroQuads / kSortThreads; i++)
+      if (first + i * kSortThreads < quads) table[first + i * kSortThreads] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (first < (values & 3)) dtable[(values & ~3ll) + first] = 0.f;
     return;
   }
   extern __shared__ __align__(16) uint8_t raw[];
-  SortShared& s = *reinterpret_cast<SortShared*>(raw);
-  const int rank = (int)cluster.block_rank();
-  const int share = ((tokens + blocks - 1) / blocks + kSortThreads - 1) / kSortThreads * kSortThreads;
-  const int n = max(0, min(share, tokens - rank * share));
   const int bins = 1 << bits;
+  SortView s(raw, share, 2, bins);
+  const int rank = (int)cluster.block_rank();
+  const int n = max(0, min(share, tokens - rank * share));
   for (int i = threadIdx.x; i < n; i += kSortThreads) {
     const int32_t v = indices[rank * share + i];
-    s.keys[0][i] = (uint32_t)v < vocab ? (uint32_t)v : vocab;
-    s.tokens[0][i] = (uint32_t)(rank * share + i);
+    s.pairs[0][i] = make_uint2((uint32_t)v < vocab ? (uint32_t)v : vocab, (uint32_t)(rank * share + i));
   }
   const int per_warp = share / kSortWarps, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int pass = 0; pass < passes; pass++) {
@@ -192,7 +207,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(
     for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(s.counts)[i] = 0;
     __syncthreads();
     uint32_t digit[kKeysPerThread], place[kKeysPerThread];
-    rank_keys(s.keys[from], n, per_warp, shift, bins, s.counts, digit, place);
+    rank_keys(s.pairs[from], n, per_warp, shift, bins, s.counts, digit, place);
     __syncthreads();
     const uint32_t total = prefix_over_warps(s.counts, bins);
     if ((int)threadIdx.x < bins) s.totals[threadIdx.x] = total;
@@ -217,16 +232,13 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(
 #pragma unroll
     for (int i = 0; i < kKeysPerThread; i++) {
       if (digit[i] == ~0u) continue;
-      const int at = warp * per_warp + i * 32 + lane;
-      const uint32_t key = s.keys[from][at], token = s.tokens[from][at];
+      const uint2 pair = s.pairs[from][warp * per_warp + i * 32 + lane];
       const int g = (int)(s.base[digit[i]] + s.counts[warp * bins + digit[i]] + place[i]);
       if (last) {
-        sorted_keys[g] = key;
-        sorted_tokens[g] = token;
+        sorted[g] = pair;
       } else {
-        const int to = g / share, slot = g - to * share;
-        cluster.map_shared_rank(s.keys[from ^ 1], to)[slot] = key;
-        cluster.map_shared_rank(s.tokens[from ^ 1], to)[slot] = token;
+        const int to = g / share;
+        cluster.map_shared_rank(s.pairs[from ^ 1], to)[g - to * share] = pair;
       }
     }
     if (!last) cluster.sync();  // the pass's writes have arrived; nobody reads this block's totals any more
@@ -234,39 +246,50 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(
   asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// More tokens: three launches a pass, over tiles of 8192 keys.
-__device__ __forceinline__ int load_tile(const int32_t* indices, const uint32_t* keys_in, const uint32_t* tokens_in,
-                                         int64_t tokens, uint32_t vocab, SortShared& s) {
-  const int64_t first = (int64_t)blockIdx.x * kSortKeys;
-  const int n = (int)(tokens - first < kSortKeys ? tokens - first : kSortKeys);
+// More tokens: three launches a pass, over tiles of `share` keys.
+__device__ __forceinline__ int load_tile(const int32_t* indices, const uint2* in, int64_t tokens, int share, uint32_t vocab,
+                                         uint2* pairs) {
+  const int64_t first = (int64_t)blockIdx.x * share;
+  const int n = (int)(tokens - first < share ? tokens - first : share);
   for (int i = threadIdx.x; i < n; i += kSortThreads) {
     if (indices) {
       const int32_t v = indices[first + i];
-      s.keys[0][i] = (uint32_t)v < vocab ? (uint32_t)v : vocab;
-      s.tokens[0][i] = (uint32_t)(first + i);
+      pairs[i] = make_uint2((uint32_t)v < vocab ? (uint32_t)v : vocab, (uint32_t)(first + i));
     } else {
-      s.keys[0][i] = keys_in[first + i];
-      s.tokens[0][i] = tokens_in[first + i];
+      pairs[i] = in[first + i];
     }
   }
   return n;
 }
-// counts[digit][tile]
-__global__ void __launch_bounds__(kSortThreads, 1) embedding_count_kernel(const int32_t* indices, const uint32_t* keys_in,
-                                                                         const uint32_t* tokens_in, int64_t tokens,
-                                                                         uint32_t vocab, int shift, int bits,
-                                                                         uint32_t* counts) {
+// PLACE false: counts[digit][tile]; true: the keys to their places, from the counts' exclusive sum.
+template <bool PLACE>
+__global__ void __launch_bounds__(kSortThreads, 1) embedding_tile_kernel(const int32_t* __restrict__ indices,
+                                                                        const uint2* __restrict__ in, int64_t tokens,
+                                                                        int share, uint32_t vocab, int shift, int bits,
+                                                                        uint32_t* __restrict__ counts,
+                                                                        uint2* __restrict__ out) {
   extern __shared__ __align__(16) uint8_t raw[];
-  SortShared& s = *reinterpret_cast<SortShared*>(raw);
   const int bins = 1 << bits;
+  SortView s(raw, share, 1, bins);
   for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(s.counts)[i] = 0;
-  const int n = load_tile(indices, keys_in, tokens_in, tokens, vocab, s);
+  const int n = load_tile(indices, in, tokens, share, vocab, s.pairs[0]);
   __syncthreads();
   uint32_t digit[kKeysPerThread], place[kKeysPerThread];
-  rank_keys(s.keys[0], n, kSortKeys / kSortWarps, shift, bins, s.counts, digit, place);
+  const int per_warp = share / kSortWarps, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  rank_keys(s.pairs[0], n, per_warp, shift, bins, s.counts, digit, place);
   __syncthreads();
   const uint32_t total = prefix_over_warps(s.counts, bins);
-  if ((int)threadIdx.x < bins) counts[(int64_t)threadIdx.x * gridDim.x + blockIdx.x] = total;
+  uint32_t* count = counts + (int64_t)threadIdx.x * gridDim.x + blockIdx.x;
+  if (!PLACE) {
+    if ((int)threadIdx.x < bins) *count = total;
+    return;
+  }
+  if ((int)threadIdx.x < bins) s.base[threadIdx.x] = *count;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kKeysPerThread; i++)
+    if (digit[i] != ~0u)
+      out[s.base[digit[i]] + s.counts[warp * bins + digit[i]] + place[i]] = s.pairs[0][warp * per_warp + i * 32 + lane];
 }
 // Exclusive sum in place, by one block.
 __global__ void __launch_bounds__(kSortThreads, 1) embedding_scan_kernel(uint32_t* counts, int64_t n) {
@@ -284,44 +307,17 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_scan_kernel(uint32_
     __syncthreads();
   }
 }
-__global__ void __launch_bounds__(kSortThreads, 1) embedding_scatter_kernel(
-    const int32_t* indices, const uint32_t* keys_in, const uint32_t* tokens_in, int64_t tokens, uint32_t vocab, int shift,
-    int bits, const uint32_t* counts, uint32_t* keys_out, uint32_t* tokens_out) {
-  extern __shared__ __align__(16) uint8_t raw[];
-  SortShared& s = *reinterpret_cast<SortShared*>(raw);
-  const int bins = 1 << bits;
-  for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t*>(s.counts)[i] = 0;
-  const int n = load_tile(indices, keys_in, tokens_in, tokens, vocab, s);
-  __syncthreads();
-  uint32_t digit[kKeysPerThread], place[kKeysPerThread];
-  rank_keys(s.keys[0], n, kSortKeys / kSortWarps, shift, bins, s.counts, digit, place);
-  __syncthreads();
-  prefix_over_warps(s.counts, bins);
-  if ((int)threadIdx.x < bins) s.base[threadIdx.x] = counts[(int64_t)threadIdx.x * gridDim.x + blockIdx.x];
-  __syncthreads();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-#pragma unroll
-  for (int i = 0; i < kKeysPerThread; i++) {
-    if (digit[i] == ~0u) continue;
-    const int at = warp * (kSortKeys / kSortWarps) + i * 32 + lane;
-    const uint32_t g = s.base[digit[i]] + s.counts[warp * bins + digit[i]] + place[i];
-    keys_out[g] = s.keys[0][at];
-    tokens_out[g] = s.tokens[0][at];
-  }
-}
 
 // ---- gradient: sums over the sorted tokens -----------------------------------------------------------------
-// A warp takes 16 sorted tokens and 32 V columns.  A table row whose tokens all lie in this chunk is
+// A warp takes CH sorted tokens (16 or 32) and 32 V columns.  A table row whose tokens all lie in this chunk is
 // finished here.  One that began in an earlier chunk leaves this chunk's share in partial[chunk][0], one
 // that begins here and goes on in partial[chunk][1].
-constexpr int kChunk = 16;
 constexpr int kBatch = 4;  // rows of dy in flight a warp
 constexpr int kSumThreads = 128;
 
-template <typename TD, int V>
+template <typename TD, int V, int CH>
 __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const TD* __restrict__ dy,
-                                                                const uint32_t* __restrict__ keys,
-                                                                const uint32_t* __restrict__ order,
+                                                                const uint2* __restrict__ sorted,
                                                                 float* __restrict__ dtable, float* __restrict__ partial,
                                                                 int64_t tokens, uint32_t vocab, int64_t width, float scale,
                                                                 int64_t tiles, int64_t items) {
@@ -331,19 +327,19 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const TD* __
   pdl_wait();
   if (item >= items) return;
   const int64_t chunk = item / tiles, col = ((item - chunk * tiles) * 32 + lane) * V;
-  const int64_t p0 = chunk * kChunk;
-  const bool held = lane < kChunk && p0 + lane < tokens;
-  const uint32_t key = held ? keys[p0 + lane] : vocab;
-  const uint32_t token = held ? order[p0 + lane] : 0;
+  const int64_t p0 = chunk * CH;
+  const bool held = lane < CH && p0 + lane < tokens;
+  const uint2 pair = held ? sorted[p0 + lane] : make_uint2(vocab, 0);
+  const uint32_t key = pair.x, token = pair.y;
   uint32_t edge = vocab;  // lane 0: the key before the chunk, lane 1: the key behind it
-  if (lane == 0 && p0 > 0) edge = keys[p0 - 1];
-  if (lane == 1 && p0 + kChunk < tokens) edge = keys[p0 + kChunk];
+  if (lane == 0 && p0 > 0) edge = sorted[p0 - 1].x;
+  if (lane == 1 && p0 + CH < tokens) edge = sorted[p0 + CH].x;
   const uint32_t before = p0 > 0 ? __shfl_sync(0xffffffffu, edge, 0) : 0xffffffffu;
   const uint32_t behind = __shfl_sync(0xffffffffu, edge, 1);
   const uint32_t next = __shfl_down_sync(0xffffffffu, key, 1);
   const uint32_t first_key = __shfl_sync(0xffffffffu, key, 0);
   const int n = __popc(__ballot_sync(0xffffffffu, key < vocab));  // keys ascend: the real ones come first
-  const uint32_t ends = __ballot_sync(0xffffffffu, key != next || lane == kChunk - 1);
+  const uint32_t ends = __ballot_sync(0xffffffffu, key != next || lane == CH - 1);
   const bool column = col < width;
   float acc[V];
 #pragma unroll
@@ -369,7 +365,7 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const TD* __
       if (!(ends >> at & 1)) continue;
       const uint32_t row = __shfl_sync(0xffffffffu, key, at);
       const bool came = row == first_key && row == before;
-      const bool goes = at == kChunk - 1 && row == behind;
+      const bool goes = at == CH - 1 && row == behind;
       if (column) {
         if (came || goes) {
           store_vec<V>(partial + (chunk * 2 + (came ? 0 : 1)) * width + col, acc);
@@ -400,8 +396,8 @@ __device__ __forceinline__ void add_shares(const float* partial, int64_t lo, int
     for (int k = 0; k < V; k++) acc[k] += v[k];
   }
 }
-template <int V>
-__global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t* __restrict__ keys,
+template <int V, int CH>
+__global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint2* __restrict__ sorted,
                                                                  const float* __restrict__ partial,
                                                                  float* __restrict__ dtable, int64_t tokens,
                                                                  uint32_t vocab, int64_t width, float scale,
@@ -409,14 +405,14 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t
   __shared__ __align__(16) float join[kJoinWarps][32 * V];
   __shared__ uint32_t long_row[kJoinWarps];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t first = (int64_t)blockIdx.x * kJoinWarps, chunk = first + warp, end = (chunk + 1) * kChunk;
+  const int64_t first = (int64_t)blockIdx.x * kJoinWarps, chunk = first + warp, end = (chunk + 1) * CH;
   pdl_wait();
   uint32_t row = vocab, behind = vocab, before = vocab, head = vocab;
   if (end < tokens) {
-    row = keys[end - 1];
-    behind = keys[end];
-    if (chunk > 0) before = keys[end - kChunk - 1];
-    if (chunk + 1 + lane < chunks) head = keys[(chunk + 1 + lane) * kChunk];
+    row = sorted[end - 1].x;
+    behind = sorted[end].x;
+    if (chunk > 0) before = sorted[end - CH - 1].x;
+    if (chunk + 1 + lane < chunks) head = sorted[(chunk + 1 + lane) * CH].x;
   }
   const bool mine = row < vocab && behind == row && before != row;
   const int more = mine ? __popc(__ballot_sync(0xffffffffu, head == row)) : 0;  // heads ascend: a run of ones
@@ -439,7 +435,7 @@ __global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint32_t
     int64_t run = 0;
     for (;;) {
       const int64_t c = first + w + 1 + run + threadIdx.x;
-      const int hit = __syncthreads_count(c < chunks && keys[c * kChunk] == long_key);
+      const int hit = __syncthreads_count(c < chunks && sorted[c * CH].x == long_key);
       run += hit;
       if (hit < kThreads) break;
     }
@@ -517,23 +513,20 @@ struct GradientArgs {
   float scale;
 };
 
-// Sorted keys and tokens in `work` (4 arrays of `tokens`, the counts behind them); *keys and *order
-// point at the sorted ones.  Writes dtable's zeros too.
-int sort_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, uint32_t* work, int64_t tiles, const uint32_t** keys,
-                const uint32_t** order) {
+// Sorts the (table row, token) pairs into *sorted, one of `buffers`, and writes dtable's zeros.  `counts`:
+// 512 for each tile of `share` keys, where there are more than 8 blocks can hold.
+int sort_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, uint2* const* buffers, uint32_t* counts, int share, int64_t tiles,
+                const uint2** sorted) {
   const Digits d = digits_of(a.vocab);
-  const int smem = (int)sizeof(SortShared);
-  uint32_t* k[2] = {work, work + 2 * a.tokens};
-  uint32_t* t[2] = {work + a.tokens, work + 3 * a.tokens};
-  if (tiles <= 8) {
-    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    // 1024 keys a block and more: below that a block's passes cost more than they share out
-    int blocks = 1;
-    while (blocks < 8 && blocks * 1024 < a.tokens) blocks *= 2;
-    const int64_t zero_blocks = ceil_div64(a.vocab * a.width, 4 * kSortThreads);
-    int64_t grid = blocks + ceil_div64(zero_blocks, blocks) * blocks;
-    const int64_t cap = (int64_t)ctx->sm_count / blocks * blocks;
-    if (grid > cap) grid = cap;
+  const int bins = 1 << d.bits;
+  if (!counts) {
+    const int blocks = (int)tiles;
+    const int smem = (int)SortView::bytes(share, 2, bins);
+    if (smem > 48 * 1024)
+      TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    const int64_t zero_blocks = ceil_div64(a.vocab * a.width, 4 * kZeroQuads);
+    const int64_t grid = blocks + ceil_div64(zero_blocks, blocks) * blocks;
+    TFJS_REQUIRE(ctx, grid < (1ll << 31), "embeddingLookupBackprop: the table is too large");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)grid);
     cfg.blockDim = dim3(kSortThreads);
@@ -545,61 +538,79 @@ int sort_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, uint32_t* work, int64
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    TFJS_CHECK_CUDA(ctx, cudaLaunchKernelEx(&cfg, embedding_sort_kernel, a.indices, (int)a.tokens, (uint32_t)a.vocab,
-                                            d.passes, d.bits, k[0], t[0], a.dtable, a.vocab * a.width));
-    *keys = k[0];
-    *order = t[0];
+    TFJS_CHECK_CUDA(ctx, cudaLaunchKernelEx(&cfg, embedding_sort_kernel, a.indices, (int)a.tokens, share, (uint32_t)a.vocab,
+                                            d.passes, d.bits, buffers[0], a.dtable, a.vocab * a.width));
+    *sorted = buffers[0];
     return post_launch(ctx, "embeddingLookupBackprop (sort)");
   }
-  TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(embedding_count_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(embedding_scatter_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int smem = (int)SortView::bytes(share, 1, bins);
+  auto count = embedding_tile_kernel<false>, place = embedding_tile_kernel<true>;
+  if (smem > 48 * 1024) {
+    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(count, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  }
   TFJS_CHECK_CUDA(ctx, cudaMemsetAsync(a.dtable, 0, (size_t)(a.vocab * a.width) * 4, ctx->stream));
-  uint32_t* counts = work + 4 * a.tokens;
   for (int pass = 0; pass < d.passes; pass++) {
-    const int32_t* idx = pass == 0 ? a.indices : nullptr;
-    const int from = (pass + 1) & 1, to = pass & 1, shift = pass * d.bits;
+    const int32_t* indices = pass == 0 ? a.indices : nullptr;
+    const uint2* in = buffers[(pass + 1) & 1];
+    uint2* out = buffers[pass & 1];
     int rc;
-    embedding_count_kernel<<<(unsigned)tiles, kSortThreads, smem, ctx->stream>>>(idx, k[from], t[from], a.tokens,
-                                                                                 (uint32_t)a.vocab, shift, d.bits, counts);
+    count<<<(unsigned)tiles, kSortThreads, smem, ctx->stream>>>(indices, in, a.tokens, share, (uint32_t)a.vocab,
+                                                                pass * d.bits, d.bits, counts, nullptr);
     if ((rc = post_launch(ctx, "embeddingLookupBackprop (count)"))) return rc;
     embedding_scan_kernel<<<1, kSortThreads, 0, ctx->stream>>>(counts, tiles << d.bits);
     if ((rc = post_launch(ctx, "embeddingLookupBackprop (scan)"))) return rc;
-    embedding_scatter_kernel<<<(unsigned)tiles, kSortThreads, smem, ctx->stream>>>(
-        idx, k[from], t[from], a.tokens, (uint32_t)a.vocab, shift, d.bits, counts, k[to], t[to]);
-    if ((rc = post_launch(ctx, "embeddingLookupBackprop (scatter)"))) return rc;
-    *keys = k[to];
-    *order = t[to];
+    place<<<(unsigned)tiles, kSortThreads, smem, ctx->stream>>>(indices, in, a.tokens, share, (uint32_t)a.vocab,
+                                                                pass * d.bits, d.bits, counts, out);
+    if ((rc = post_launch(ctx, "embeddingLookupBackprop (place)"))) return rc;
+    *sorted = out;
   }
   return TFJS_CUDA_OK;
 }
 
-template <typename TD, int V>
-int sum_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, const uint32_t* keys, const uint32_t* order, float* partial) {
-  const int64_t chunks = ceil_div64(a.tokens, kChunk), tiles = ceil_div64(a.width, 32 * V), items = chunks * tiles;
-  TFJS_REQUIRE(ctx, items < (1ll << 33), "embeddingLookupBackprop: too many tokens times columns");
-  launch_dependent(ctx, embedding_sum_kernel<TD, V>, dim3((unsigned)ceil_div64(items, kSumThreads / 32)), dim3(kSumThreads),
-                   (const TD*)a.dy, keys, order, a.dtable, partial, a.tokens, (uint32_t)a.vocab, a.width, a.scale, tiles,
-                   items);
+template <typename TD, int V, int CH>
+int sum_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, const uint2* sorted, float* partial) {
+  const int64_t chunks = ceil_div64(a.tokens, CH), tiles = ceil_div64(a.width, 32 * V), items = chunks * tiles;
+  TFJS_REQUIRE(ctx, items < (1ll << 32), "embeddingLookupBackprop: too many tokens times columns");
+  launch_dependent(ctx, embedding_sum_kernel<TD, V, CH>, dim3((unsigned)ceil_div64(items, kSumThreads / 32)), dim3(kSumThreads),
+                   (const TD*)a.dy, sorted, a.dtable, partial, a.tokens, (uint32_t)a.vocab, a.width, a.scale, tiles, items);
   const int rc = post_launch(ctx, "embeddingLookupBackprop (sum)");
   if (rc || chunks < 2) return rc;
-  launch_dependent(ctx, embedding_join_kernel<V>, dim3((unsigned)ceil_div64(chunks - 1, kJoinWarps), (unsigned)(tiles < 64 ? tiles : 64)),
-                   dim3(kThreads), keys, (const float*)partial, a.dtable, a.tokens, (uint32_t)a.vocab, a.width, a.scale, chunks);
+  launch_dependent(ctx, embedding_join_kernel<V, CH>, dim3((unsigned)ceil_div64(chunks - 1, kJoinWarps), (unsigned)(tiles < 64 ? tiles : 64)),
+                   dim3(kThreads), sorted, (const float*)partial, a.dtable, a.tokens, (uint32_t)a.vocab, a.width, a.scale, chunks);
   return post_launch(ctx, "embeddingLookupBackprop (join)");
 }
 
 template <typename TD>
 int launch_gradient(tfjs_cuda_ctx* ctx, const GradientArgs& a) {
-  const int64_t tiles = ceil_div64(a.tokens, kSortKeys), chunks = ceil_div64(a.tokens, kChunk);
-  // sorted pairs (twice where the passes go through global memory), counts, partial sums
-  const int64_t words = 4 * a.tokens + (tiles > 8 ? tiles * kMaxBins : 0), at = (words + 3) / 4 * 4;
-  void* work;
+  // one cluster, 1024 keys a block and more (below that a block's passes cost more than they share out), or
+  // tiles of 2048 keys, of 8192 where there are so many that their counts would grow past the keys
+  const bool cluster = a.tokens <= 8 * kSortKeys;
+  int64_t tiles = 1;
+  int share = a.tokens > (1 << 20) ? kSortKeys : 2048;
+  if (cluster) {
+    while (tiles < 8 && tiles * 1024 < a.tokens) tiles *= 2;
+    share = (int)ceil_div64(ceil_div64(a.tokens, tiles), kSortThreads) * kSortThreads;
+  } else {
+    tiles = ceil_div64(a.tokens, share);
+  }
+  const bool long_chunks = a.tokens >= 32768;  // fewer shares to join, once 16 tokens a warp fill the SMs twice over
+  const int64_t chunks = ceil_div64(a.tokens, long_chunks ? 32 : 16);
+  const size_t pair_bytes = (size_t)(a.tokens + 1) / 2 * 16, partial_bytes = (size_t)(chunks * 2 * a.width) * 4;
+  const size_t count_bytes = cluster ? 0 : (size_t)tiles * kMaxBins * 4;
+  uint8_t* work;
   size_t cap;
-  int rc = ctx_alloc(ctx, (size_t)(at + chunks * 2 * a.width) * 4, &work, &cap);
+  int rc = ctx_alloc(ctx, (cluster ? 1 : 2) * pair_bytes + count_bytes + partial_bytes + 16, (void**)&work, &cap);
   if (rc) return rc;
-  const uint32_t *keys, *order;
-  rc = sort_tokens(ctx, a, (uint32_t*)work, tiles, &keys, &order);
-  float* partial = (float*)work + at;
-  if (!rc) rc = a.width % 4 == 0 ? sum_tokens<TD, 4>(ctx, a, keys, order, partial) : sum_tokens<TD, 1>(ctx, a, keys, order, partial);
+  uint2* buffers[2] = {(uint2*)work, (uint2*)(work + pair_bytes)};
+  uint8_t* behind = work + (cluster ? 1 : 2) * pair_bytes;
+  const uint2* sorted;
+  rc = sort_tokens(ctx, a, buffers, cluster ? nullptr : (uint32_t*)behind, share, tiles, &sorted);
+  float* partial = (float*)(behind + count_bytes);
+  if (!rc) {
+    if (a.width % 4 == 0) rc = long_chunks ? sum_tokens<TD, 4, 32>(ctx, a, sorted, partial) : sum_tokens<TD, 4, 16>(ctx, a, sorted, partial);
+    else rc = long_chunks ? sum_tokens<TD, 1, 32>(ctx, a, sorted, partial) : sum_tokens<TD, 1, 16>(ctx, a, sorted, partial);
+  }
   ctx_free(ctx, work, cap);
   return rc;
 }

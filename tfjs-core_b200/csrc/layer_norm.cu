@@ -9,14 +9,15 @@
 //
 // Forward.  A row is read once and stays on chip: the mean and then the centred square sum (which
 // does not cancel, unlike E[x^2] - m^2) come from the same registers.  Three forms by width:
-//   up to 1024     L lanes a row (4 .. 32), no shared memory
+//   up to 1024     L lanes a row (4 .. 32), no shared memory; where rows start off the 16-byte
+//                  boundaries (then up to 2046 halves), a warp with a ring of rows in shared memory
 //   up to 16384    one block a row
-//   above          a cluster of 8 blocks a row, the row in their shared memory, sums joined over DSMEM
+//   above          a cluster of 1 to 8 blocks a row, the row in their shared memory, sums joined over DSMEM
 // Gradient.  One pass over dy and x gives dx and, per block, the weights' gradients:
 //   up to 8192     persistent blocks; a ring of stages (several rows each) filled by cp.async.  First
 //                  the lanes of a row sum a and a n, then every thread takes the same columns of every
 //                  row: it writes dx and keeps its columns' dg, db in registers.
-//   above          a cluster of 8 blocks a row; dg, db accumulate in a buffer of the cluster's own
+//   above          a cluster of 1 to 8 blocks a row; dg, db add up in the blocks' shared memory
 // and a second kernel adds the blocks' partial dg, db in order.
 #include <cooperative_groups.h>
 
@@ -127,6 +128,138 @@ __global__ void __launch_bounds__(256) layer_norm_lanes_kernel(const TX* __restr
   if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
 }
 
+__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_async8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// The whole 16-byte units that [first, first + bytes) touches, into shared memory, by LANES threads.  The units lie
+// within the tensor's buffer: its start is 16-byte aligned and its size class a multiple of 16.
+template <int LANES>
+__device__ __forceinline__ void stage_copy(uint8_t* dst, const uint8_t* base, int64_t first, int bytes) {
+  const int off = (int)(first & 15), units = (off + bytes + 15) >> 4;
+  const uint8_t* src = base + (first - off);
+#pragma unroll 4
+  for (int i = threadIdx.x & (LANES - 1); i < units; i += LANES) copy_async16(dst + i * 16, src + i * 16);
+}
+
+// Rows that do not start on 16-byte boundaries.  A warp has a ring of two row slots in shared memory that
+// cp.async fills with the row's 16-byte units, so the loads are wide whatever the row's offset; it takes the
+// row from there into registers as 4-byte words, NW a lane (P values each: two halves or one float), and
+// needs no barrier but its own.  Where halves start at an odd place, the first word (and maybe the last)
+// holds one value of the neighbouring row, which is left out.  gamma and beta lie beside each other in
+// shared memory in the words' order, once for even and once for odd rows.
+// (One value a load in place of this: 33000 x 1001 half 93 us.)
+constexpr int kRingWarps = 8;
+template <typename TX, typename TY, int NW>
+__global__ void __launch_bounds__(kRingWarps * 32) layer_norm_ring_kernel(const TX* __restrict__ x,
+                                                                         const float* __restrict__ gamma,
+                                                                         const float* __restrict__ beta, TY* __restrict__ y,
+                                                                         float* __restrict__ stats, int64_t rows, int width,
+                                                                         float epsilon, int slot_bytes) {
+  constexpr int P = 4 / (int)sizeof(TX);
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint8_t* ring = smem + warp * 2 * slot_bytes;
+  const int most = width / P + 1;  // words of a row, at most
+  float* weights = reinterpret_cast<float*>(smem + kRingWarps * 2 * slot_bytes);  // [odd][most][2 P]: P of gamma, P of beta
+  const int64_t step = (int64_t)gridDim.x * kRingWarps, first = (int64_t)blockIdx.x * kRingWarps + warp;
+  auto fill = [&](int64_t row, int slot) {
+    if (row < rows)
+      stage_copy<32>(ring + slot * slot_bytes, (const uint8_t*)x, row * width * (int64_t)sizeof(TX), width * (int)sizeof(TX));
+    copy_commit();
+  };
+  fill(first, 0);
+  for (int j = threadIdx.x; j < P * most * P; j += kRingWarps * 32) {
+    const int odd = j / (most * P), e = j - odd * most * P, col = e - odd;
+    float* w = weights + (odd * most + e / P) * 2 * P + e % P;
+    const bool there = col >= 0 && col < width;
+    w[0] = gamma && there ? gamma[col] : 1.f;
+    w[P] = beta && there ? beta[col] : 0.f;
+  }
+  __syncthreads();
+  const float inv = 1.f / (float)width;
+  int slot = 0;
+  for (int64_t row = first; row < rows; row += step, slot ^= 1) {
+    fill(row + step, slot ^ 1);
+    copy_wait<1>();
+    __syncwarp();  // the row is there for all lanes
+    const int64_t at = row * width;
+    const int odd = (int)(at & (P - 1)), words = (odd + width + P - 1) / P;
+    const TX* r = reinterpret_cast<const TX*>(ring + slot * slot_bytes + ((at * (int64_t)sizeof(TX)) & 15)) - odd;
+    const bool cut = P == 2 && ((odd + width) & 1);  // the last word's second value is the next row's
+    uint32_t q[NW];
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      const int w = lane + 32 * i;
+      q[i] = w < words ? *reinterpret_cast<const uint32_t*>(r + w * P) : 0u;
+      if (P == 2) {
+        if (w == 0 && odd) q[i] &= 0xffff0000u;
+        if (w == words - 1 && cut) q[i] &= 0x0000ffffu;
+      }
+    }
+    __syncwarp();  // read by all lanes: the slot may be filled again
+    const TX* none = nullptr;
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      float v[P];
+      unpack_word(q[i], none, v);
+#pragma unroll
+      for (int k = 0; k < P; k++) s += v[k];
+    }
+    const float mean = lanes_sum<32>(s) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      const int w = lane + 32 * i;
+      if (w >= words) break;
+      float v[P];
+      unpack_word(q[i], none, v);
+#pragma unroll
+      for (int k = 0; k < P; k++) {
+        float d = v[k] - mean;
+        if (P == 2 && ((k == 0 && w == 0 && odd) || (k == 1 && w == words - 1 && cut))) d = 0.f;
+        s = fmaf(d, d, s);
+      }
+    }
+    const float rstd = 1.f / sqrtf(lanes_sum<32>(s) * inv + epsilon);
+    TY* out = y + at - odd;
+    const float* mine = weights + odd * most * 2 * P;
+#pragma unroll
+    for (int i = 0; i < NW; i++) {
+      const int w = lane + 32 * i;
+      if (w >= words) break;
+      float v[P], gb[2 * P];
+      unpack_word(q[i], none, v);
+      load_vec<2 * P>(mine + w * 2 * P, gb);
+#pragma unroll
+      for (int k = 0; k < P; k++) v[k] = fmaf((v[k] - mean) * rstd, gb[k], gb[P + k]);
+      const bool low = P == 2 && w == 0 && odd, high = P == 2 && w == words - 1 && cut;
+      if (!low && !high) {
+        store_vec<P>(out + w * P, v);
+      } else {
+        if (!low) {
+          const float o[1] = {v[0]};
+          store_vec<1>(out + w * P, o);
+        }
+        if (!high) {
+          const float o[1] = {v[P - 1]};
+          store_vec<1>(out + w * P + P - 1, o);
+        }
+      }
+    }
+    if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
+  }
+}
+
 // One block of NT threads a row: width <= NT * NV * V, a multiple of V.
 template <typename TX, typename TY, int V, int NV, int NT>
 __global__ void __launch_bounds__(NT) layer_norm_block_kernel(const TX* __restrict__ x, const float* __restrict__ gamma,
@@ -173,30 +306,25 @@ __global__ void __launch_bounds__(NT) layer_norm_block_kernel(const TX* __restri
   }
 }
 
-constexpr int kClusterBlocks = 8;
 constexpr int kClusterThreads = 512;
 
-// Sum over the cluster in the order of its blocks.  `mine` is this block's slot in its own shared
-// memory; two uses of the same slot must have another cluster-wide sum between them.
-__device__ __forceinline__ float2 cluster_sum(float a, float b, float2* slot, float* scratch) {
+// Sums of a and b over the cluster's C blocks, in their order.  `slot` is this block's place in its own
+// shared memory; two uses of the same slot must have another cluster-wide sum between them.
+__device__ __forceinline__ float2 cluster_sum(float a, float b, int C, float2* slot, float2* scratch) {
   cg::cluster_group cluster = cg::this_cluster();
   a = lanes_sum<32>(a);
   b = lanes_sum<32>(b);
-  if ((threadIdx.x & 31) == 0) {
-    scratch[2 * (threadIdx.x >> 5)] = a;
-    scratch[2 * (threadIdx.x >> 5) + 1] = b;
-  }
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = make_float2(a, b);
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const int w = threadIdx.x & (kClusterThreads / 32 - 1);
-    a = lanes_sum<kClusterThreads / 32>(scratch[2 * w]);
-    b = lanes_sum<kClusterThreads / 32>(scratch[2 * w + 1]);
-    if (threadIdx.x == 0) *slot = make_float2(a, b);
-  }
+  const float2 v = scratch[threadIdx.x & (kClusterThreads / 32 - 1)];
+  float2 t = make_float2(lanes_sum<kClusterThreads / 32>(v.x), lanes_sum<kClusterThreads / 32>(v.y));
+  if (C == 1) return t;
+  if (threadIdx.x == 0) *slot = t;
   cluster.sync();
-  float2 t = make_float2(0.f, 0.f);
+  t = make_float2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < kClusterBlocks; i++) {
+  for (int i = 0; i < 8; i++) {
+    if (i >= C) break;
     const float2 o = *cluster.map_shared_rank(slot, i);
     t.x += o.x;
     t.y += o.y;
@@ -204,35 +332,36 @@ __device__ __forceinline__ float2 cluster_sum(float a, float b, float2* slot, fl
   return t;
 }
 
-// A cluster of 8 blocks a row.  `cached`: the block's share of the row fits into its dynamic shared
+// A cluster of C blocks a row.  `cached`: the block's share of the row fits into its dynamic shared
 // memory and is read from there the second and third time, else from global memory (L2).
 template <typename TX, typename TY, int V>
 __global__ void __launch_bounds__(kClusterThreads) layer_norm_cluster_kernel(
     const TX* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, TY* __restrict__ y,
-    float* __restrict__ stats, int64_t rows, int64_t width, float epsilon, int cached) {
+    float* __restrict__ stats, int64_t rows, int64_t width, float epsilon, int C, int cached) {
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float scratch[2][2 * kClusterThreads / 32];
+  __shared__ float2 scratch[2][kClusterThreads / 32];
   __shared__ float2 slot[2];
   TX* kept = reinterpret_cast<TX*>(smem);
-  const int64_t vecs = width / V, clusters = gridDim.x / kClusterBlocks;
-  const int64_t rank = blockIdx.x % kClusterBlocks;
-  const int64_t lo = vecs * rank / kClusterBlocks, n = vecs * (rank + 1) / kClusterBlocks - lo;
-  for (int64_t row = blockIdx.x / kClusterBlocks; row < rows; row += clusters) {
+  const int64_t vecs = width / V, clusters = gridDim.x / C;
+  const int64_t rank = blockIdx.x % C;
+  const int64_t lo = vecs * rank / C;
+  const int n = (int)(vecs * (rank + 1) / C - lo);
+  for (int64_t row = blockIdx.x / C; row < rows; row += clusters) {
     const TX* r = x + row * width + lo * V;
     float s = 0.f;
 #pragma unroll 4
-    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+    for (int j = threadIdx.x; j < n; j += kClusterThreads) {
       float v[V];
       load_vec<V>(r + j * V, v);
       if (cached) store_vec<V>(kept + j * V, v);  // exact: the values came from this type
 #pragma unroll
       for (int k = 0; k < V; k++) s += v[k];
     }
-    const float mean = cluster_sum(s, 0.f, &slot[0], scratch[0]).x / (float)width;
+    const float mean = cluster_sum(s, 0.f, C, &slot[0], scratch[0]).x / (float)width;
     s = 0.f;
     const TX* from = cached ? kept : r;  // a thread reads back only what it wrote
 #pragma unroll 4
-    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+    for (int j = threadIdx.x; j < n; j += kClusterThreads) {
       float v[V];
       load_vec<V>(from + j * V, v);
 #pragma unroll
@@ -241,9 +370,9 @@ __global__ void __launch_bounds__(kClusterThreads) layer_norm_cluster_kernel(
         s = fmaf(d, d, s);
       }
     }
-    const float rstd = 1.f / sqrtf(cluster_sum(s, 0.f, &slot[1], scratch[1]).x / (float)width + epsilon);
+    const float rstd = 1.f / sqrtf(cluster_sum(s, 0.f, C, &slot[1], scratch[1]).x / (float)width + epsilon);
 #pragma unroll 2
-    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+    for (int j = threadIdx.x; j < n; j += kClusterThreads) {
       float v[V];
       load_vec<V>(from + j * V, v);
       finish_vec<V>(v, mean, rstd, gamma, beta, (lo + j) * V, y + row * width + (lo + j) * V);
@@ -258,18 +387,6 @@ constexpr int kStagedWidth = 8192;
 constexpr int kStagedThreads = 256;
 constexpr int kMaxStageRows = 256;
 
-__device__ __forceinline__ void copy_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_async8(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 struct StagedParams {
   const float* gamma;
   const float* stats;
@@ -279,15 +396,6 @@ struct StagedParams {
   int width, stage_rows;        // stage_rows: a power of two
   int x_bytes, stage_bytes;     // of the dy and the whole stage area
 };
-
-// The whole 16-byte units that [first, first + bytes) touches, into shared memory.  The units lie
-// within the tensor's buffer: its start is 16-byte aligned and its size class a multiple of 16.
-__device__ __forceinline__ void stage_copy(uint8_t* dst, const uint8_t* base, int64_t first, int bytes) {
-  const int off = (int)(first & 15), units = (off + bytes + 15) >> 4;
-  const uint8_t* src = base + (first - off);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < units; i += kStagedThreads) copy_async16(dst + i * 16, src + i * 16);
-}
 
 constexpr int kStages = 3;
 
@@ -325,8 +433,8 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
       const int64_t row = item * R;
       const int n = (int)(p.rows - row < R ? p.rows - row : R);
       uint8_t* dst = ring + slot * p.stage_bytes;
-      stage_copy(dst, (const uint8_t*)dy, row * width * (int64_t)sizeof(TD), n * width * (int)sizeof(TD));
-      stage_copy(dst + p.x_bytes, (const uint8_t*)x, row * width * (int64_t)sizeof(TX), n * width * (int)sizeof(TX));
+      stage_copy<kStagedThreads>(dst, (const uint8_t*)dy, row * width * (int64_t)sizeof(TD), n * width * (int)sizeof(TD));
+      stage_copy<kStagedThreads>(dst + p.x_bytes, (const uint8_t*)x, row * width * (int64_t)sizeof(TX), n * width * (int)sizeof(TX));
       float2* st = reinterpret_cast<float2*>(dst + p.stage_bytes) - R;
       if (tid < n) copy_async8(st + tid, p.stats + 2 * (row + tid));
     }
@@ -441,50 +549,85 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
   }
 }
 
-// ---- gradient, longer rows: a cluster of 8 blocks a row --------------------------------------------
-// The row is read twice (the second time from L2).  partial [clusters][2][width]: each thread adds
-// its own columns there, the first row of the cluster stores.
-template <typename TD, typename TX, int V>
-__global__ void __launch_bounds__(kClusterThreads) layer_norm_backprop_cluster_kernel(
-    const TD* __restrict__ dy, const TX* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ stats,
-    float* __restrict__ dx, float* __restrict__ partial, int64_t rows, int64_t width) {
-  __shared__ float scratch[2][2 * kClusterThreads / 32];
+// ---- gradient, longer rows: a cluster of C blocks a row --------------------------------------------
+// RING: the block's share of dy and x comes into shared memory by cp.async, the next row's while this one is
+// summed and written, and its columns' dg and db add up there over the cluster's rows; else both passes read
+// global memory (the second one L2), and partial [clusters][2][width] is where dg and db add up.  In both
+// a thread meets its own columns only, but for the copies, which the barriers of the sums order.
+struct ClusterParams {
+  const float *gamma, *stats;
+  float *dx, *partial;
+  int64_t rows, width;
+  int C, d_bytes, slot_bytes;  // RING: of the dy area of a slot, and of a slot
+};
+template <typename TD, typename TX, int V, bool RING>
+__global__ void __launch_bounds__(kClusterThreads, 2) layer_norm_backprop_cluster_kernel(const TD* __restrict__ dy,
+                                                                                        const TX* __restrict__ x,
+                                                                                        ClusterParams p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float2 scratch[2][kClusterThreads / 32];
   __shared__ float2 slot[2];
-  const int64_t vecs = width / V, clusters = gridDim.x / kClusterBlocks, cluster = blockIdx.x / kClusterBlocks;
-  const int64_t rank = blockIdx.x % kClusterBlocks;
-  const int64_t lo = vecs * rank / kClusterBlocks * V, n = vecs * (rank + 1) / kClusterBlocks - vecs * rank / kClusterBlocks;
-  float* pg = partial ? partial + cluster * 2 * width + lo : nullptr;
+  const int C = p.C, tid = threadIdx.x;
+  const int64_t width = p.width, vecs = width / V, clusters = gridDim.x / C, cluster = blockIdx.x / C;
+  const int64_t rank = blockIdx.x % C, lo = vecs * rank / C * V;
+  const int n = (int)(vecs * (rank + 1) / C - vecs * rank / C);
+  float* pg = p.partial ? p.partial + cluster * 2 * width + lo : nullptr;
+  float* pb = pg ? pg + width : nullptr;
+  const float* gamma = p.gamma ? p.gamma + lo : nullptr;
+  float* sg = reinterpret_cast<float*>(smem + 2 * p.slot_bytes);  // dg and db, V columns of each in turn
+  auto fill = [&](int64_t row, int at) {
+    if (row < p.rows) {
+      const int64_t first = row * width + lo;
+      uint8_t* dst = smem + at * p.slot_bytes;
+      stage_copy<kClusterThreads>(dst, (const uint8_t*)dy, first * (int64_t)sizeof(TD), n * V * (int)sizeof(TD));
+      stage_copy<kClusterThreads>(dst + p.d_bytes, (const uint8_t*)x, first * (int64_t)sizeof(TX), n * V * (int)sizeof(TX));
+    }
+    copy_commit();
+  };
+  if (RING) fill(cluster, 0);
   pdl_launch_dependents();  // the join kernel waits for this one's end before it reads
   int turn = 0;
-  for (int64_t row = cluster; row < rows; row += clusters, turn ^= 1) {
-    const TD* d0 = dy + row * width + lo;
-    const TX* x0 = x + row * width + lo;
-    const float2 mr = *reinterpret_cast<const float2*>(stats + 2 * row);
+  for (int64_t row = cluster; row < p.rows; row += clusters, turn ^= 1) {
+    const int64_t first = row * width + lo;
+    const TD* d0 = dy + first;
+    const TX* x0 = x + first;
+    if (RING) {
+      __syncthreads();  // all are done with the row before this one: its slot takes the next
+      fill(row + clusters, turn ^ 1);
+      copy_wait<1>();
+      __syncthreads();
+      const uint8_t* at = smem + turn * p.slot_bytes;
+      d0 = reinterpret_cast<const TD*>(at + ((first * (int64_t)sizeof(TD)) & 15));
+      x0 = reinterpret_cast<const TX*>(at + p.d_bytes + ((first * (int64_t)sizeof(TX)) & 15));
+    }
+    const float2 mr = *reinterpret_cast<const float2*>(p.stats + 2 * row);
     float sa = 0.f, sn = 0.f;
 #pragma unroll 4
-    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+    for (int j = tid; j < n; j += kClusterThreads) {
       float d[V], v[V], g[V];
       load_vec<V>(d0 + j * V, d);
       load_vec<V>(x0 + j * V, v);
-      if (gamma) load_vec<V>(gamma + lo + j * V, g);
+      if (gamma) load_vec<V>(gamma + j * V, g);
 #pragma unroll
       for (int k = 0; k < V; k++) {
         const float a = gamma ? d[k] * g[k] : d[k];
         sa += a;
-        sn = fmaf(a, (v[k] - mr.x) * mr.y, sn);
+        sn = fmaf(a, v[k] - mr.x, sn);
       }
     }
-    const float2 t = cluster_sum(sa, sn, &slot[turn], scratch[turn]);
-    const float ma = t.x / (float)width, man = t.y / (float)width;
+    const float2 t = cluster_sum(sa, sn, C, &slot[turn], scratch[turn]);
+    const float ma = t.x / (float)width, man = t.y * mr.y / (float)width;
+    const bool fresh = row == cluster;                     // nothing added up yet
+    const bool hand_over = !RING || row + clusters >= p.rows;  // the cluster's last row
 #pragma unroll 2
-    for (int64_t j = threadIdx.x; j < n; j += kClusterThreads) {
+    for (int j = tid; j < n; j += kClusterThreads) {
       float d[V], v[V], g[V], o[V], wg[V], wb[V];
       load_vec<V>(d0 + j * V, d);
       load_vec<V>(x0 + j * V, v);
-      if (gamma) load_vec<V>(gamma + lo + j * V, g);
-      if (pg && row != cluster) {
-        load_vec<V>(pg + j * V, wg);
-        load_vec<V>(pg + width + j * V, wb);
+      if (gamma) load_vec<V>(gamma + j * V, g);
+      if (pg && !fresh) {
+        load_vec<V>(RING ? sg + 2 * j * V : pg + j * V, wg);
+        load_vec<V>(RING ? sg + (2 * j + 1) * V : pb + j * V, wb);
       } else {
 #pragma unroll
         for (int k = 0; k < V; k++) wg[k] = wb[k] = 0.f;
@@ -492,41 +635,43 @@ __global__ void __launch_bounds__(kClusterThreads) layer_norm_backprop_cluster_k
 #pragma unroll
       for (int k = 0; k < V; k++) {
         const float nn = (v[k] - mr.x) * mr.y;
-        o[k] = mr.y * ((gamma ? d[k] * g[k] : d[k]) - ma - nn * man);
+        o[k] = mr.y * fmaf(-nn, man, (gamma ? d[k] * g[k] : d[k]) - ma);
         wg[k] = fmaf(d[k], nn, wg[k]);
         wb[k] += d[k];
       }
-      if (dx) store_vec<V>(dx + row * width + lo + j * V, o);
+      if (p.dx) store_vec<V>(p.dx + first + j * V, o);
       if (pg) {
-        store_vec<V>(pg + j * V, wg);
-        store_vec<V>(pg + width + j * V, wb);
+        store_vec<V>(hand_over ? pg + j * V : sg + 2 * j * V, wg);
+        store_vec<V>(hand_over ? pb + j * V : sg + (2 * j + 1) * V, wb);
       }
     }
   }
   cg::this_cluster().sync();
 }
 
-// out[j] = sum over the blocks, in order, of partial[block][j]: 32 columns a block, 8 threads a column
-// take every eighth block's row and join theirs in order.  j runs over dg and then db.
-__global__ void __launch_bounds__(256) layer_norm_join_kernel(const float* __restrict__ partial, float* __restrict__ dgamma,
-                                                             float* __restrict__ dbeta, int blocks, int64_t width) {
-  __shared__ float part[8][32];
+// out[j] = sum over the blocks of partial[block][j]: 32 columns a block, 32 threads a column take every
+// 32nd block's row and join theirs in order.  j runs over dg and then db.
+constexpr int kJoinThreads = 1024;
+__global__ void __launch_bounds__(kJoinThreads) layer_norm_join_kernel(const float* __restrict__ partial,
+                                                                      float* __restrict__ dgamma, float* __restrict__ dbeta,
+                                                                      int blocks, int64_t width) {
+  __shared__ float part[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   pdl_wait();
   for (int64_t j0 = (int64_t)blockIdx.x * 32; j0 < 2 * width; j0 += (int64_t)gridDim.x * 32) {
     const int64_t j = j0 + lane;
     float s = 0.f;
     if (j < 2 * width) {
-#pragma unroll 8
-      for (int b = w; b < blocks; b += 8) s += partial[(int64_t)b * 2 * width + j];
+#pragma unroll 10
+      for (int b = w; b < blocks; b += 32) s += partial[(int64_t)b * 2 * width + j];
     }
     part[w][lane] = s;
     __syncthreads();
-    if (w == 0 && j < 2 * width) {
-#pragma unroll
-      for (int i = 1; i < 8; i++) s += part[i][lane];
-      float* out = j < width ? dgamma : dbeta;
-      if (out) out[j < width ? j : j - width] = s;
+    s = lanes_sum<32>(part[lane][w]);  // warp w joins column w
+    const int64_t c = j0 + w;
+    if (lane == 0 && c < 2 * width) {
+      float* out = c < width ? dgamma : dbeta;
+      if (out) out[c < width ? c : c - width] = s;
     }
     __syncthreads();
   }
@@ -558,21 +703,21 @@ void block_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
       (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon);
 }
 
-// A launch of clusters of 8 blocks; `smem` bytes of dynamic shared memory a block.
+// A launch of clusters of C blocks; `smem` bytes of dynamic shared memory a block.
 template <typename... Params, typename... Args>
-cudaError_t launch_clusters(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), int64_t clusters, size_t smem, Args... args) {
+cudaError_t launch_clusters(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), int64_t clusters, int C, size_t smem, Args... args) {
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * kClusterBlocks));
+  cfg.gridDim = dim3((unsigned)(clusters * C));
   cfg.blockDim = dim3(kClusterThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = ctx->stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kClusterBlocks;
+  attr[0].val.clusterDim.x = C;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
@@ -581,12 +726,17 @@ cudaError_t launch_clusters(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), int64
 
 template <typename TX, typename TY, int V>
 int cluster_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
-  const int64_t share = (ceil_div64(a.width / V, kClusterBlocks) * V * (int64_t)sizeof(TX) + 15) / 16 * 16;
+  // Blocks a row: so many that three blocks' shares fit into an SM's shared memory (one loads while another
+  // sums), and with few rows so many that the SMs have a block each.  Every block costs each row two
+  // cluster-wide waits of about a microsecond: 1000 x 33000 is 137 us with 8 blocks a row.
+  const auto share_of = [&](int C) { return (ceil_div64(a.width / V, C) * V * (int64_t)sizeof(TX) + 15) / 16 * 16; };
+  int C = 1;
+  while (C < 8 && (share_of(C) > 72 * 1024 || a.rows * C < ctx->sm_count)) C *= 2;
+  const int64_t share = share_of(C), cap = 1 << 24;
   const bool cached = share <= 200 * 1024;
-  const int64_t cap = (int64_t)ctx->sm_count * 2 / kClusterBlocks;
-  TFJS_CHECK_CUDA(ctx, launch_clusters(ctx, layer_norm_cluster_kernel<TX, TY, V>, a.rows < cap ? a.rows : cap,
+  TFJS_CHECK_CUDA(ctx, launch_clusters(ctx, layer_norm_cluster_kernel<TX, TY, V>, a.rows < cap ? a.rows : cap, C,
                                        cached ? (size_t)share : 0, (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats,
-                                       a.rows, a.width, a.epsilon, cached ? 1 : 0));
+                                       a.rows, a.width, a.epsilon, C, cached ? 1 : 0));
   return post_launch(ctx, "layerNorm (clusters)");
 }
 
@@ -599,28 +749,47 @@ int forward_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
     if (w <= 4 * V) lanes_form<TX, TY, V, 1, 4>(ctx, a);
     else if (w <= 16 * V) lanes_form<TX, TY, V, 1, 16>(ctx, a);
     else if (w <= 64 * V) lanes_form<TX, TY, V, 2, 32>(ctx, a);
-    else if (w <= 128 * V) lanes_form<TX, TY, V, 4, 32>(ctx, a);
-    else if constexpr (V <= 4) {
-      if (w <= 256 * V) lanes_form<TX, TY, V, 8, 32>(ctx, a);
-      else if constexpr (V <= 2) {
-        if (w <= 512 * V) lanes_form<TX, TY, V, 16, 32>(ctx, a);
-        else if constexpr (V == 1) lanes_form<TX, TY, V, 32, 32>(ctx, a);
-      }
+    else if constexpr (V >= 4) {  // rows off the 16-byte boundaries come here up to 64 V columns only
+      if (w <= 128 * V) lanes_form<TX, TY, V, 4, 32>(ctx, a);
+      else if constexpr (V == 4) lanes_form<TX, TY, V, 8, 32>(ctx, a);
     }
     return post_launch(ctx, "layerNorm (lanes)");
   }
   constexpr int NV = 32 / V;  // 32 values a thread
-  if (w <= 256 * 8) block_form<TX, TY, V, NV / 4, 256>(ctx, a);
+  if (V >= 4 && w <= 256 * 8) block_form<TX, TY, V, V >= 4 ? NV / 4 : NV / 2, 256>(ctx, a);
   else if (w <= 256 * 16) block_form<TX, TY, V, NV / 2, 256>(ctx, a);
   else if (w <= 256 * 32) block_form<TX, TY, V, NV, 256>(ctx, a);
   else block_form<TX, TY, V, NV, 512>(ctx, a);
   return post_launch(ctx, "layerNorm (blocks)");
 }
 
+template <typename TX, typename TY, int NW>
+int ring_launch(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+  constexpr int P = 4 / (int)sizeof(TX);
+  const int slot_bytes = ((int)a.width * (int)sizeof(TX) + 31) / 16 * 16;  // one unit more for the row's own offset
+  const int smem = kRingWarps * 2 * slot_bytes + P * ((int)a.width / P + 1) * 2 * P * 4;
+  auto kernel = layer_norm_ring_kernel<TX, TY, NW>;
+  if (smem > 48 * 1024)
+    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  const int per_sm = smem <= 36 * 1024 ? 6 : smem <= 55 * 1024 ? 4 : smem <= 74 * 1024 ? 3 : 2;
+  kernel<<<grid_rows(ctx, ceil_div64(a.rows, kRingWarps), per_sm), kRingWarps * 32, smem, ctx->stream>>>(
+      (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon, slot_bytes);
+  return post_launch(ctx, "layerNorm (ring)");
+}
+// Words of a row that starts at an odd place: width / P + 1 at most.
+template <typename TX, typename TY>
+int ring_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+  const int64_t words = a.width / (4 / (int)sizeof(TX)) + 1;
+  if (words <= 256) return ring_launch<TX, TY, 8>(ctx, a);
+  if (words <= 512) return ring_launch<TX, TY, 16>(ctx, a);
+  return ring_launch<TX, TY, 32>(ctx, a);
+}
+
 template <typename TX, typename TY>
 int launch_forward(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;  // 16 bytes of the result
   if (a.width % W == 0) return forward_form<TX, TY, W>(ctx, a);
+  if (a.width > (a.width % 2 ? 64 : 128) && a.width / (4 / (int)sizeof(TX)) + 1 <= 1024) return ring_form<TX, TY>(ctx, a);
   if (a.width % 2 == 0) return forward_form<TX, TY, 2>(ctx, a);
   return forward_form<TX, TY, 1>(ctx, a);
 }
@@ -633,7 +802,7 @@ struct BackwardArgs {
 };
 
 int join(tfjs_cuda_ctx* ctx, const BackwardArgs& a, const float* partial, int blocks) {
-  launch_dependent(ctx, layer_norm_join_kernel, dim3(grid_rows(ctx, ceil_div64(2 * a.width, 32), 16)), dim3(256), partial,
+  launch_dependent(ctx, layer_norm_join_kernel, dim3(grid_rows(ctx, ceil_div64(2 * a.width, 32), 2)), dim3(kJoinThreads), partial,
                    a.dgamma, a.dbeta, blocks, a.width);
   return post_launch(ctx, "layerNormBackprop (join)");
 }
@@ -690,13 +859,32 @@ int staged_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
 
 template <typename TD, typename TX, int V>
 int backward_cluster_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
-  const int64_t cap = (int64_t)ctx->sm_count * 2 / kClusterBlocks, clusters = a.rows < cap ? a.rows : cap;
+  ClusterParams p = {a.gamma, a.stats, a.dx, nullptr, a.rows, a.width, 1, 0, 0};
+  const auto bytes_of = [&](int C) {
+    const int64_t share = ceil_div64(a.width / V, C) * V;
+    p.C = C;
+    p.d_bytes = (int)((share * (int64_t)sizeof(TD) + 31) / 16 * 16);  // one unit more for the row's own offset
+    p.slot_bytes = p.d_bytes + (int)((share * (int64_t)sizeof(TX) + 31) / 16 * 16);
+    return 2 * (int64_t)p.slot_bytes + share * 8;
+  };
+  // as for the forward pass: two blocks an SM, and with few rows a block for every SM
+  int C = 1;
+  int64_t smem = a.width < (1 << 22) ? bytes_of(C) : INT64_MAX;
+  while (C < 8 && (smem > 112 * 1024 || a.rows * C < ctx->sm_count)) {
+    C *= 2;
+    if (a.width < (1 << 22)) smem = bytes_of(C);
+  }
+  p.C = C;
+  const bool ring = smem <= 224 * 1024;
+  if (!ring) p.slot_bytes = 0;
+  const int64_t cap = (int64_t)ctx->sm_count * (!ring || smem <= 112 * 1024 ? 2 : 1) / C, clusters = a.rows < cap ? a.rows : cap;
   void* partial = nullptr;
   size_t partial_cap = 0;
   int rc = TFJS_CUDA_OK;
   if ((a.dgamma || a.dbeta) && (rc = ctx_alloc(ctx, (size_t)clusters * 2 * a.width * 4, &partial, &partial_cap))) return rc;
-  const cudaError_t e = launch_clusters(ctx, layer_norm_backprop_cluster_kernel<TD, TX, V>, clusters, 0, (const TD*)a.dy,
-                                        (const TX*)a.x, a.gamma, a.stats, a.dx, (float*)partial, a.rows, a.width);
+  p.partial = (float*)partial;
+  auto kernel = ring ? layer_norm_backprop_cluster_kernel<TD, TX, V, true> : layer_norm_backprop_cluster_kernel<TD, TX, V, false>;
+  const cudaError_t e = launch_clusters(ctx, kernel, clusters, C, ring ? (size_t)smem : 0, (const TD*)a.dy, (const TX*)a.x, p);
   if (e != cudaSuccess) rc = set_error(ctx, TFJS_CUDA_ERR_CUDA, "layerNormBackprop failed: %s", cudaGetErrorString(e));
   if (!rc) rc = post_launch(ctx, "layerNormBackprop (clusters)");
   if (!rc && partial) rc = join(ctx, a, (const float*)partial, (int)clusters);

@@ -32,6 +32,9 @@ __device__ __forceinline__ uint32_t narrow2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
+// A 4-byte word as the values it holds.
+__device__ __forceinline__ void unpack_word(uint32_t q, const float*, float (&v)[1]) { v[0] = __uint_as_float(q); }
+__device__ __forceinline__ void unpack_word(uint32_t q, const __half*, float (&v)[2]) { widen2(q, v[0], v[1]); }
 template <int V>
 __device__ __forceinline__ void load_vec(const __half* p, float (&v)[V]) {
   if constexpr (V == 8) {
