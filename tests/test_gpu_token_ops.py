@@ -64,7 +64,9 @@ def _ln_reference(x, g, b):
 LN_SHAPES = [(1, 1), (3, 1), (1, 1024), (5, 3), (7, 8), (130, 32), (33, 48), (64, 64), (19, 100), (301, 128), (9, 255),
              (77, 256), (150, 300), (40, 512), (29, 768), (301, 1000), (6, 1001), (10, 1024), (13, 1028), (9, 1536),
              (5, 2048), (200, 2050), (3, 4096), (4, 4104), (301, 5000), (2, 8192), (3, 8200), (2, 10001), (2, 16384),
-             (1, 16392), (3, 25088), (2, 50177), (1, 100352), (2, 131072), (1, 262147), (160, 9000), (1, 600000)]
+             (1, 16392), (3, 25088), (2, 50177), (1, 100352), (2, 131072), (1, 262147), (160, 9000), (1, 600000), (150, 66), (50, 114), (400, 130), (90, 515), (70, 1023), (70, 1030), (40, 2046),
+             (40, 2047), (30, 3001), (30, 4098), (20, 6143), (20, 8191), (12, 16383), (6, 16386), (150, 16400), (150, 20003),
+             (40, 33000), (30, 50002), (160, 8200)]
 
 
 @pytest.mark.parametrize("rows,width", LN_SHAPES)

@@ -9,9 +9,10 @@
 //
 // Forward.  A row is read once and stays on chip: the mean and then the centred square sum (which
 // does not cancel, unlike E[x^2] - m^2) come from the same registers.  Three forms by width:
-//   up to 1024     L lanes a row (4 .. 32), no shared memory; where rows start off the 16-byte
-//                  boundaries (then up to 2046 halves), a warp with a ring of rows in shared memory
+//   up to 1024     L lanes a row (4 .. 32), no shared memory
 //   up to 16384    one block a row
+//   either         where rows start off the 16-byte boundaries, a warp or a block with a ring of rows in
+//                  shared memory
 //   above          a cluster of 1 to 8 blocks a row, the row in their shared memory, sums joined over DSMEM
 // Gradient.  One pass over dy and x gives dx and, per block, the weights' gradients:
 //   up to 8192     persistent blocks; a ring of stages (several rows each) filled by cp.async.  First
@@ -150,34 +151,41 @@ __device__ __forceinline__ void stage_copy(uint8_t* dst, const uint8_t* base, in
   for (int i = threadIdx.x & (LANES - 1); i < units; i += LANES) copy_async16(dst + i * 16, src + i * 16);
 }
 
-// Rows that do not start on 16-byte boundaries.  A warp has a ring of two row slots in shared memory that
-// cp.async fills with the row's 16-byte units, so the loads are wide whatever the row's offset; it takes the
-// row from there into registers as 4-byte words, NW a lane (P values each: two halves or one float), and
-// needs no barrier but its own.  Where halves start at an odd place, the first word (and maybe the last)
-// holds one value of the neighbouring row, which is left out.  gamma and beta lie beside each other in
-// shared memory in the words' order, once for even and once for odd rows.
-// (One value a load in place of this: 33000 x 1001 half 93 us.)
-constexpr int kRingWarps = 8;
-template <typename TX, typename TY, int NW>
-__global__ void __launch_bounds__(kRingWarps * 32) layer_norm_ring_kernel(const TX* __restrict__ x,
+// Rows that do not start on 16-byte boundaries.  A group of G threads, a warp or the block, has a ring of two
+// row slots in shared memory that cp.async fills with the row's 16-byte units, so the loads are wide whatever
+// the row's offset; it takes the row from there into registers as 4-byte words, NW a thread (P values each:
+// two halves or one float).  Where halves start at an odd place, the first word (and maybe the last) holds
+// one value of the neighbouring row, which is left out.  For a warp's rows, gamma and beta lie beside each
+// other in shared memory in the words' order, once for even and once for odd rows.
+// (One value a load in place of this: 33000 x 1001 half 93 us, 9000 x 3001 half 76 us.)
+constexpr int kRingThreads = 256;
+template <typename TX, typename TY, int NW, int G>
+__global__ void __launch_bounds__(kRingThreads) layer_norm_ring_kernel(const TX* __restrict__ x,
                                                                          const float* __restrict__ gamma,
                                                                          const float* __restrict__ beta, TY* __restrict__ y,
                                                                          float* __restrict__ stats, int64_t rows, int width,
                                                                          float epsilon, int slot_bytes) {
   constexpr int P = 4 / (int)sizeof(TX);
   extern __shared__ __align__(16) uint8_t smem[];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint8_t* ring = smem + warp * 2 * slot_bytes;
+  constexpr int kGroups = kRingThreads / G;
+  __shared__ float scratch[2][kRingThreads / 32];
+  const int lane = threadIdx.x & (G - 1), group = threadIdx.x / G;
+  uint8_t* ring = smem + group * 2 * slot_bytes;
+  auto sync = [] {
+    if (G == 32) __syncwarp();
+    else __syncthreads();
+  };
+  auto sum = [&](float v, int turn) { return G == 32 ? lanes_sum<32>(v) : block_sum<kRingThreads>(v, scratch[turn]); };
   const int most = width / P + 1;  // words of a row, at most
-  float* weights = reinterpret_cast<float*>(smem + kRingWarps * 2 * slot_bytes);  // [odd][most][2 P]: P of gamma, P of beta
-  const int64_t step = (int64_t)gridDim.x * kRingWarps, first = (int64_t)blockIdx.x * kRingWarps + warp;
+  float* weights = reinterpret_cast<float*>(smem + kGroups * 2 * slot_bytes);  // [odd][most][2 P]: P of gamma, P of beta
+  const int64_t step = (int64_t)gridDim.x * kGroups, first = (int64_t)blockIdx.x * kGroups + group;
   auto fill = [&](int64_t row, int slot) {
     if (row < rows)
-      stage_copy<32>(ring + slot * slot_bytes, (const uint8_t*)x, row * width * (int64_t)sizeof(TX), width * (int)sizeof(TX));
+      stage_copy<G>(ring + slot * slot_bytes, (const uint8_t*)x, row * width * (int64_t)sizeof(TX), width * (int)sizeof(TX));
     copy_commit();
   };
   fill(first, 0);
-  for (int j = threadIdx.x; j < P * most * P; j += kRingWarps * 32) {
+  for (int j = threadIdx.x; G == 32 && j < P * most * P; j += kRingThreads) {
     const int odd = j / (most * P), e = j - odd * most * P, col = e - odd;
     float* w = weights + (odd * most + e / P) * 2 * P + e % P;
     const bool there = col >= 0 && col < width;
@@ -190,7 +198,7 @@ __global__ void __launch_bounds__(kRingWarps * 32) layer_norm_ring_kernel(const 
   for (int64_t row = first; row < rows; row += step, slot ^= 1) {
     fill(row + step, slot ^ 1);
     copy_wait<1>();
-    __syncwarp();  // the row is there for all lanes
+    sync();  // the row is there for all
     const int64_t at = row * width;
     const int odd = (int)(at & (P - 1)), words = (odd + width + P - 1) / P;
     const TX* r = reinterpret_cast<const TX*>(ring + slot * slot_bytes + ((at * (int64_t)sizeof(TX)) & 15)) - odd;
@@ -198,14 +206,14 @@ __global__ void __launch_bounds__(kRingWarps * 32) layer_norm_ring_kernel(const 
     uint32_t q[NW];
 #pragma unroll
     for (int i = 0; i < NW; i++) {
-      const int w = lane + 32 * i;
+      const int w = lane + G * i;
       q[i] = w < words ? *reinterpret_cast<const uint32_t*>(r + w * P) : 0u;
       if (P == 2) {
         if (w == 0 && odd) q[i] &= 0xffff0000u;
         if (w == words - 1 && cut) q[i] &= 0x0000ffffu;
       }
     }
-    __syncwarp();  // read by all lanes: the slot may be filled again
+    sync();  // read by all: the slot may be filled again
     const TX* none = nullptr;
     float s = 0.f;
 #pragma unroll
@@ -215,11 +223,11 @@ __global__ void __launch_bounds__(kRingWarps * 32) layer_norm_ring_kernel(const 
 #pragma unroll
       for (int k = 0; k < P; k++) s += v[k];
     }
-    const float mean = lanes_sum<32>(s) * inv;
+    const float mean = sum(s, 0) * inv;
     s = 0.f;
 #pragma unroll
     for (int i = 0; i < NW; i++) {
-      const int w = lane + 32 * i;
+      const int w = lane + G * i;
       if (w >= words) break;
       float v[P];
       unpack_word(q[i], none, v);
@@ -230,16 +238,25 @@ __global__ void __launch_bounds__(kRingWarps * 32) layer_norm_ring_kernel(const 
         s = fmaf(d, d, s);
       }
     }
-    const float rstd = 1.f / sqrtf(lanes_sum<32>(s) * inv + epsilon);
+    const float rstd = 1.f / sqrtf(sum(s, 1) * inv + epsilon);
     TY* out = y + at - odd;
     const float* mine = weights + odd * most * 2 * P;
 #pragma unroll
     for (int i = 0; i < NW; i++) {
-      const int w = lane + 32 * i;
+      const int w = lane + G * i;
       if (w >= words) break;
       float v[P], gb[2 * P];
       unpack_word(q[i], none, v);
-      load_vec<2 * P>(mine + w * 2 * P, gb);
+      if (G == 32) {
+        load_vec<2 * P>(mine + w * 2 * P, gb);
+      } else {
+#pragma unroll
+        for (int k = 0; k < P; k++) {
+          const int col = min(max(w * P + k - odd, 0), width - 1);
+          gb[k] = gamma ? gamma[col] : 1.f;
+          gb[P + k] = beta ? beta[col] : 0.f;
+        }
+      }
 #pragma unroll
       for (int k = 0; k < P; k++) v[k] = fmaf((v[k] - mean) * rstd, gb[k], gb[P + k]);
       const bool low = P == 2 && w == 0 && odd, high = P == 2 && w == words - 1 && cut;
@@ -332,38 +349,44 @@ __device__ __forceinline__ float2 cluster_sum(float a, float b, int C, float2* s
   return t;
 }
 
-// A cluster of C blocks a row.  `cached`: the block's share of the row fits into its dynamic shared
-// memory and is read from there the second and third time, else from global memory (L2).
+// A cluster of C blocks a row.  `cached`: the block's share of the row comes into its dynamic shared memory
+// by cp.async, whatever its offset, and is read from there; else three times from global memory (L2).
 template <typename TX, typename TY, int V>
-__global__ void __launch_bounds__(kClusterThreads) layer_norm_cluster_kernel(
+__global__ void __launch_bounds__(kClusterThreads, 3) layer_norm_cluster_kernel(
     const TX* __restrict__ x, const float* __restrict__ gamma, const float* __restrict__ beta, TY* __restrict__ y,
     float* __restrict__ stats, int64_t rows, int64_t width, float epsilon, int C, int cached) {
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ float2 scratch[2][kClusterThreads / 32];
   __shared__ float2 slot[2];
-  TX* kept = reinterpret_cast<TX*>(smem);
   const int64_t vecs = width / V, clusters = gridDim.x / C;
   const int64_t rank = blockIdx.x % C;
   const int64_t lo = vecs * rank / C;
   const int n = (int)(vecs * (rank + 1) / C - lo);
   for (int64_t row = blockIdx.x / C; row < rows; row += clusters) {
     const TX* r = x + row * width + lo * V;
+    if (cached) {
+      const int64_t first = row * width + lo * V;
+      __syncthreads();  // all are done with the row before
+      stage_copy<kClusterThreads>(smem, (const uint8_t*)x, first * (int64_t)sizeof(TX), n * V * (int)sizeof(TX));
+      copy_commit();
+      copy_wait<0>();
+      __syncthreads();
+      r = reinterpret_cast<const TX*>(smem + ((first * (int64_t)sizeof(TX)) & 15));
+    }
     float s = 0.f;
 #pragma unroll 4
     for (int j = threadIdx.x; j < n; j += kClusterThreads) {
       float v[V];
       load_vec<V>(r + j * V, v);
-      if (cached) store_vec<V>(kept + j * V, v);  // exact: the values came from this type
 #pragma unroll
       for (int k = 0; k < V; k++) s += v[k];
     }
     const float mean = cluster_sum(s, 0.f, C, &slot[0], scratch[0]).x / (float)width;
     s = 0.f;
-    const TX* from = cached ? kept : r;  // a thread reads back only what it wrote
 #pragma unroll 4
     for (int j = threadIdx.x; j < n; j += kClusterThreads) {
       float v[V];
-      load_vec<V>(from + j * V, v);
+      load_vec<V>(r + j * V, v);
 #pragma unroll
       for (int k = 0; k < V; k++) {
         const float d = v[k] - mean;
@@ -374,7 +397,7 @@ __global__ void __launch_bounds__(kClusterThreads) layer_norm_cluster_kernel(
 #pragma unroll 2
     for (int j = threadIdx.x; j < n; j += kClusterThreads) {
       float v[V];
-      load_vec<V>(from + j * V, v);
+      load_vec<V>(r + j * V, v);
       finish_vec<V>(v, mean, rstd, gamma, beta, (lo + j) * V, y + row * width + (lo + j) * V);
     }
     if (stats && rank == 0 && threadIdx.x == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
@@ -387,11 +410,18 @@ constexpr int kStagedWidth = 8192;
 constexpr int kStagedThreads = 256;
 constexpr int kMaxStageRows = 256;
 
+// Where a block (or cluster) leaves its dg and db: its row of a buffer that the join kernel adds up, or, where
+// there is only one, the results themselves.  Either may be null (not wanted).
+struct WeightSums {
+  float *dg, *db;
+  int64_t stride;  // from one block's row to the next
+};
+
 struct StagedParams {
   const float* gamma;
   const float* stats;
   float* dx;
-  float* partial;  // [gridDim.x][2][width] or null
+  WeightSums sums;
   int64_t rows, items;
   int width, stage_rows;        // stage_rows: a power of two
   int x_bytes, stage_bytes;     // of the dy and the whole stage area
@@ -520,9 +550,10 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
     }
     if (++slot == kStages) slot = 0;
   }
-  if (!p.partial) return;
-  // ---- the row groups' sums, in order; then this block's partial sums
-  float* mine = p.partial + (int64_t)blockIdx.x * 2 * width;
+  if (!p.sums.dg && !p.sums.db) return;
+  // ---- the row groups' sums, in order; then this block's
+  float* to_g = p.sums.dg ? p.sums.dg + blockIdx.x * p.sums.stride : nullptr;
+  float* to_b = p.sums.db ? p.sums.db + blockIdx.x * p.sums.stride : nullptr;
   if (RG > 1) {
     copy_wait<0>();
     __syncthreads();
@@ -535,15 +566,16 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
     for (int j = tid; j < 2 * width; j += kStagedThreads) {
       float s = 0.f;
       for (int g = 0; g < RG; g++) s += join[g * 2 * width + j];
-      mine[j] = s;
+      float* to = j < width ? to_g : to_b;
+      if (to) to[j < width ? j : j - width] = s;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < MC; i++) {
       const int c = c0 + i * kStagedThreads;
       if (owner && c < nc) {
-        store_vec<V>(mine + c * V, dg[i]);
-        store_vec<V>(mine + width + c * V, db[i]);
+        if (to_g) store_vec<V>(to_g + c * V, dg[i]);
+        if (to_b) store_vec<V>(to_b + c * V, db[i]);
       }
     }
   }
@@ -552,11 +584,12 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
 // ---- gradient, longer rows: a cluster of C blocks a row --------------------------------------------
 // RING: the block's share of dy and x comes into shared memory by cp.async, the next row's while this one is
 // summed and written, and its columns' dg and db add up there over the cluster's rows; else both passes read
-// global memory (the second one L2), and partial [clusters][2][width] is where dg and db add up.  In both
+// global memory (the second one L2), and the cluster's row of the sums is where dg and db add up.  In both
 // a thread meets its own columns only, but for the copies, which the barriers of the sums order.
 struct ClusterParams {
   const float *gamma, *stats;
-  float *dx, *partial;
+  float* dx;
+  WeightSums sums;
   int64_t rows, width;
   int C, d_bytes, slot_bytes;  // RING: of the dy area of a slot, and of a slot
 };
@@ -571,8 +604,8 @@ __global__ void __launch_bounds__(kClusterThreads, 2) layer_norm_backprop_cluste
   const int64_t width = p.width, vecs = width / V, clusters = gridDim.x / C, cluster = blockIdx.x / C;
   const int64_t rank = blockIdx.x % C, lo = vecs * rank / C * V;
   const int n = (int)(vecs * (rank + 1) / C - vecs * rank / C);
-  float* pg = p.partial ? p.partial + cluster * 2 * width + lo : nullptr;
-  float* pb = pg ? pg + width : nullptr;
+  float* pg = p.sums.dg ? p.sums.dg + cluster * p.sums.stride + lo : nullptr;
+  float* pb = p.sums.db ? p.sums.db + cluster * p.sums.stride + lo : nullptr;
   const float* gamma = p.gamma ? p.gamma + lo : nullptr;
   float* sg = reinterpret_cast<float*>(smem + 2 * p.slot_bytes);  // dg and db, V columns of each in turn
   auto fill = [&](int64_t row, int at) {
@@ -625,13 +658,10 @@ __global__ void __launch_bounds__(kClusterThreads, 2) layer_norm_backprop_cluste
       load_vec<V>(d0 + j * V, d);
       load_vec<V>(x0 + j * V, v);
       if (gamma) load_vec<V>(gamma + j * V, g);
-      if (pg && !fresh) {
-        load_vec<V>(RING ? sg + 2 * j * V : pg + j * V, wg);
-        load_vec<V>(RING ? sg + (2 * j + 1) * V : pb + j * V, wb);
-      } else {
 #pragma unroll
-        for (int k = 0; k < V; k++) wg[k] = wb[k] = 0.f;
-      }
+      for (int k = 0; k < V; k++) wg[k] = wb[k] = 0.f;
+      if (pg && !fresh) load_vec<V>(RING ? sg + 2 * j * V : pg + j * V, wg);
+      if (pb && !fresh) load_vec<V>(RING ? sg + (2 * j + 1) * V : pb + j * V, wb);
 #pragma unroll
       for (int k = 0; k < V; k++) {
         const float nn = (v[k] - mr.x) * mr.y;
@@ -640,18 +670,16 @@ __global__ void __launch_bounds__(kClusterThreads, 2) layer_norm_backprop_cluste
         wb[k] += d[k];
       }
       if (p.dx) store_vec<V>(p.dx + first + j * V, o);
-      if (pg) {
-        store_vec<V>(hand_over ? pg + j * V : sg + 2 * j * V, wg);
-        store_vec<V>(hand_over ? pb + j * V : sg + (2 * j + 1) * V, wb);
-      }
+      if (pg) store_vec<V>(hand_over ? pg + j * V : sg + 2 * j * V, wg);
+      if (pb) store_vec<V>(hand_over ? pb + j * V : sg + (2 * j + 1) * V, wb);
     }
   }
   cg::this_cluster().sync();
 }
 
-// out[j] = sum over the blocks of partial[block][j]: 32 columns a block, 32 threads a column take every
-// 32nd block's row and join theirs in order.  j runs over dg and then db.
-constexpr int kJoinThreads = 1024;
+// out[j] = sum over the blocks of partial[block][j]; j runs over dg and then db.  Many blocks: 32 columns a
+// block, 32 threads a column take every 32nd block's row and join theirs in order.  Up to 64: a thread a column.
+constexpr int kJoinThreads = 1024, kFewBlocks = 64;
 __global__ void __launch_bounds__(kJoinThreads) layer_norm_join_kernel(const float* __restrict__ partial,
                                                                       float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                                       int blocks, int64_t width) {
@@ -675,6 +703,19 @@ __global__ void __launch_bounds__(kJoinThreads) layer_norm_join_kernel(const flo
     }
     __syncthreads();
   }
+}
+__global__ void __launch_bounds__(256) layer_norm_join_few_kernel(const float* __restrict__ partial,
+                                                                 float* __restrict__ dgamma, float* __restrict__ dbeta,
+                                                                 int blocks, int64_t width) {
+  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  pdl_wait();
+  if (j >= 2 * width) return;
+  float* out = j < width ? dgamma : dbeta;
+  if (!out) return;
+  float s = 0.f;
+#pragma unroll 8
+  for (int b = 0; b < blocks; b++) s += partial[(int64_t)b * 2 * width + j];
+  out[j < width ? j : j - width] = s;
 }
 
 // ---- launchers -----------------------------------------------------------------------------------
@@ -703,25 +744,39 @@ void block_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
       (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon);
 }
 
-// A launch of clusters of C blocks; `smem` bytes of dynamic shared memory a block.
+// Clusters of C blocks with `smem` bytes of dynamic shared memory each: a launch, and how many run at once.
+struct ClusterLaunch {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  ClusterLaunch(const tfjs_cuda_ctx* ctx, int64_t clusters, int C, size_t smem) {
+    cfg.gridDim = dim3((unsigned)(clusters * C));
+    cfg.blockDim = dim3(kClusterThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = ctx ? ctx->stream : nullptr;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+};
+template <typename Kernel>
+cudaError_t allow_smem(Kernel kernel, size_t smem) {
+  return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
+}
+template <typename Kernel>
+cudaError_t clusters_at_once(Kernel kernel, int C, size_t smem, int* most) {
+  const cudaError_t e = allow_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
+  ClusterLaunch l(nullptr, 1, C, smem);
+  return cudaOccupancyMaxActiveClusters(most, kernel, &l.cfg);
+}
 template <typename... Params, typename... Args>
 cudaError_t launch_clusters(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), int64_t clusters, int C, size_t smem, Args... args) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * C));
-  cfg.blockDim = dim3(kClusterThreads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = ctx->stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = C;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
+  const cudaError_t e = allow_smem(kernel, smem);
+  if (e != cudaSuccess) return e;
+  ClusterLaunch l(ctx, clusters, C, smem);
+  return cudaLaunchKernelEx(&l.cfg, kernel, static_cast<Params>(args)...);
 }
 
 template <typename TX, typename TY, int V>
@@ -729,7 +784,7 @@ int cluster_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   // Blocks a row: so many that three blocks' shares fit into an SM's shared memory (one loads while another
   // sums), and with few rows so many that the SMs have a block each.  Every block costs each row two
   // cluster-wide waits of about a microsecond: 1000 x 33000 is 137 us with 8 blocks a row.
-  const auto share_of = [&](int C) { return (ceil_div64(a.width / V, C) * V * (int64_t)sizeof(TX) + 15) / 16 * 16; };
+  const auto share_of = [&](int C) { return (ceil_div64(a.width / V, C) * V * (int64_t)sizeof(TX) + 31) / 16 * 16; };
   int C = 1;
   while (C < 8 && (share_of(C) > 72 * 1024 || a.rows * C < ctx->sm_count)) C *= 2;
   const int64_t share = share_of(C), cap = 1 << 24;
@@ -740,58 +795,70 @@ int cluster_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   return post_launch(ctx, "layerNorm (clusters)");
 }
 
-// V values a load: 16 bytes where every row starts on a 16-byte boundary, else 2 values, else 1.
+// Rows on the 16-byte boundaries: V values, 16 bytes of the result, a load.
 template <typename TX, typename TY, int V>
-int forward_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
+int aligned_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   const int64_t w = a.width;
-  if (w > 16384) return cluster_form<TX, TY, V>(ctx, a);
+  constexpr int NV = 32 / V;  // 32 values a thread
   if (w <= 1024) {
     if (w <= 4 * V) lanes_form<TX, TY, V, 1, 4>(ctx, a);
     else if (w <= 16 * V) lanes_form<TX, TY, V, 1, 16>(ctx, a);
-    else if (w <= 64 * V) lanes_form<TX, TY, V, 2, 32>(ctx, a);
-    else if constexpr (V >= 4) {  // rows off the 16-byte boundaries come here up to 64 V columns only
-      if (w <= 128 * V) lanes_form<TX, TY, V, 4, 32>(ctx, a);
-      else if constexpr (V == 4) lanes_form<TX, TY, V, 8, 32>(ctx, a);
-    }
+    else if (w <= 256) lanes_form<TX, TY, V, 8 / V, 32>(ctx, a);
+    else if (w <= 512) lanes_form<TX, TY, V, 16 / V, 32>(ctx, a);
+    else lanes_form<TX, TY, V, NV, 32>(ctx, a);
     return post_launch(ctx, "layerNorm (lanes)");
   }
-  constexpr int NV = 32 / V;  // 32 values a thread
-  if (V >= 4 && w <= 256 * 8) block_form<TX, TY, V, V >= 4 ? NV / 4 : NV / 2, 256>(ctx, a);
+  if (w > 16384) return cluster_form<TX, TY, V>(ctx, a);
+  if (w <= 256 * 8) block_form<TX, TY, V, NV / 4, 256>(ctx, a);
   else if (w <= 256 * 16) block_form<TX, TY, V, NV / 2, 256>(ctx, a);
   else if (w <= 256 * 32) block_form<TX, TY, V, NV, 256>(ctx, a);
   else block_form<TX, TY, V, NV, 512>(ctx, a);
   return post_launch(ctx, "layerNorm (blocks)");
 }
 
-template <typename TX, typename TY, int NW>
+template <typename TX, typename TY, int NW, int G>
 int ring_launch(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
-  constexpr int P = 4 / (int)sizeof(TX);
+  constexpr int P = 4 / (int)sizeof(TX), groups = kRingThreads / G;
   const int slot_bytes = ((int)a.width * (int)sizeof(TX) + 31) / 16 * 16;  // one unit more for the row's own offset
-  const int smem = kRingWarps * 2 * slot_bytes + P * ((int)a.width / P + 1) * 2 * P * 4;
-  auto kernel = layer_norm_ring_kernel<TX, TY, NW>;
+  const int smem = groups * 2 * slot_bytes + (G == 32 ? P * ((int)a.width / P + 1) * 2 * P * 4 : 0);
+  auto kernel = layer_norm_ring_kernel<TX, TY, NW, G>;
   if (smem > 48 * 1024)
     TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   const int per_sm = smem <= 36 * 1024 ? 6 : smem <= 55 * 1024 ? 4 : smem <= 74 * 1024 ? 3 : 2;
-  kernel<<<grid_rows(ctx, ceil_div64(a.rows, kRingWarps), per_sm), kRingWarps * 32, smem, ctx->stream>>>(
+  kernel<<<grid_rows(ctx, ceil_div64(a.rows, groups), per_sm), kRingThreads, smem, ctx->stream>>>(
       (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon, slot_bytes);
   return post_launch(ctx, "layerNorm (ring)");
 }
 // Words of a row that starts at an odd place: width / P + 1 at most.
+constexpr int kRingWords = 32 * kRingThreads;
 template <typename TX, typename TY>
 int ring_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   const int64_t words = a.width / (4 / (int)sizeof(TX)) + 1;
-  if (words <= 256) return ring_launch<TX, TY, 8>(ctx, a);
-  if (words <= 512) return ring_launch<TX, TY, 16>(ctx, a);
-  return ring_launch<TX, TY, 32>(ctx, a);
+  if (words <= 256) return ring_launch<TX, TY, 8, 32>(ctx, a);
+  if (words <= 512) return ring_launch<TX, TY, 16, 32>(ctx, a);
+  if (words <= 1024) return ring_launch<TX, TY, 32, 32>(ctx, a);
+  if (words <= 8 * kRingThreads) return ring_launch<TX, TY, 8, kRingThreads>(ctx, a);
+  if (words <= 16 * kRingThreads) return ring_launch<TX, TY, 16, kRingThreads>(ctx, a);
+  return ring_launch<TX, TY, 32, kRingThreads>(ctx, a);
 }
 
 template <typename TX, typename TY>
 int launch_forward(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   constexpr int W = sizeof(TX) == 2 && sizeof(TY) == 2 ? 8 : 4;  // 16 bytes of the result
-  if (a.width % W == 0) return forward_form<TX, TY, W>(ctx, a);
-  if (a.width > (a.width % 2 ? 64 : 128) && a.width / (4 / (int)sizeof(TX)) + 1 <= 1024) return ring_form<TX, TY>(ctx, a);
-  if (a.width % 2 == 0) return forward_form<TX, TY, 2>(ctx, a);
-  return forward_form<TX, TY, 1>(ctx, a);
+  const int64_t w = a.width;
+  if (w % W == 0) return aligned_form<TX, TY, W>(ctx, a);
+  if (w % 2 == 0 && w <= 128) {
+    if (w <= 32) lanes_form<TX, TY, 2, 1, 16>(ctx, a);
+    else lanes_form<TX, TY, 2, 2, 32>(ctx, a);
+    return post_launch(ctx, "layerNorm (lanes)");
+  }
+  if (w <= 64) {
+    if (w <= 16) lanes_form<TX, TY, 1, 1, 16>(ctx, a);
+    else lanes_form<TX, TY, 1, 2, 32>(ctx, a);
+    return post_launch(ctx, "layerNorm (lanes)");
+  }
+  if (w / (4 / (int)sizeof(TX)) + 1 <= kRingWords) return ring_form<TX, TY>(ctx, a);
+  return w % 2 == 0 ? cluster_form<TX, TY, 2>(ctx, a) : cluster_form<TX, TY, 1>(ctx, a);
 }
 
 struct BackwardArgs {
@@ -801,9 +868,26 @@ struct BackwardArgs {
   int64_t rows, width;
 };
 
-int join(tfjs_cuda_ctx* ctx, const BackwardArgs& a, const float* partial, int blocks) {
-  launch_dependent(ctx, layer_norm_join_kernel, dim3(grid_rows(ctx, ceil_div64(2 * a.width, 32), 2)), dim3(kJoinThreads), partial,
-                   a.dgamma, a.dbeta, blocks, a.width);
+// Where `blocks` blocks leave their weights' sums: *partial is a workspace for more than one, and the caller
+// gives it back after join_sums.
+int place_sums(tfjs_cuda_ctx* ctx, const BackwardArgs& a, int64_t blocks, WeightSums* sums, void** partial, size_t* cap) {
+  *partial = nullptr;
+  *cap = 0;
+  *sums = {a.dgamma, a.dbeta, 0};
+  if (blocks == 1 || (!a.dgamma && !a.dbeta)) return TFJS_CUDA_OK;
+  const int rc = ctx_alloc(ctx, (size_t)blocks * 2 * a.width * 4, partial, cap);
+  if (rc) return rc;
+  *sums = {(float*)*partial, (float*)*partial + a.width, 2 * a.width};
+  return TFJS_CUDA_OK;
+}
+int join_sums(tfjs_cuda_ctx* ctx, const BackwardArgs& a, const void* partial, int64_t blocks) {
+  if (!partial) return TFJS_CUDA_OK;
+  if (blocks <= kFewBlocks)
+    launch_dependent(ctx, layer_norm_join_few_kernel, dim3((unsigned)ceil_div64(2 * a.width, 256)), dim3(256),
+                     (const float*)partial, a.dgamma, a.dbeta, (int)blocks, a.width);
+  else
+    launch_dependent(ctx, layer_norm_join_kernel, dim3(grid_rows(ctx, ceil_div64(2 * a.width, 32), 2)), dim3(kJoinThreads),
+                     (const float*)partial, a.dgamma, a.dbeta, (int)blocks, a.width);
   return post_launch(ctx, "layerNormBackprop (join)");
 }
 
@@ -819,10 +903,12 @@ int staged_launch(tfjs_cuda_ctx* ctx, const BackwardArgs& a, StagedParams& p, in
 template <typename TD, typename TX, int V>
 int staged_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
   const int width = (int)a.width, row_bytes = width * (int)(sizeof(TD) + sizeof(TX));
-  // rows a stage: about 32 KB, so that two blocks with three stages each share an SM, but not so many
-  // that the blocks have fewer than two stages each
+  // rows a stage: about 32 KB, so that two blocks with three stages each share an SM, but not so many that
+  // the blocks have fewer than two stages each; and all rows where they fit (one block, and no join)
   int R = 1;
   while (R < kMaxStageRows && 2 * R * row_bytes <= 32 * 1024 && ceil_div64(a.rows, 2 * R) >= 4 * ctx->sm_count) R *= 2;
+  if (a.rows <= kMaxStageRows && a.rows * row_bytes <= 32 * 1024)
+    while (R < a.rows) R *= 2;
   StagedParams p = {};
   p.gamma = a.gamma;
   p.stats = a.stats;
@@ -839,27 +925,24 @@ int staged_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
   const size_t smem = (size_t)kStages * p.stage_bytes + (size_t)(width + 3) / 4 * 16 + (size_t)R * parts * 8;
   const int64_t cap = (int64_t)ctx->sm_count * (smem <= 113 * 1024 ? 2 : 1);
   const int blocks = (int)(p.items < cap ? p.items : cap);
-  void* partial = nullptr;
-  size_t partial_cap = 0;
-  int rc;
-  if (a.dgamma || a.dbeta) {
-    if ((rc = ctx_alloc(ctx, (size_t)blocks * 2 * width * 4, &partial, &partial_cap))) return rc;
-    p.partial = (float*)partial;
-  }
+  void* partial;
+  size_t partial_cap;
+  int rc = place_sums(ctx, a, blocks, &p.sums, &partial, &partial_cap);
+  if (rc) return rc;
   // 4, 8, 16 or 32 columns a thread
   const int columns = (width + kStagedThreads - 1) / kStagedThreads;
   if (columns <= 4) rc = staged_launch<TD, TX, V, 4 / V>(ctx, a, p, blocks, smem);
   else if (columns <= 8) rc = staged_launch<TD, TX, V, 8 / V>(ctx, a, p, blocks, smem);
   else if (columns <= 16) rc = staged_launch<TD, TX, V, 16 / V>(ctx, a, p, blocks, smem);
   else rc = staged_launch<TD, TX, V, 32 / V>(ctx, a, p, blocks, smem);
-  if (!rc && partial) rc = join(ctx, a, (const float*)partial, blocks);
+  if (!rc) rc = join_sums(ctx, a, partial, blocks);
   ctx_free(ctx, partial, partial_cap);
   return rc;
 }
 
 template <typename TD, typename TX, int V>
 int backward_cluster_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
-  ClusterParams p = {a.gamma, a.stats, a.dx, nullptr, a.rows, a.width, 1, 0, 0};
+  ClusterParams p = {a.gamma, a.stats, a.dx, {}, a.rows, a.width, 1, 0, 0};
   const auto bytes_of = [&](int C) {
     const int64_t share = ceil_div64(a.width / V, C) * V;
     p.C = C;
@@ -877,17 +960,23 @@ int backward_cluster_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
   p.C = C;
   const bool ring = smem <= 224 * 1024;
   if (!ring) p.slot_bytes = 0;
-  const int64_t cap = (int64_t)ctx->sm_count * (!ring || smem <= 112 * 1024 ? 2 : 1) / C, clusters = a.rows < cap ? a.rows : cap;
-  void* partial = nullptr;
-  size_t partial_cap = 0;
-  int rc = TFJS_CUDA_OK;
-  if ((a.dgamma || a.dbeta) && (rc = ctx_alloc(ctx, (size_t)clusters * 2 * a.width * 4, &partial, &partial_cap))) return rc;
-  p.partial = (float*)partial;
   auto kernel = ring ? layer_norm_backprop_cluster_kernel<TD, TX, V, true> : layer_norm_backprop_cluster_kernel<TD, TX, V, false>;
+  // as many clusters as run at once (the SMs of a cluster lie together, so it is fewer than SMs / C): one that
+  // had to wait for another's end would double the time
+  int64_t clusters = a.rows;
+  if (clusters * C > ctx->sm_count) {
+    int most = 0;
+    TFJS_CHECK_CUDA(ctx, clusters_at_once(kernel, C, ring ? (size_t)smem : 0, &most));
+    if (clusters > most) clusters = most > 0 ? most : 1;
+  }
+  void* partial;
+  size_t partial_cap;
+  int rc = place_sums(ctx, a, clusters, &p.sums, &partial, &partial_cap);
+  if (rc) return rc;
   const cudaError_t e = launch_clusters(ctx, kernel, clusters, C, ring ? (size_t)smem : 0, (const TD*)a.dy, (const TX*)a.x, p);
   if (e != cudaSuccess) rc = set_error(ctx, TFJS_CUDA_ERR_CUDA, "layerNormBackprop failed: %s", cudaGetErrorString(e));
   if (!rc) rc = post_launch(ctx, "layerNormBackprop (clusters)");
-  if (!rc && partial) rc = join(ctx, a, (const float*)partial, (int)clusters);
+  if (!rc) rc = join_sums(ctx, a, partial, clusters);
   ctx_free(ctx, partial, partial_cap);
   return rc;
 }
