@@ -107,7 +107,7 @@ class BackendCuda:
     def _id(self, t, want="float32"):
         """Device tensor id of `t`, converting when the stored dtype differs from the dtype
         the tensor claims (cast-up aliases share storage, backend_util.ts:50-54)."""
-        rec = self._rec(t.dataId)
+        rec = self._data.get(t.dataId) or self._rec(t.dataId)
         if rec["dtype"] == want:
             return rec["id"], None
         tmp = self._new_id(t.shape, want)
@@ -141,7 +141,7 @@ class BackendCuda:
     def _activation_id(self, t):
         """Device id of an activation operand for the kernels that read float32 and half storage
         alike; any other storage is converted to float32 first."""
-        rec = self._rec(t.dataId)
+        rec = self._data.get(t.dataId) or self._rec(t.dataId)
         if rec["dtype"] in ("float32", "float16"):
             return rec["id"], None
         return self._id(t)

@@ -8,6 +8,7 @@ reference counts (engine.ts:502-572), tidy scopes (engine.ts:365-399, 675-718) a
 runKernel dispatcher (engine.ts:435-498), the gradient tape (engine.ts:660-669, 726-774;
 tape.ts) including nested tapes for higher-order gradients.
 """
+import math
 import warnings
 
 import numpy as np
@@ -21,19 +22,16 @@ class DataId:
 
 
 def size_from_shape(shape):
-    n = 1
-    for s in shape:
-        n *= int(s)
-    return n
+    return math.prod(map(int, shape))
 
 
 class Tensor:
     """tensor.ts:419-484: a shape, a dtype and a dataId registered with the engine."""
 
     def __init__(self, shape, dtype, values=None, data_id=None, backend=None):
-        self.shape = [int(s) for s in shape]
+        self.shape = list(map(int, shape))
         self.dtype = dtype
-        self.size = size_from_shape(self.shape)
+        self.size = math.prod(self.shape)
         self.dataId = data_id if data_id is not None else DataId()
         self.isDisposed = False
         self.kept = False
