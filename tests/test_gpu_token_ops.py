@@ -369,6 +369,17 @@ def test_distillation_with_masked_classes_and_special_logits(tf):
         assert np.isfinite(dz[:3]).all() and np.isnan(dz[3:5]).all() and not dz[5].any()
 
 
+@pytest.mark.parametrize("size", [1, 30, 700, 3000, 1e5, 1e20])
+def test_distillation_of_large_logits(tf, size):
+    """Across the point where max * log2(e) / T no longer fits beside the terms."""
+    rng = _rng(int(np.log(size)), 4)
+    z = rng.normal(0, 1, (9, 1200)) * size + size * rng.choice([-1, 1], (9, 1))
+    idx, u = _teacher(rng, 9, 1200, 7)
+    z[np.arange(9)[:, None], idx] = z.max(-1, keepdims=True) - rng.uniform(0, 3, idx.shape)   # some q are not 0
+    for t in (1.0, 0.7):
+        _check_distillation(tf, z, u * min(size, 1e3), idx, t, "float32", "float32")
+
+
 def test_distillation_ignores_rows_without_weight(tf):
     rng = _rng(8)
     z = rng.normal(0, 2, (4, 50))
@@ -508,6 +519,102 @@ def test_guard_patterns_stay_intact(tf):
             bk.sync()   # an overwritten guard would be reported here
     finally:
         bk.setOption("debug_canary", 0)
+
+
+def _filled(bk, shape, storage, fill):
+    import torch
+    t = bk.registerStored(list(shape), storage)
+    view = torch.as_tensor(bk.deviceArray(t), device="cuda")
+    fill(view)
+    return t, view
+
+
+@pytest.mark.parametrize("rows,width", [(2100000, 1024), (2145003, 1003), (66000, 33000)])
+def test_layer_norm_offsets_past_32_bits(tf, rows, width):
+    import torch
+    bk = tf.ENGINE.backend
+    torch.manual_seed(3)
+    x, vx = _filled(bk, (rows, width), "float16", lambda v: v.normal_())
+    g = _rng(1).normal(1, 0.2, width).astype(np.float32)
+    torch.cuda.synchronize()
+    y, stats = bk.layerNorm(x, tf.ops.tensor(g), None, EPS, True, "float16")
+    bk.sync()
+    vy, vs = (torch.as_tensor(bk.deviceArray(t), device="cuda") for t in (y, stats))
+    dx, dg, db = bk.layerNormBackprop(y, x, tf.ops.tensor(g), stats)
+    bk.sync()
+    vd = torch.as_tensor(bk.deviceArray(dx), device="cuda")
+    for rows_at in (slice(0, 3), slice(rows // 2, rows // 2 + 3), slice(rows - 3, rows)):
+        xs, ys, ss, ds = (v[rows_at].float().cpu().numpy() for v in (vx, vy, vs, vd))
+        want, off, _, _ = _ln_reference(xs, g, np.zeros(width, np.float32))
+        _within(ys, want, off + _half_step(want, "float16"))
+        (want, off), _, _ = _ln_backward_reference(ys, xs, g, ss)
+        _within(ds, want, off)
+    # dbeta: a column's sum of two million terms; its error is far below the share of one row that a wrong
+    # offset would lose or count twice, taken over all columns
+    total = sum(vy[i:i + 10000].double().sum(0) for i in range(0, rows, 10000)).cpu().numpy()
+    assert np.abs(db.dataSync() - total).max() <= CHAIN * U * rows
+    for t in (x, y, stats, dx, dg, db):
+        t.dispose()
+
+
+def test_embedding_offsets_past_32_bits(tf):
+    import torch
+    bk = tf.ENGINE.backend
+    rows, width = 2100000, 1024
+    table, vt = _filled(bk, (rows, width), "float16", lambda v: v.normal_())
+    idx = np.array([rows - 1, 0, 2097152, rows, 2097151, rows - 1], np.int32)
+    torch.cuda.synchronize()
+    out = bk.embeddingLookup(table, tf.ops.tensor(idx, dtype="int32"), 1.0, "float16").dataSync().reshape(6, width)
+    for k in (0, 1, 2, 4, 5):
+        assert np.array_equal(out[k], vt[int(idx[k])].float().cpu().numpy())
+    assert not out[3].any()
+    small = bk.registerStored([50, width], "float16", _rng(1).normal(0, 1, 50 * width).astype(np.float32))
+    many, vi = _filled(bk, (rows,), "int32", lambda v: v.copy_(torch.arange(rows, device="cuda") % 50))
+    torch.cuda.synchronize()
+    wide = bk.embeddingLookup(small, many, 1.0, "float16")
+    bk.sync()
+    vw = torch.as_tensor(bk.deviceArray(wide), device="cuda")
+    assert torch.equal(vw[-100:], vw[:50].repeat(2, 1)) and torch.equal(vw[:50].cpu().float().reshape(-1), torch.from_numpy(small.dataSync()))
+    # gradients: of a table past 32 bits from few tokens, of a small one from rows past 32 bits (all ones: counts)
+    dy = tf.ops.tensor(np.arange(6, dtype=np.float32)[:, None] * np.ones((6, width), np.float32))
+    dt = bk.embeddingLookupBackprop(dy, tf.ops.tensor(idx, dtype="int32"), rows, 1.0)
+    bk.sync()
+    vd = torch.as_tensor(bk.deviceArray(dt), device="cuda")
+    want = {rows - 1: 5.0, 0: 1.0, 2097152: 2.0, 2097151: 4.0}
+    for r, v in want.items():
+        assert bool((vd[r] == v).all())
+    assert float(vd.sum(dtype=torch.float64)) == sum(want.values()) * width
+    dt.dispose()
+    vw.fill_(1.0)
+    torch.cuda.synchronize()
+    counts = bk.embeddingLookupBackprop(wide, many, 50, 1.0)
+    assert np.array_equal(counts.dataSync().reshape(50, width), np.full((50, width), rows // 50, np.float32))
+    for t in (table, wide, many, counts):
+        t.dispose()
+
+
+def test_distillation_offsets_past_32_bits(tf):
+    import torch
+    bk = tf.ENGINE.backend
+    rows, classes, top = 16401, 131073, 4
+    z, vz = _filled(bk, (rows, classes), "float16", lambda v: v.normal_())
+    rng = _rng(5)
+    idx = rng.integers(0, classes, (rows, top)).astype(np.int32)
+    u = rng.normal(0, 2, (rows, top)).astype(np.float32)
+    dloss = rng.uniform(0.5, 1, rows).astype(np.float32)
+    tu, ti = tf.ops.tensor(u), tf.ops.tensor(idx, dtype="int32")
+    torch.cuda.synchronize()
+    loss, stats = bk.distillationLoss(z, tu, ti, 1.0)
+    dz = bk.distillationLossBackprop(tf.ops.tensor(dloss), z, tu, ti, stats, 1.0)
+    bk.sync()
+    vd = torch.as_tensor(bk.deviceArray(dz), device="cuda")
+    got = loss.dataSync()
+    for at in (slice(0, 2), slice(rows // 2, rows // 2 + 2), slice(rows - 2, rows)):
+        want, off, dwant, doff, _ = _distillation_reference(vz[at].float().cpu().numpy(), u[at], idx[at], dloss[at], 1.0)
+        _within(got[at], want, off)
+        _within(vd[at].cpu().numpy(), dwant, doff)
+    for t in (z, loss, stats, dz):
+        t.dispose()
 
 
 def test_two_contexts_at_once(tf):

@@ -29,8 +29,8 @@ namespace {
 constexpr int kMaxTop = 1024;
 constexpr int kThreads = 256;      // of a block of the loss
 constexpr int kGradThreads = 256;  // of a block of the gradient
-constexpr int kBatch = 4;          // 16-byte loads in flight a thread of the loss
-constexpr int kGradBatch = 4;      // and of the gradient
+constexpr int kBatch = 8;          // 16-byte loads in flight a thread of the loss
+constexpr int kGradBatch = 8;      // and of the gradient
 constexpr float kLn2 = 0.693147180559945f;
 constexpr float kLog2e = 1.44269504088896f;
 
@@ -121,7 +121,7 @@ __device__ __forceinline__ float units_max(const Unit<__half> (&u)[N]) {
 
 // The exponent (z - m) k - l of a value z is taken as fma(z, k, shift), shift = -(m k + l): one packed
 // instruction for two values.  What the rounding of `shift` loses is the same for all of them, so it
-// goes into a factor for the whole: 2^((z - m) k - l) = 2^fma(z, k, shift) * factor.  Where m k is too
+// goes into a factor for the whole: 2^((z - m) k - l) = 2^fma(z, k, shift) * factor.  Where m k + l is too
 // large for that (a row of the type's lowest values), `exact` is set and the difference comes first.
 struct Shift {
   float shift, factor;
@@ -131,8 +131,8 @@ struct Shift {
     const float sum = hi + l, back = sum - hi;
     const float lost = (hi - (sum - back)) + (l - back) + lo;
     shift = -sum;
-    factor = 1.f - lost * kLn2;  // |lost| < 2^-20 |shift|: 2^-lost to float32's precision
-    exact = !(fabsf(sum) < 1e4f);
+    factor = 1.f - lost * kLn2;  // |lost| <= 2^-13: 2^-lost to 4e-9
+    exact = !(fabsf(sum) < 2048.f);
   }
 };
 
