@@ -324,7 +324,8 @@ def _check_distillation(tf, z, u, idx, t, sz, su, dloss=None):
 
 @pytest.mark.parametrize("rows,classes,top", [(1, 1, 1), (3, 2, 1), (5, 7, 7), (64, 10, 3), (33, 100, 5), (128, 1000, 5),
                                               (7, 1001, 64), (2, 4099, 32), (300, 515, 9), (5, 32000, 64), (2, 32001, 128),
-                                              (1, 131101, 1), (2, 150000, 1024), (700, 2048, 17), (9, 12345, 0)])
+                                              (1, 131101, 1), (2, 150000, 1024), (700, 2048, 17), (9, 12345, 0),
+                                              (1300, 1025, 128), (1300, 5001, 5), (1250, 8192, 3), (1200, 8193, 2), (40, 3000, 129)])
 @pytest.mark.parametrize("sz,su", [("float32", "float32"), ("float16", "float16"), ("float16", "float32"), ("float32", "float16")])
 def test_distillation_loss(tf, rows, classes, top, sz, su):
     rng = _rng(rows, classes, top)
@@ -484,7 +485,7 @@ def _upload(tf, arrays):
     return {k: tf.ops.tensor(v, dtype="int32" if v.dtype == np.int32 else "float32") for k, v in arrays.items()}
 
 
-@pytest.mark.parametrize("tokens", [300, 5000])
+@pytest.mark.parametrize("tokens", [300, 5000, 70000])
 def test_captured_graph_replays_on_new_inputs(tf, tokens):
     bk = tf.ENGINE.backend
     first, second, third = (_step_inputs(tf, s, tokens) for s in (1, 2, 3))
@@ -508,11 +509,52 @@ def test_captured_graph_replays_on_new_inputs(tf, tokens):
     bk.graphDestroy(graph2)
 
 
+def test_captured_clusters(tf):
+    bk = tf.ENGINE.backend
+    rng = _rng(31)
+    x, dy = rng.normal(0, 1, (2, 200, 20004)).astype(np.float32)
+    g = rng.normal(1, 0.2, 20004).astype(np.float32)
+    tx, td, tg = (tf.ops.tensor(v) for v in (x, dy, g))
+
+    def step():
+        y, stats = bk.layerNorm(tx, tg, tg, EPS, True)
+        return [y, stats, *bk.layerNormBackprop(td, tx, tg, stats)]
+    bk.graphBegin()
+    outs = step()
+    graph = bk.graphEnd()
+    for v in (x, dy):
+        bk.write(tx.dataId, v)
+        bk.graphLaunch(graph)
+        for a, b in zip(outs, step()):
+            assert np.array_equal(a.dataSync(), b.dataSync())
+    bk.graphDestroy(graph)
+
+
+@pytest.mark.parametrize("option", ["pdl", "debug_sync"])
+def test_launch_options_do_not_change_results(tf, option):
+    bk = tf.ENGINE.backend
+    t = _upload(tf, _step_inputs(tf, 41, 4000))
+    want = [o.dataSync() for o in _step(tf, t)]
+    bk.setOption(option, 1)
+    try:
+        for _ in range(3):
+            outs = _step(tf, t)
+            soft = bk.softmax(outs[-1])      # a kernel of the library behind the last one
+            got = [o.dataSync() for o in outs]
+            for a, b in zip(got, want):
+                assert np.array_equal(a, b)
+            e = np.exp(got[-1].reshape(70, -1).astype(np.float64) - got[-1].reshape(70, -1).max(-1, keepdims=True))
+            assert np.abs(soft.dataSync().reshape(70, -1) - e / e.sum(-1, keepdims=True)).max() < 1e-6
+    finally:
+        bk.setOption(option, 0)
+
+
 def test_guard_patterns_stay_intact(tf):
     bk = tf.ENGINE.backend
     bk.setOption("debug_canary", 1)
     try:
-        for tokens, vocab, width in [(7, 5, 33), (65, 20, 1001), (1030, 3, 64), (70000, 40, 6), (3, 4, 20003)]:
+        for tokens, vocab, width in [(7, 5, 33), (65, 20, 1001), (1030, 3, 64), (70000, 40, 6), (3, 4, 20003),
+                                     (200, 9, 9001), (150, 7, 16400), (31, 5, 3001), (2000, 11, 130)]:
             outs = tf.ENGINE.tidy(lambda: _step(tf, _upload(tf, _step_inputs(tf, width, tokens, vocab, width, 3))))
             for o in outs:
                 o.dispose()

@@ -14,9 +14,14 @@
 // pass leaves (max z, log2 of z's sum, max u, log2 of u's sum) of each row for the backward pass,
 // apart, because the logarithm would be lost beside a large maximum.  max u is -inf for an empty list.
 //
-// Both passes stream the logits once and are bound by memory.  A row starts anywhere, so its elements
-// before the first 16-byte boundary and behind the last one are taken one by one and all others in
-// 16-byte loads; the float32 gradient has the same element offsets, so its stores are aligned too.
+// Both passes stream the logits once.  A row starts anywhere, so its elements before the first 16-byte
+// boundary and behind the last one are taken one by one and all others in 16-byte loads; the float32
+// gradient has the same element offsets, so its stores are aligned too.
+// The gradient is bound by memory: 8192 x 32000 half with 64 entries 239 us, 1.57 GB at 6.6 TB/s; with 16-byte
+// loads of halves, whose gradients are then two stores a lane that do not lie side by side, 296 us; with four
+// units a thread in place of eight 264 us.  The loss of the same rows takes 112 us, 524 MB at 4.7 TB/s: half
+// the unit that computes exp2 is busy, and every row ends in three joins of its block; single-value arithmetic
+// instead of the packed one 172 us, two blocks of 512 threads an SM instead of five of 256 129 us.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -437,12 +442,16 @@ int launch_forward(tfjs_cuda_ctx* ctx, const Operands& o, float* loss, float* st
   const TZ* z = (const TZ*)o.z->ptr;
   const TU* u = (const TU*)o.u->ptr;
   const int32_t* indices = (const int32_t*)o.indices->ptr;
-  if (classes <= 1024 && top <= 128) {
+  // A warp a row, for short rows and, where the rows fill the SMs with warps, for longer ones: a block's three
+  // joins cost it 5 us whatever the row holds.  8192 rows of 1000 classes: 12 us, 53 with blocks; of 8000 (half)
+  // 38 and 72; of 16000 the block is ahead (4096 rows: 61 and 55), and so it is with 100 rows of 4000 (6 and 4).
+  if (top <= 128 && (classes <= 1024 || (classes <= 8192 && rows >= 8 * ctx->sm_count))) {
     distillation_kernel<TZ, TU, 32, 4><<<(unsigned)ceil_div64(rows, 8), 256, 0, ctx->stream>>>(
         z, u, indices, loss, stats, rows, (int)classes, top, temperature, 1);
     return post_launch(ctx, "distillationLoss (warps)");
   }
-  // few rows: up to 8 blocks share one, while each still has 8192 classes or more
+  // few rows: up to 8 blocks share one, while each still has 8192 classes or more (7 rows of 131101: 6 us, 12
+  // with a block each)
   int C = 1;
   while (C < 8 && rows * C * 2 <= 2 * ctx->sm_count && classes / (2 * C) >= 8192) C *= 2;
   cudaLaunchConfig_t cfg = {};
@@ -464,7 +473,9 @@ template <typename TZ, typename TU>
 int launch_backward(tfjs_cuda_ctx* ctx, const float* dloss, const Operands& o, const float* stats, float* dz,
                     int64_t rows, int64_t classes, int top, float temperature) {
   constexpr int V = 4;
-  const bool warps = classes <= 32 * kGradBatch * V && top <= 128;
+  // a warp takes up to four tiles of 1024 classes: a block's tile is 8192 (8192 rows of 1000 classes: 11 us, 31
+  // with blocks; of 4000 40 and 50; of 8000 half 87 and 74)
+  const bool warps = classes <= 4 * 32 * kGradBatch * V && top <= 128;
   const int G = warps ? 32 : kGradThreads, groups = kGradThreads / G;
   const int64_t tiles = classes <= G * kGradBatch * V ? 1 : ceil_div64(classes, (int64_t)G * kGradBatch * V);
   const int64_t blocks = ceil_div64(rows * tiles, groups);

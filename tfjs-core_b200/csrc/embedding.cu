@@ -1,7 +1,17 @@
 // Embedding lookup with scaling, and the gradient of its table.
 //
 //   out[t] = scale * table[i_t],      zeros where i_t lies outside [0, vocab) (padding)
-//   dtable[v] = scale * sum of dy[t] over the tokens t with i_t == v, in the order of t
+//   dtable[v] = scale * sum of dy[t] over the tokens t with i_t == v
+//
+// The lookup is bound by the bytes of the result.  The gradient writes the whole table and reads dy; adding
+// rows with atomics would make the result's last bits depend on their order, so the tokens are sorted by table
+// row first and each table row has its rows of dy added in a fixed order: three launches,
+//   sort   one cluster sorts up to 65536 (row, token) pairs in shared memory while all other blocks write the
+//          table's zeros (32000 x 768, 16384 tokens: 18 us; the zeros alone need 16, the sort alone 11)
+//   sum    a warp adds 16 or 32 sorted tokens over 128 columns and writes the rows that end within them
+//          (12 us: 50 MB of dy, latency as much as bandwidth)
+//   join   rows that go on over several warps' tokens have their shares added, in order (6 us)
+// Sums are float32; the scale multiplies each finished sum.
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -491,6 +501,7 @@ void lookup_lanes(tfjs_cuda_ctx* ctx, const LookupArgs& a) {
 template <typename TT, typename TO, int V>
 void lookup_width(tfjs_cuda_ctx* ctx, const LookupArgs& a) {
   constexpr int U = sizeof(TT) == 1 ? 8 : 4;
+  // narrow rows share a warp: 500000 tokens x 16 columns 22 us, 58 with a warp each
   if (a.width <= 8 * V) lookup_lanes<TT, TO, V, 8, 1>(ctx, a);
   else if (a.width <= 64 * V) lookup_lanes<TT, TO, V, 32, 2>(ctx, a);
   else lookup_lanes<TT, TO, V, 32, U>(ctx, a);
@@ -583,8 +594,9 @@ int sum_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, const uint2* sorted, f
 
 template <typename TD>
 int launch_gradient(tfjs_cuda_ctx* ctx, const GradientArgs& a) {
-  // one cluster, 1024 keys a block and more (below that a block's passes cost more than they share out), or
-  // tiles of 2048 keys, of 8192 where there are so many that their counts would grow past the keys
+  // One cluster, up to 1024 keys a block (4000 keys: 10 us with four blocks, 14 with one; 8000: 10 with eight,
+  // 20), as long as eight blocks hold them (65536 keys: 26 us beside the zeros, where tiles take 50 after them).
+  // Else tiles of 2048 keys, of 8192 where there are so many that their counts would grow past the keys.
   const bool cluster = a.tokens <= 8 * kSortKeys;
   int64_t tiles = 1;
   int share = a.tokens > (1 << 20) ? kSortKeys : 2048;
@@ -594,7 +606,9 @@ int launch_gradient(tfjs_cuda_ctx* ctx, const GradientArgs& a) {
   } else {
     tiles = ceil_div64(a.tokens, share);
   }
-  const bool long_chunks = a.tokens >= 32768;  // fewer shares to join, once 16 tokens a warp fill the SMs twice over
+  // 32 tokens a warp leave fewer shares to join (65536 tokens x 768: the join 14 us, 25 with 16 tokens a warp),
+  // 16 make more warps (1021 tokens x 130: the sums 5 us, 10 with 32); at 16384 tokens both take the same
+  const bool long_chunks = a.tokens >= 32768;
   const int64_t chunks = ceil_div64(a.tokens, long_chunks ? 32 : 16);
   const size_t pair_bytes = (size_t)(a.tokens + 1) / 2 * 16, partial_bytes = (size_t)(chunks * 2 * a.width) * 4;
   const size_t count_bytes = cluster ? 0 : (size_t)tiles * kMaxBins * 4;

@@ -8,18 +8,24 @@
 // store.  Every sum has a fixed order, so equal inputs give equal bits.
 //
 // Forward.  A row is read once and stays on chip: the mean and then the centred square sum (which
-// does not cancel, unlike E[x^2] - m^2) come from the same registers.  Three forms by width:
-//   up to 1024     L lanes a row (4 .. 32), no shared memory
-//   up to 16384    one block a row
+// does not cancel, unlike E[x^2] - m^2) come from the same registers.  By width:
+//   up to 1024     L lanes a row (4 .. 32), no shared memory (32768 x 1024: 45 us, 6.0 TB/s; a block a row 62)
+//   up to 16384    one block a row (2048 x 16384: 48 us, 5.6 TB/s; clusters 66)
 //   either         where rows start off the 16-byte boundaries, a warp or a block with a ring of rows in
-//                  shared memory
+//                  shared memory (33000 x 1001 half: 39 us; one value a load 93)
 //   above          a cluster of 1 to 8 blocks a row, the row in their shared memory, sums joined over DSMEM
+//                  (1000 x 33000: 76 us, 3.5 TB/s)
+// The first two are bound by memory, the ring by its instructions (4-byte words instead of 16), the clusters
+// by the latency of a row: load, two cluster-wide joins, store.
 // Gradient.  One pass over dy and x gives dx and, per block, the weights' gradients:
 //   up to 8192     persistent blocks; a ring of stages (several rows each) filled by cp.async.  First
 //                  the lanes of a row sum a and a n, then every thread takes the same columns of every
-//                  row: it writes dx and keeps its columns' dg, db in registers.
-//   above          a cluster of 1 to 8 blocks a row; dg, db add up in the blocks' shared memory
-// and a second kernel adds the blocks' partial dg, db in order.
+//                  row: it writes dx and keeps its columns' dg, db in registers.  16384 x 1024: 37 us, 5.4 TB/s
+//                  (with 8 KB rows and 512 threads, whose fixed cost a stage was 60 % of all instructions, 68);
+//                  4096 x 8192: 79 us, clusters 141
+//   above          a cluster of 1 to 8 blocks a row; dg, db add up in the blocks' shared memory.  1000 x 33000:
+//                  185 us, bound by the latency of a row
+// and a second kernel adds the blocks' partial dg, db in order (4 us at 16384 x 1024, 2.4 MB from L2).
 #include <cooperative_groups.h>
 
 #include "common.cuh"
@@ -59,19 +65,19 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 }
 
 // ---- forward -------------------------------------------------------------------------------------
-// L lanes a row, NV vectors of V values a lane: width <= L * NV * V, a multiple of V.  Up to 16 values a
-// lane, gamma and beta are fetched with the row; with more, the registers serve more rows at once instead.
+// L lanes a row, NV vectors of V values a lane: width <= L * NV * V, a multiple of V.  gamma and beta come from
+// L1 when the row is finished: fetched with the row they took registers from other rows in flight (100352 x
+// 256 float32 36 us so, 34 us now; 25088 x 512 half 16 and 13.5 us).
 template <typename TX, typename TY, int V, int NV, int L>
 __global__ void __launch_bounds__(256) layer_norm_lanes_kernel(const TX* __restrict__ x, const float* __restrict__ gamma,
                                                               const float* __restrict__ beta, TY* __restrict__ y,
                                                               float* __restrict__ stats, int64_t rows, int width,
                                                               float epsilon) {
-  constexpr bool kAhead = NV * V <= 16;
   const int lane = threadIdx.x & (L - 1);
   const int64_t row = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   const bool there = row < rows;  // lanes without a row go along, for the shuffles
   const TX* r = x + row * width;
-  float v[NV][V], g[kAhead ? NV : 1][V], b[kAhead ? NV : 1][V];
+  float v[NV][V];
 #pragma unroll
   for (int i = 0; i < NV; i++) {
     const int col = (i * L + lane) * V;
@@ -80,19 +86,6 @@ __global__ void __launch_bounds__(256) layer_norm_lanes_kernel(const TX* __restr
     } else {
 #pragma unroll
       for (int k = 0; k < V; k++) v[i][k] = 0.f;
-    }
-  }
-  if constexpr (kAhead) {
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int col = (i * L + lane) * V;
-#pragma unroll
-      for (int k = 0; k < V; k++) {
-        g[i][k] = 1.f;
-        b[i][k] = 0.f;
-      }
-      if (gamma && col < width) load_vec<V>(gamma + col, g[i]);
-      if (beta && col < width) load_vec<V>(beta + col, b[i]);
     }
   }
   float s = 0.f;
@@ -117,14 +110,7 @@ __global__ void __launch_bounds__(256) layer_norm_lanes_kernel(const TX* __restr
   for (int i = 0; i < NV; i++) {
     const int col = (i * L + lane) * V;
     if (col >= width) break;
-    if constexpr (kAhead) {
-      float o[V];
-#pragma unroll
-      for (int k = 0; k < V; k++) o[k] = (v[i][k] - mean) * rstd * g[i][k] + b[i][k];
-      store_vec<V>(y + row * width + col, o);
-    } else {
-      finish_vec<V>(v[i], mean, rstd, gamma, beta, col, y + row * width + col);
-    }
+    finish_vec<V>(v[i], mean, rstd, gamma, beta, col, y + row * width + col);
   }
   if (stats && lane == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(mean, rstd);
 }
@@ -430,6 +416,9 @@ struct StagedParams {
 constexpr int kStages = 3;
 
 // MC vectors of V columns a thread: width <= 256 * MC * V, a multiple of V.
+// The products of dx are rounded before they are added or subtracted (no contraction): in rows of one or two
+// columns the terms cancel, and a product kept unrounded on one side only would leave its rounding error,
+// times rstd, where the formula gives 0.
 template <typename TD, typename TX, int V, int MC>
 __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(const TD* __restrict__ dy,
                                                                               const TX* __restrict__ x,
@@ -490,7 +479,7 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
     {
       float sa = 0.f, sn = 0.f;
       if (row1 < n) {
-        const float m = ss[row1].x;
+        const float2 mr = ss[row1];
         const TD* d1 = sd + row1 * width;
         const TX* x1 = sx + row1 * width;
 #pragma unroll 4
@@ -501,9 +490,9 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
           load_vec<V>(s_gamma + j * V, g);
 #pragma unroll
           for (int k = 0; k < V; k++) {
-            const float a = d[k] * g[k];
+            const float a = __fmul_rn(d[k], g[k]);
             sa += a;
-            sn = fmaf(a, v[k] - m, sn);
+            sn += __fmul_rn(a, __fmul_rn(v[k] - mr.x, mr.y));
           }
         }
       }
@@ -525,7 +514,7 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
           t.x += o.x;
           t.y += o.y;
         }
-        const float ma = t.x * inv, man = t.y * mr.y * inv;
+        const float ma = t.x * inv, man = t.y * inv;
         const TD* d2 = sd + row * width;
         const TX* x2 = sx + row * width;
         float* out = p.dx + (row0 + row) * width;
@@ -539,8 +528,8 @@ __global__ void __launch_bounds__(kStagedThreads, 2) layer_norm_staged_kernel(co
           load_vec<V>(s_gamma + c * V, g);
 #pragma unroll
           for (int k = 0; k < V; k++) {
-            const float nn = (v[k] - mr.x) * mr.y;
-            o[k] = mr.y * fmaf(-nn, man, fmaf(d[k], g[k], -ma));
+            const float nn = __fmul_rn(v[k] - mr.x, mr.y);
+            o[k] = mr.y * ((__fmul_rn(d[k], g[k]) - ma) - __fmul_rn(nn, man));
             dg[i][k] = fmaf(d[k], nn, dg[i][k]);
             db[i][k] += d[k];
           }
@@ -782,8 +771,8 @@ cudaError_t launch_clusters(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), int64
 template <typename TX, typename TY, int V>
 int cluster_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   // Blocks a row: so many that three blocks' shares fit into an SM's shared memory (one loads while another
-  // sums), and with few rows so many that the SMs have a block each.  Every block costs each row two
-  // cluster-wide waits of about a microsecond: 1000 x 33000 is 137 us with 8 blocks a row.
+  // sums), and with few rows so many that the SMs have a block each.  1000 x 33000: 76 us with the two that
+  // gives, 94 with one, 151 with eight; 8 x 33000: 7 us with eight, 12 with one.
   const auto share_of = [&](int C) { return (ceil_div64(a.width / V, C) * V * (int64_t)sizeof(TX) + 31) / 16 * 16; };
   int C = 1;
   while (C < 8 && (share_of(C) > 72 * 1024 || a.rows * C < ctx->sm_count)) C *= 2;
