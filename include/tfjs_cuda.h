@@ -177,7 +177,8 @@ int tfjs_cuda_event_wait(tfjs_cuda_event* ev, int timeout_ms);
 int tfjs_cuda_event_destroy(tfjs_cuda_event* ev);
 /* Idempotent, like backend_cpu.ts:228-237; unknown ids are ignored. */
 int tfjs_cuda_tensor_dispose(tfjs_cuda_ctx* ctx, tfjs_tensor_id id);
-/* Device pointer and byte size of a tensor's storage (zero-copy interop, benchmarks). */
+/* Device pointer and byte size of a tensor's storage (zero-copy interop, benchmarks).  Work enqueued on the
+ * context's stream from now on runs after an asynchronous upload of the tensor. */
 int tfjs_cuda_tensor_device_ptr(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, void** ptr, size_t* nbytes);
 /* Pinned host staging memory for write/read_async callers. */
 int tfjs_cuda_host_alloc(void** ptr, size_t nbytes);

@@ -252,6 +252,21 @@ def test_embedding_lookup_backprop_of_many_tokens(tf, count, vocab, width):
     _within(out.dataSync(), want, (named + 2) * U * total)
 
 
+@pytest.mark.parametrize("count", [1, 16, 17, 1000, 8192, 40000, 65536, 66000])
+@pytest.mark.parametrize("token", [-1, 0, 4, 5])
+def test_embedding_gradient_of_one_token_throughout(tf, count, token):
+    bk = tf.ENGINE.backend
+    dy = _rng(count).normal(0, 1, (count, 20)).astype(np.float32)
+    idx = np.full(count, token, np.int32)
+    got = bk.embeddingLookupBackprop(tf.ops.tensor(dy), tf.ops.tensor(idx, dtype="int32"), 5, 0.5).dataSync().reshape(5, 20)
+    want, off = np.zeros((2, 5, 20))
+    if 0 <= token < 5:
+        want[token] = dy.astype(np.float64).sum(0) * 0.5
+        # chains: 32 tokens a share, an eighth of the shares a warp, 8 warps
+        off[token] = (32 + count / 256 + 16) * U * np.abs(dy).sum(0) * 0.5 + U * np.abs(want[token])
+    _within(got, want, off)
+
+
 def test_embedding_gradient_keeps_special_values_in_their_rows(tf):
     bk = tf.ENGINE.backend
     idx = np.array([2, 0, 2, -1, 0, 5], np.int32)
@@ -785,6 +800,57 @@ def test_operands_of_other_storage_and_dtype_are_converted(tf):
     table = _rng(2).normal(0, 1, (4, 3)).astype(np.float32)
     out = bk.embeddingLookup(tf.ops.tensor(table), tf.ops.cast(tf.ops.tensor([1, 0, 1], dtype="bool"), "int32"))
     assert np.array_equal(out.dataSync().reshape(3, 3), table[[1, 0, 1]])
+
+
+def test_single_rows_without_a_batch_axis(tf):
+    ops = tf.ops
+    rng = _rng(51)
+    z, u = rng.normal(0, 2, 40).astype(np.float32), rng.normal(0, 2, 3).astype(np.float32)
+    idx = np.array([3, 39, 7], np.int32)
+    loss, (dz,) = ops.value_and_grads(lambda v: ops.distillation_loss(v, ops.tensor(u), ops.tensor(idx, dtype="int32"), 2.0))([ops.tensor(z)])
+    want, off, dwant, doff, _ = _distillation_reference(z[None], u[None], idx[None], np.ones(1), 2.0)
+    assert loss.shape == [] and dz.shape == [40]
+    _within(loss.dataSync(), want, off)
+    _within(dz.dataSync(), dwant, doff.reshape(1, 40))
+    y, off, _, _ = _ln_reference(z[None], np.ones(40, np.float32), np.zeros(40, np.float32))
+    _within(ops.layer_norm(ops.tensor(z)).dataSync(), y, off)
+    assert ops.embedding_lookup(ops.tensor(z.reshape(10, 4)), ops.scalar(9, "int32")).dataSync().tolist() == z[36:].tolist()
+
+
+def test_threads_with_contexts_of_their_own(tf):
+    """Two host threads, each with its context on the same device, at sizes that need different shared memory."""
+    import threading
+    from tfjs_core_b200 import BackendCuda
+    failures = []
+
+    def work(widths, seed):
+        try:
+            bk = BackendCuda(0)
+            lib, ctx = bk._lib, bk._ctx
+            rng = _rng(seed)
+            for repeat in range(40):
+                for rows, width in widths:
+                    arrays = [rng.normal(0, 1, (rows, width)).astype(np.float32), rng.normal(0, 1, (rows, width)).astype(np.float32)]
+                    arrays.append(np.stack([arrays[1].mean(-1), 1 / np.sqrt(arrays[1].var(-1) + EPS)], -1).astype(np.float32))
+                    ids = []
+                    for a in arrays + [np.zeros((rows, width), np.float32), np.zeros(width, np.float32), np.zeros(width, np.float32)]:
+                        ids.append(bk._new_id(a.shape, "float32"))
+                        bk._check(lib.tfjs_cuda_tensor_write(ctx, ids[-1], np.ascontiguousarray(a).ctypes.data_as(C.c_void_p), a.nbytes))
+                    bk._check(lib.tfjs_cuda_layer_norm_backprop(ctx, ids[0], ids[1], 0, ids[2], *ids[3:], rows, width))
+                    out = np.empty((rows, width), np.float32)
+                    bk._check(lib.tfjs_cuda_tensor_read(ctx, ids[3], out.ctypes.data_as(C.c_void_p), out.nbytes))
+                    (want, off), _, _ = _ln_backward_reference(arrays[0], arrays[1], np.ones(width, np.float32), arrays[2])
+                    _within(out, want, off)
+                    bk._free_tmp(*ids)
+            bk.dispose()
+        except BaseException as e:   # seen by the main thread
+            failures.append(repr(e)[:500])
+    threads = [threading.Thread(target=work, args=a) for a in (([(2, 8192), (3, 4096)], 1), ([(64, 1020), (40, 2048)], 2))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(120)
+    assert not failures, failures
 
 
 def test_upload_in_flight_is_waited_for(tf):

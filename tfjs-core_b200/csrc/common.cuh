@@ -194,6 +194,15 @@ inline void launch_dependent(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), dim3
   cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
+// Lets a kernel take more than 48 KB of dynamic shared memory: always up to the same bound, so that two
+// threads whose contexts launch it with different sizes cannot lower the other's between this and its launch.
+constexpr size_t kMostSmem = 226 * 1024;  // of the 227 KB of a block; the kernels' static arrays take the rest
+template <typename Kernel>
+inline cudaError_t allow_smem(Kernel kernel, size_t smem) {
+  if (smem > kMostSmem) return cudaErrorInvalidValue;
+  return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem) : cudaSuccess;
+}
+
 // Allocator (context.cu).
 int ctx_alloc(tfjs_cuda_ctx* ctx, size_t nbytes, void** ptr, size_t* capacity);
 void ctx_free(tfjs_cuda_ctx* ctx, void* ptr, size_t capacity);

@@ -700,7 +700,9 @@ extern "C" int tfjs_cuda_tensor_device_ptr(tfjs_cuda_ctx* ctx, tfjs_tensor_id id
   if (!t) return set_error(ctx, TFJS_CUDA_ERR_NOT_FOUND, "unknown tensor id %lld", (long long)id);
   if (ptr) *ptr = t->ptr;
   if (nbytes) *nbytes = t->nbytes;
-  return TFJS_CUDA_OK;
+  if (!t->copy_pending) return TFJS_CUDA_OK;
+  cudaSetDevice(ctx->device);
+  return wait_for_upload(ctx, t);  // whoever orders itself after the context's stream sees the upload too
 }
 
 extern "C" int tfjs_cuda_host_alloc(void** ptr, size_t nbytes) {

@@ -533,8 +533,7 @@ int sort_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, uint2* const* buffers
   if (!counts) {
     const int blocks = (int)tiles;
     const int smem = (int)SortView::bytes(share, 2, bins);
-    if (smem > 48 * 1024)
-      TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(embedding_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    TFJS_CHECK_CUDA(ctx, allow_smem(embedding_sort_kernel, smem));
     const int64_t zero_blocks = ceil_div64(a.vocab * a.width, 4 * kZeroQuads);
     const int64_t grid = blocks + ceil_div64(zero_blocks, blocks) * blocks;
     TFJS_REQUIRE(ctx, grid < (1ll << 31), "embeddingLookupBackprop: the table is too large");
@@ -556,10 +555,8 @@ int sort_tokens(tfjs_cuda_ctx* ctx, const GradientArgs& a, uint2* const* buffers
   }
   const int smem = (int)SortView::bytes(share, 1, bins);
   auto count = embedding_tile_kernel<false>, place = embedding_tile_kernel<true>;
-  if (smem > 48 * 1024) {
-    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(count, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  }
+  TFJS_CHECK_CUDA(ctx, allow_smem(count, smem));
+  TFJS_CHECK_CUDA(ctx, allow_smem(place, smem));
   TFJS_CHECK_CUDA(ctx, cudaMemsetAsync(a.dtable, 0, (size_t)(a.vocab * a.width) * 4, ctx->stream));
   for (int pass = 0; pass < d.passes; pass++) {
     const int32_t* indices = pass == 0 ? a.indices : nullptr;

@@ -750,10 +750,6 @@ struct ClusterLaunch {
   }
 };
 template <typename Kernel>
-cudaError_t allow_smem(Kernel kernel, size_t smem) {
-  return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) : cudaSuccess;
-}
-template <typename Kernel>
 cudaError_t clusters_at_once(Kernel kernel, int C, size_t smem, int* most) {
   const cudaError_t e = allow_smem(kernel, smem);
   if (e != cudaSuccess) return e;
@@ -811,8 +807,7 @@ int ring_launch(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   const int slot_bytes = ((int)a.width * (int)sizeof(TX) + 31) / 16 * 16;  // one unit more for the row's own offset
   const int smem = groups * 2 * slot_bytes + (G == 32 ? P * ((int)a.width / P + 1) * 2 * P * 4 : 0);
   auto kernel = layer_norm_ring_kernel<TX, TY, NW, G>;
-  if (smem > 48 * 1024)
-    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  TFJS_CHECK_CUDA(ctx, allow_smem(kernel, smem));
   const int per_sm = smem <= 36 * 1024 ? 6 : smem <= 55 * 1024 ? 4 : smem <= 74 * 1024 ? 3 : 2;
   kernel<<<grid_rows(ctx, ceil_div64(a.rows, groups), per_sm), kRingThreads, smem, ctx->stream>>>(
       (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon, slot_bytes);
@@ -883,8 +878,7 @@ int join_sums(tfjs_cuda_ctx* ctx, const BackwardArgs& a, const void* partial, in
 template <typename TD, typename TX, int V, int MC>
 int staged_launch(tfjs_cuda_ctx* ctx, const BackwardArgs& a, StagedParams& p, int blocks, size_t smem) {
   auto kernel = layer_norm_staged_kernel<TD, TX, V, MC>;
-  if (smem > 48 * 1024)
-    TFJS_CHECK_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  TFJS_CHECK_CUDA(ctx, allow_smem(kernel, smem));
   kernel<<<blocks, kStagedThreads, smem, ctx->stream>>>((const TD*)a.dy, (const TX*)a.x, p);
   return post_launch(ctx, "layerNormBackprop");
 }
