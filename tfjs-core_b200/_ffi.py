@@ -142,9 +142,15 @@ def load():
     return _lib
 
 
-_SHAPE = [C.c_int64 * max(rank, 1) for rank in range(9)]   # the library takes ranks up to 8
+_shapes = {}
 
 
 def shape_array(shape):
-    rank = len(shape)
-    return (_SHAPE[rank] if rank < 9 else C.c_int64 * rank)(*map(int, shape))
+    """The shape as the library takes it; the same array for the same shape (the library only reads it)."""
+    key = tuple(shape)
+    array = _shapes.get(key)
+    if array is None:
+        if len(_shapes) >= 4096:
+            _shapes.clear()
+        array = _shapes[key] = (C.c_int64 * max(len(key), 1))(*map(int, key))
+    return array

@@ -127,14 +127,14 @@ class BackendCuda:
                 self._lib.tfjs_cuda_tensor_dispose(self._ctx, i)
 
     def _out(self, shape, dtype="float32"):
-        return Tensor.make(shape, {}, dtype, self)
+        return Tensor(shape, dtype, None, None, self)   # Tensor.make(shape, {}, dtype, self)
 
     def _out_activation(self, shape, storage=None):
         """Output of a convolution: a float32 tensor whose storage follows the activation-storage
         mode (or `storage` when the caller names one)."""
         self._pending_storage = storage or self.activation_storage
         try:
-            return Tensor.make(shape, {}, "float32", self)
+            return Tensor(shape, "float32", None, None, self)
         finally:
             self._pending_storage = None
 

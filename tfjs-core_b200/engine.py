@@ -176,12 +176,11 @@ class Engine:
         if info is None:
             b = backend or self.backend
             nbytes = t.size * (1 if t.dtype == "bool" else 4)
-            self.tensorInfo[t.dataId] = {"backend": b, "refCount": 0, "shape": t.shape,
-                                         "dtype": t.dtype, "bytes": nbytes}
+            info = {"backend": b, "refCount": 0, "shape": t.shape, "dtype": t.dtype, "bytes": nbytes}
+            self.tensorInfo[t.dataId] = info
             self.numBytes += nbytes
             self.numDataBuffers += 1
             b.register(t.dataId, t.shape, t.dtype)
-            info = self.tensorInfo[t.dataId]
         info["refCount"] += 1
         if self.scopeStack:
             self.scopeStack[-1]["track"].append(t)
