@@ -232,13 +232,13 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_sort_kernel(const i
       }
     }
     const bool last = pass + 1 == passes;
-    // The last pass writes to global memory only: its barrier, which keeps the blocks until their totals
-    // have been read, is entered here, so that it does not wait for those writes (they queue behind the
-    // other blocks' zeros).
-    if (last) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     const uint32_t smaller = block_exclusive(all, s.warps);
     if ((int)threadIdx.x < bins) s.base[threadIdx.x] = smaller + before;
     __syncthreads();
+    // The last pass writes to global memory only: its barrier, which keeps the blocks until the others have
+    // read their totals, is entered here, so that it does not wait for those writes (they queue behind the
+    // other blocks' zeros).  The totals that this block read have been used by now.
+    if (last) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < kKeysPerThread; i++) {
       if (digit[i] == ~0u) continue;
@@ -324,10 +324,12 @@ __global__ void __launch_bounds__(kSortThreads, 1) embedding_scan_kernel(uint32_
 // that begins here and goes on in partial[chunk][1].
 constexpr int kBatch = 4;  // rows of dy in flight a warp
 constexpr int kSumThreads = 128;
+// In this kernel and the next, what the kernel before wrote is read through pointers without __restrict__: a load
+// that the compiler may take for one of constant data could be moved ahead of pdl_wait().
 
 template <typename TD, int V, int CH>
 __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const TD* __restrict__ dy,
-                                                                const uint2* __restrict__ sorted,
+                                                                const uint2* sorted,
                                                                 float* __restrict__ dtable, float* __restrict__ partial,
                                                                 int64_t tokens, uint32_t vocab, int64_t width, float scale,
                                                                 int64_t tiles, int64_t items) {
@@ -407,8 +409,8 @@ __device__ __forceinline__ void add_shares(const float* partial, int64_t lo, int
   }
 }
 template <int V, int CH>
-__global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint2* __restrict__ sorted,
-                                                                 const float* __restrict__ partial,
+__global__ void __launch_bounds__(kThreads) embedding_join_kernel(const uint2* sorted,
+                                                                 const float* partial,
                                                                  float* __restrict__ dtable, int64_t tokens,
                                                                  uint32_t vocab, int64_t width, float scale,
                                                                  int64_t chunks) {

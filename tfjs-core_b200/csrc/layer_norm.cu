@@ -668,8 +668,10 @@ __global__ void __launch_bounds__(kClusterThreads, 2) layer_norm_backprop_cluste
 
 // out[j] = sum over the blocks of partial[block][j]; j runs over dg and then db.  Many blocks: 32 columns a
 // block, 32 threads a column take every 32nd block's row and join theirs in order.  Up to 64: a thread a column.
+// `partial` comes without __restrict__: a load that the compiler may take for one of constant data could be moved
+// ahead of pdl_wait().
 constexpr int kJoinThreads = 1024, kFewBlocks = 64;
-__global__ void __launch_bounds__(kJoinThreads) layer_norm_join_kernel(const float* __restrict__ partial,
+__global__ void __launch_bounds__(kJoinThreads) layer_norm_join_kernel(const float* partial,
                                                                       float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                                       int blocks, int64_t width) {
   __shared__ float part[32][33];
@@ -693,7 +695,7 @@ __global__ void __launch_bounds__(kJoinThreads) layer_norm_join_kernel(const flo
     __syncthreads();
   }
 }
-__global__ void __launch_bounds__(256) layer_norm_join_few_kernel(const float* __restrict__ partial,
+__global__ void __launch_bounds__(256) layer_norm_join_few_kernel(const float* partial,
                                                                  float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                                  int blocks, int64_t width) {
   const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
