@@ -335,7 +335,14 @@ export class BackendCuda extends KernelBackend {
       throw new Error(`storage must be 'float32', 'int32' or 'float16', got ${storage}`);
     }
     const t = storage === 'int32' ? this.makeOutput<Tensor>(shape, 'int32') : this.makeActivation<Tensor>(shape, storage);
-    if (values != null) this.write(t.dataId, values);
+    if (values != null) {
+      try {
+        this.write(t.dataId, values);
+      } catch (e) {
+        t.dispose();
+        throw e;
+      }
+    }
     return t;
   }
 

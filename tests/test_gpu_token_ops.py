@@ -745,6 +745,8 @@ def test_refusals_leave_the_context_usable(tf):
         lambda: bk.distillationLossBackprop(z(3), z(2, 8), z(2, 2), i(2, 2), z(2, 4)),
         lambda: bk.distillationLossBackprop(z(2), z(2, 8), z(2, 2), i(2, 2), z(2, 3)),
         lambda: bk.layerNorm(bk.registerQuantized([2, 8], np.zeros(16), 1, 0), None, None, EPS),
+        lambda: bk.registerStored([3], "float32", np.zeros(2)),
+        lambda: bk.registerStored([3], "float16", np.zeros(4)),
     ]
     for call in calls:
         with pytest.raises(CudaError):

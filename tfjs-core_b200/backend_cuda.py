@@ -321,7 +321,11 @@ class BackendCuda:
         finally:
             self._pending_storage = None
         if values is not None:
-            ENGINE.write(self, t.dataId, values)
+            try:
+                ENGINE.write(self, t.dataId, values)
+            except Exception:
+                t.dispose()
+                raise
         return t
 
     def deviceArray(self, t):
