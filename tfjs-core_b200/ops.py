@@ -711,14 +711,27 @@ def embedding_lookup(table, indices, scale=1.0):
     _assert(indices.dtype == "int32",
             f"Argument 'indices' passed to 'embeddingLookup' must be int32 tensor, but got {indices.dtype} tensor")
 
+    return _lookup(table, indices, scale, None)
+
+
+def _lookup(table, indices, scale, storage):
     def forward(b, save):
         save([indices])
-        return b.embeddingLookup(table, indices, scale)
+        return b.embeddingLookup(table, indices, scale, storage)
 
     def backward(dy, saved):
-        return {"table": lambda: ENGINE.runKernel(
-            lambda b: b.embeddingLookupBackprop(dy, saved[0], table.shape[0], scale), "embeddingLookupBackprop")}
+        return {"table": lambda: _lookup_gradient(dy, saved[0], table.shape[0], scale)}
     return ENGINE.runKernel(forward, "embeddingLookup", {"table": table}, backward)
+
+
+def _lookup_gradient(dy, indices, vocab, scale):
+    """The gradient of the table.  It is linear in dy, and its own gradient is the lookup: a gradient, so
+    it is stored as float32 in half-storage mode too."""
+    def forward(b, save):
+        save([indices])
+        return b.embeddingLookupBackprop(dy, indices, vocab, scale)
+    return ENGINE.runKernel(forward, "embeddingLookupBackprop", {"dy": dy},
+                            lambda ddtable, saved: {"dy": lambda: _lookup(ddtable, saved[0], scale, "float32")})
 
 
 def distillation_loss(logits, teacherLogits, teacherIndices, temperature=1.0):
