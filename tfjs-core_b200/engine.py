@@ -255,13 +255,13 @@ class Engine:
         # not the kernels a kernel calls, and only while some gradients() scope is open
         tape_on = self.gradientDepth > 0 and self.kernelDepth == 0
         self.kernelDepth += 1
-        saved = []
+        saved, clones = [], []
 
         def save(tensors):
             # not saved unless recording: nothing would ever dispose the kept clones
             if tape_on:
                 for t in tensors:
-                    saved.append(self.keep(self._clone_on_tape(t)))
+                    saved.append(self.keep(self._clone_on_tape(t, clones)))
         try:
             if name:
                 self.kernelNames.append(name)
@@ -277,16 +277,21 @@ class Engine:
             self.activeTape.append({"id": self.nextTapeNodeId, "name": name, "inputs": dict(inputs),
                                     "outputs": [result], "saved": saved,
                                     "gradient": (lambda dy, _s=saved: backward(dy, _s))})
+        # behind the kernel's own node: a clone of its result comes after the node that makes the result,
+        # or a walk along the tape would not find the way from the kernel's inputs to the clone
+        for node in clones:
+            self.nextTapeNodeId += 1
+            self.activeTape.append(dict(node, id=self.nextTapeNodeId))
         return result
 
-    def _clone_on_tape(self, x):
-        """engine.ts:401-409 clone(): an alias of x recorded on the tape as an identity node.  The
-        saved tensors of a kernel are such clones; the node keeps them connected to x, which is
+    @staticmethod
+    def _clone_on_tape(x, nodes):
+        """engine.ts:401-409 clone(): an alias of x recorded as an identity node, which goes to `nodes`.
+        The saved tensors of a kernel are such clones; the node keeps them connected to x, which is
         what lets an outer gradients() differentiate through an inner backward pass."""
         y = Tensor(x.shape, x.dtype, None, x.dataId)
-        self.nextTapeNodeId += 1
-        self.activeTape.append({"id": self.nextTapeNodeId, "name": "clone", "inputs": {"x": x}, "outputs": [y],
-                                "saved": [], "gradient": (lambda dy: {"x": lambda: dy.clone()})})
+        nodes.append({"name": "clone", "inputs": {"x": x}, "outputs": [y], "saved": [],
+                      "gradient": (lambda dy: {"x": lambda: dy.clone()})})
         return y
 
     def keep(self, t):
