@@ -83,3 +83,62 @@ def test_embedding_lookup_three_times(host):  # noqa: F811
     f = lambda x: ops.sum(ops.square(ops.square(ops.embedding_lookup(x, ti, 2.0))))  # noqa: E731
     g = ops.grad(ops.grad(ops.grad(f)))(ops.tensor(t))
     np.testing.assert_allclose(g.dataSync(), [384.0, 0.0, 384.0], rtol=TOL)
+
+
+def _normalised(x, epsilon):
+    c = x - x.mean(-1, keepdims=True)
+    r = 1 / np.sqrt((c * c).mean(-1, keepdims=True) + epsilon)
+    return c * r, r
+
+
+def _layer_norm_gradients(dy, x, gamma, epsilon):
+    n, r = _normalised(x, epsilon)
+    a = dy * gamma
+    dx = r * (a - a.mean(-1, keepdims=True) - n * (a * n).mean(-1, keepdims=True))
+    return dx, (dy * n).sum(0), dy.sum(0)
+
+
+@pytest.mark.parametrize("weights", [True, False])
+def test_layer_norm(host, weights):  # noqa: F811
+    rng = np.random.default_rng(1)
+    x = rng.normal(0.5, 1, (3, 5)).astype(np.float32)
+    g, b = rng.normal(1, 0.3, 5).astype(np.float32), rng.normal(0, 0.3, 5).astype(np.float32)
+    v = rng.normal(0, 1, (3, 5)).astype(np.float32)
+
+    # f = sum(v y^2) + sum(x^2), y = layer_norm(x, g, b): dy depends on y, and so on all three leaves
+    def f(p, q=None, s=None):
+        y = ops.layer_norm(p, q, s, epsilon=0.1)
+        return ops.add(ops.sum(ops.mul(ops.tensor(v), ops.square(y))), ops.sum(ops.square(p)))
+
+    def gradients(p, q=np.ones(5), s=np.zeros(5)):
+        dx, dg, db = _layer_norm_gradients(2 * v * (_normalised(p, 0.1)[0] * q + s), p, q, 0.1)
+        return [dx + 2 * p, dg, db][:3 if weights else 1]
+    _check(f, gradients, [x, g, b] if weights else [x], rng)
+
+
+def test_layer_norm_over_several_axes(host):  # noqa: F811
+    rng = np.random.default_rng(2)
+    x = rng.normal(0, 1, (2, 3, 2)).astype(np.float32)
+    g, v = rng.normal(1, 0.3, (3, 2)).astype(np.float32), rng.normal(0, 1, (2, 3, 2)).astype(np.float32)
+
+    def f(p, q):
+        return ops.sum(ops.mul(ops.tensor(v), ops.square(ops.layer_norm(p, q, axis=[1, 2], epsilon=0.1))))
+
+    def gradients(p, q):
+        x2, g1 = p.reshape(2, 6), q.reshape(6)
+        dx, dg, _ = _layer_norm_gradients(2 * v.reshape(2, 6) * _normalised(x2, 0.1)[0] * g1, x2, g1, 0.1)
+        return [dx.reshape(p.shape), dg.reshape(q.shape)]
+    _check(f, gradients, [x, g], rng)
+
+
+def test_layer_norm_three_times(host):  # noqa: F811
+    """Row [t, 0, -t], epsilon 1: y_0 = t / sqrt(2 t^2 / 3 + 1) along (1, 0, -1); the third derivative of y_0 in
+    t is the sum of the third partial derivatives along it, taken here as nested gradients along that direction."""
+    t, e = 0.7, np.array([1.0, 0.0, -1.0], np.float32)
+    along = lambda h: (lambda x: ops.sum(ops.mul(ops.grad(h)(x), ops.tensor(e))))  # noqa: E731
+    f = lambda x: ops.sum(ops.mul(ops.layer_norm(x, epsilon=1.0), ops.tensor(np.array([1.0, 0, 0], np.float32))))  # noqa: E731
+    got = float(along(along(along(f)))(ops.tensor(t * e)).dataSync()[0])
+    # d^3/dt^3 of t (1 + c t^2)^-1/2, c = 2/3: (12 c^2 t^2 - 3 c) (1 + c t^2)^-7/2
+    c = 2 / 3
+    want = (12 * c * c * t * t - 3 * c) * (1 + c * t * t) ** -3.5
+    assert abs(got - want) <= 4 * TOL * 3 * c   # the two terms of the numerator cancel in part

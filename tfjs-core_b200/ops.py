@@ -686,13 +686,15 @@ def layer_norm(x, gamma=None, beta=None, axis=-1, epsilon=1e-5):
         return y
 
     def backward(dy, saved):
+        gamma_saved = saved[2] if g1 is not None else None
+        if ENGINE.gradientDepth > 0:   # an outer gradients() records this pass
+            return _layer_norm_gradients(dy, saved[0], gamma_saved, epsilon)
         state = []
 
         def gradients():
             if not state:   # one kernel call gives all three
                 state.append(ENGINE.runKernel(
-                    lambda b: b.layerNormBackprop(dy, saved[0], saved[2] if g1 is not None else None, saved[1]),
-                    "layerNormBackprop"))
+                    lambda b: b.layerNormBackprop(dy, saved[0], gamma_saved, saved[1]), "layerNormBackprop"))
             return state[0]
         return {"x": lambda: gradients()[0], "gamma": lambda: gradients()[1], "beta": lambda: gradients()[2]}
     res = ENGINE.runKernel(forward, "layerNorm", dict(weights, x=x2), backward)
@@ -700,6 +702,25 @@ def layer_norm(x, gamma=None, beta=None, axis=-1, epsilon=1e-5):
     for t in [x2, res] + list(weights.values()):
         t.dispose()
     return out
+
+
+def _layer_norm_gradients(dy, x, gamma, epsilon):
+    """layer_norm's gradients, x [rows, width], as a chain of recorded ops: what the kernel gives, to float32
+    rounding, but differentiable in dy, x and gamma any number of times.  The inverse root is
+    exp(-log(var + epsilon) / 2), good to 2^-19 relative.  Temporaries belong to the backward pass's scope."""
+    width = x.shape[1]
+    one_over = scalar(1.0 / width if width else 0.0)
+
+    def mean(t):
+        return mul(sum(t, [1], True), one_over)
+    centred = sub(x, mean(x))
+    rstd = exp(mul(log(add(mean(square(centred)), scalar(epsilon))), scalar(-0.5)))
+    n = mul(centred, rstd)
+
+    def dx():
+        a = dy if gamma is None else mul(dy, gamma)
+        return mul(rstd, sub(sub(a, mean(a)), mul(n, mean(mul(a, n)))))
+    return {"x": dx, "gamma": lambda: sum(mul(dy, n), [0]), "beta": lambda: sum(dy, [0])}
 
 
 def embedding_lookup(table, indices, scale=1.0):
