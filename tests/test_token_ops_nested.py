@@ -7,11 +7,39 @@ chain of at most 64 of them with terms of up to 8 times the result's largest val
 import numpy as np
 import pytest
 
-from test_token_ops_host import host  # noqa: F401  (the fixture)
+from test_token_ops_host import TokenBackend
 from tfjs_core_b200 import ops
 from tfjs_core_b200.engine import ENGINE
 
 TOL = 64 * 8 * 2.0 ** -24
+
+
+class EmptyRowsBackend(TokenBackend):
+    """Like the kernels, exactly 0 in the rows whose list is empty, whatever their logits hold."""
+
+    def _there(self, logits, indices):
+        i = self._i(indices)
+        return ((i >= 0) & (i < logits.shape[-1])).any(-1)
+
+    def distillationLoss(self, logits, teacherLogits, teacherIndices, temperature=1.0, withStats=True):
+        loss, stats = super().distillationLoss(logits, teacherLogits, teacherIndices, temperature, withStats)
+        return self._make(np.where(self._there(logits, teacherIndices), self._v(loss), 0)), stats
+
+    def distillationLossBackprop(self, dloss, logits, teacherLogits, teacherIndices, stats, temperature=1.0):
+        dz = super().distillationLossBackprop(dloss, logits, teacherLogits, teacherIndices, stats, temperature)
+        return self._make(np.where(self._there(logits, teacherIndices)[..., None], self._v(dz), 0))
+
+
+@pytest.fixture()
+def host():
+    prev = ENGINE.backendName
+    bk = EmptyRowsBackend()
+    ENGINE.registerBackend("numpy-token-nested-test", lambda: bk, 1000)
+    assert ENGINE.setBackend("numpy-token-nested-test")
+    yield bk
+    ENGINE.removeBackend("numpy-token-nested-test")
+    if prev:
+        ENGINE.setBackend(prev)
 
 
 def _directional(gradients, arrays, i, at):
@@ -43,7 +71,7 @@ def _nested(f, weights):
     return outer
 
 
-def _check(f, gradients, arrays, rng):
+def _check(f, gradients, arrays, rng, tol=TOL):
     weights = [rng.normal(0, 1, a.shape).astype(np.float32) for a in arrays]
     want = _second(gradients, [a.astype(np.float64) for a in arrays], [w.astype(np.float64) for w in weights])
     tensors = [ops.tensor(a) for a in arrays]
@@ -52,10 +80,10 @@ def _check(f, gradients, arrays, rng):
     assert ENGINE.numTensors == before + len(got)   # the inner tape leaves nothing behind
     for g, w in zip(got, want):
         assert g.shape == list(w.shape)
-        np.testing.assert_allclose(g.dataSync().reshape(w.shape), w, rtol=0, atol=TOL * np.abs(w).max())
+        np.testing.assert_allclose(g.dataSync().reshape(w.shape), w, rtol=0, atol=tol * np.abs(w).max())
 
 
-def test_embedding_lookup(host):  # noqa: F811
+def test_embedding_lookup(host):
     rng = np.random.default_rng(0)
     table = rng.normal(0, 1, (5, 3)).astype(np.float32)
     idx = np.array([[1, 1], [4, -1], [7, 0]])      # a row named twice, two indices outside the table
@@ -76,7 +104,7 @@ def test_embedding_lookup(host):  # noqa: F811
     _check(f, gradients, [table], rng)
 
 
-def test_embedding_lookup_three_times(host):  # noqa: F811
+def test_embedding_lookup_three_times(host):
     """d^3/dt^3 of sum(e^4) along ones, e = 2 t[i]: 24 * 2^4 t for each place that names the row."""
     t = np.array([[1.0], [-2.0], [0.5]], np.float32)
     ti = ops.tensor(np.array([0, 2, 2, 3]), dtype="int32")
@@ -99,7 +127,7 @@ def _layer_norm_gradients(dy, x, gamma, epsilon):
 
 
 @pytest.mark.parametrize("weights", [True, False])
-def test_layer_norm(host, weights):  # noqa: F811
+def test_layer_norm(host, weights):
     rng = np.random.default_rng(1)
     x = rng.normal(0.5, 1, (3, 5)).astype(np.float32)
     g, b = rng.normal(1, 0.3, 5).astype(np.float32), rng.normal(0, 0.3, 5).astype(np.float32)
@@ -116,7 +144,7 @@ def test_layer_norm(host, weights):  # noqa: F811
     _check(f, gradients, [x, g, b] if weights else [x], rng)
 
 
-def test_layer_norm_over_several_axes(host):  # noqa: F811
+def test_layer_norm_over_several_axes(host):
     rng = np.random.default_rng(2)
     x = rng.normal(0, 1, (2, 3, 2)).astype(np.float32)
     g, v = rng.normal(1, 0.3, (3, 2)).astype(np.float32), rng.normal(0, 1, (2, 3, 2)).astype(np.float32)
@@ -131,7 +159,7 @@ def test_layer_norm_over_several_axes(host):  # noqa: F811
     _check(f, gradients, [x, g], rng)
 
 
-def test_layer_norm_three_times(host):  # noqa: F811
+def test_layer_norm_three_times(host):
     """Row [t, 0, -t], epsilon 1: y_0 = t / sqrt(2 t^2 / 3 + 1) along (1, 0, -1); the third derivative of y_0 in
     t is the sum of the third partial derivatives along it, taken here as nested gradients along that direction."""
     t, e = 0.7, np.array([1.0, 0.0, -1.0], np.float32)
@@ -142,3 +170,79 @@ def test_layer_norm_three_times(host):  # noqa: F811
     c = 2 / 3
     want = (12 * c * c * t * t - 3 * c) * (1 + c * t * t) ** -3.5
     assert abs(got - want) <= 4 * TOL * 3 * c   # the two terms of the numerator cancel in part
+
+
+def _distillation_gradient(z, u, idx, dloss, t):
+    """dloss t (q - p) of rows [rows, classes]; complex z allowed."""
+    e = np.exp(z / t - (z.real / t).max(-1, keepdims=True))
+    q = e / e.sum(-1, keepdims=True)
+    ok = (idx >= 0) & (idx < z.shape[-1])
+    w = np.where(ok, np.exp(u.astype(np.float64) / t), 0)
+    some = ok.any(-1, keepdims=True)
+    w = w / np.where(some, w.sum(-1, keepdims=True), 1)
+    p = np.zeros(z.shape)
+    for r, k in zip(*np.nonzero(ok)):
+        p[r, idx[r, k]] += w[r, k]
+    return np.where(some, dloss[:, None] * t * (q - p), 0)
+
+
+def _distillation_case(rng):
+    z = rng.normal(0, 1, (4, 6)).astype(np.float32)
+    idx = np.stack([rng.permutation(6)[:3] for _ in range(4)]).astype(np.int32)
+    idx[1] = -1                      # no teacher
+    idx[2, 1] = idx[2, 0]            # a class named twice
+    idx[3, 2] = 6                    # a shorter list
+    return z, rng.normal(0, 1, (4, 3)).astype(np.float32), idx
+
+
+@pytest.mark.parametrize("t", [1.0, 2.5])
+def test_distillation_loss(host, t):
+    rng = np.random.default_rng(3)
+    z, u, idx = _distillation_case(rng)
+    tu, ti = ops.tensor(u), ops.tensor(idx, dtype="int32")
+
+    # f = sum(c(z) loss(z)) + sum(z^2), c = (sum z)^2 of the row: the inner dloss depends on the logits too
+    def f(v):
+        c = ops.square(ops.sum(v, [1]))
+        return ops.add(ops.sum(ops.mul(c, ops.distillation_loss(v, tu, ti, t))), ops.sum(ops.square(v)))
+
+    def gradients(v):
+        s = v.sum(-1)
+        log_q = v / t - np.log(np.exp(v / t).sum(-1, keepdims=True))
+        ok = (idx >= 0) & (idx < 6)
+        w = np.where(ok, np.exp(u.astype(np.float64) / t), 0)
+        p = w / np.maximum(w.sum(-1, keepdims=True), 1e-300)
+        gap = np.log(np.where(p > 0, p, 1)) - np.take_along_axis(log_q, np.where(ok, idx, 0), -1)
+        loss = t * t * (p * gap).sum(-1)
+        return [_distillation_gradient(v, u, idx, s * s, t) + (2 * s * loss)[:, None] + 2 * v]
+    _check(f, gradients, [z], rng)
+
+
+def test_distillation_loss_leaves_out_rows_without_a_teacher(host):
+    """What such a row's logits hold does not matter to a nested gradient either."""
+    rng = np.random.default_rng(4)
+    z, u, idx = _distillation_case(rng)
+    w = rng.normal(0, 1, z.shape).astype(np.float32)
+    tu, ti, tw = ops.tensor(u), ops.tensor(idx, dtype="int32"), ops.tensor(w)
+    outer = lambda v: ops.sum(ops.mul(ops.grad(lambda s: ops.sum(ops.distillation_loss(s, tu, ti)))(v), tw))  # noqa: E731
+    want = ops.grad(outer)(ops.tensor(z)).dataSync().reshape(z.shape)
+    z[1, 2] = np.nan
+    got = ops.grad(outer)(ops.tensor(z)).dataSync().reshape(z.shape)
+    assert not got[1].any() and np.array_equal(got, want)
+
+
+def test_distillation_loss_three_times(host):
+    """Two classes with logits (t, 0) and the teacher on the second: loss = log(1 + e^t); its derivatives
+    along (1, 0) are s, s (1 - s) and s (1 - s) (1 - 2 s), s = 1 / (1 + e^-t).  The teacher of the second row
+    is equal over both classes, like its student: q - p is 0 there, its derivative is not."""
+    u, ti = ops.tensor(np.zeros((2, 2), np.float32)), ops.tensor(np.array([[1, -1], [0, 1]]), dtype="int32")
+    e = ops.tensor(np.array([[1.0, 0.0], [1.0, 0.0]], np.float32))
+    t = np.array([0.4, 0.0])
+    x = ops.tensor(np.stack([t, 0 * t], -1).astype(np.float32))
+    along = lambda h: (lambda v: ops.sum(ops.mul(ops.grad(lambda s: ops.sum(h(s)))(v), e), [1]))  # noqa: E731
+    f = lambda v: ops.distillation_loss(v, u, ti)  # noqa: E731
+    s = 1 / (1 + np.exp(-t))
+    first = s - np.array([0, 0.5])
+    for want in (first, s * (1 - s), s * (1 - s) * (1 - 2 * s)):
+        f = along(f)
+        np.testing.assert_allclose(f(x).dataSync(), want, rtol=0, atol=TOL)

@@ -779,9 +779,64 @@ def distillation_loss(logits, teacherLogits, teacherIndices, temperature=1.0):
         return loss
 
     def backward(dy, saved):
-        return {"logits": lambda: ENGINE.runKernel(
-            lambda b: b.distillationLossBackprop(dy, *saved, temperature), "distillationLossBackprop")}
+        return {"logits": lambda: _distillation_gradient(dy, *saved, temperature)}
     return ENGINE.runKernel(forward, "distillationLoss", {"logits": logits}, backward)
+
+
+def _distillation_gradient(dy, logits, teacherLogits, teacherIndices, stats, temperature):
+    """dy T (q - p), 0 in the rows without a teacher.  Differentiable in dy and, through q, in the logits."""
+    axis = [logits.rank - 1]
+
+    def forward(b, save):
+        save([dy, logits, teacherLogits, teacherIndices, stats])
+        return b.distillationLossBackprop(dy, logits, teacherLogits, teacherIndices, stats, temperature)
+
+    def backward(ddlogits, saved):
+        weight, rest = saved[0], saved[1:]
+
+        def ddy():
+            return sum(mul(ddlogits, _distillation_gradient(ones(weight.shape), *rest, temperature)), axis)
+
+        def dlogits():   # T J ddlogits / T, J = diag(q) - q q^T
+            q = _distillation_softmax(*rest, temperature)
+            t = mul(q, ddlogits)
+            return mul(reshape(weight, weight.shape + [1]), sub(t, mul(q, sum(t, axis, True))))
+        return {"dy": ddy, "logits": dlogits}
+    return ENGINE.runKernel(forward, "distillationLossBackprop", {"dy": dy, "logits": logits}, backward)
+
+
+def _distillation_softmax(logits, teacherLogits, teacherIndices, stats, temperature):
+    """q in the rows that have a teacher, 0 in the others whatever their logits hold: the loss's gradient
+    without p.  p is the same for every student, so it drops out of the difference from a student of equal
+    logits: (q - p) - (1/classes - p), and 1/classes comes back in the rows with a teacher.  Those are found
+    by the losses of two constant students, which cannot both be 0 (a single class aside, where the Jacobian
+    is 0 anyway), since no p equals both; in a row without a teacher both are."""
+    rows, classes, axis = logits.shape[:-1], logits.shape[-1], [logits.rank - 1]
+
+    def forward(b, save):
+        def run():
+            def constant(values):
+                return mul(ones(rows + [1]), tensor(np.asarray(values, np.float32), [classes]))
+
+            def loss(student, t, withStats):
+                return b.distillationLoss(student, teacherLogits, teacherIndices, t, withStats)
+            one, equal = ones(rows), constant(np.zeros(classes))
+            first = constant(np.where(np.arange(classes) == 0, 100.0, 0.0))
+            there = reshape(step(add(loss(equal, 1.0, False)[0], loss(first, 1.0, False)[0])), rows + [1])
+            g = b.distillationLossBackprop(one, logits, teacherLogits, teacherIndices, stats, temperature)
+            g0 = b.distillationLossBackprop(one, equal, teacherLogits, teacherIndices,
+                                            loss(equal, temperature, True)[1], temperature)
+            return add(mul(sub(g, g0), scalar(1.0 / temperature)), mul(there, scalar(1.0 / classes if classes else 0.0)))
+        q = ENGINE.tidy(run)
+        save([q])
+        return q
+
+    def backward(dy, saved):
+        def dlogits():
+            t = mul(saved[0], dy)
+            return mul(sub(t, mul(saved[0], sum(t, axis, True))), scalar(1.0 / temperature))
+        return {"logits": dlogits}
+    return ENGINE.runKernel(forward, "distillationSoftmax", {"logits": logits}, backward)
 
 
 # ---- gradients (ops/gradients.ts) ----------------------------------------------------------------
