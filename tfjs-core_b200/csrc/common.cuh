@@ -194,13 +194,16 @@ inline void launch_dependent(tfjs_cuda_ctx* ctx, void (*kernel)(Params...), dim3
   cudaLaunchKernelEx(&cfg, kernel, static_cast<Params>(args)...);
 }
 
-// Lets a kernel take more than 48 KB of dynamic shared memory: always up to the same bound, so that two
-// threads whose contexts launch it with different sizes cannot lower the other's between this and its launch.
-constexpr size_t kMostSmem = 226 * 1024;  // of the 227 KB of a block; the kernels' static arrays take the rest
+// Lets a kernel take more than 48 KB of shared memory: always up to the same bound, so that two threads whose
+// contexts launch it with different sizes cannot lower the other's between this and its launch.  Without this
+// permission the 48 KB hold the kernel's static arrays too, so it is asked for as soon as `smem` bytes beside the
+// most static bytes (1 KB; the 227 KB of a block bound the two together) would pass them.
+constexpr size_t kStaticSmem = 1024, kMostSmem = 227 * 1024 - kStaticSmem;
 template <typename Kernel>
 inline cudaError_t allow_smem(Kernel kernel, size_t smem) {
   if (smem > kMostSmem) return cudaErrorInvalidValue;
-  return smem > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem) : cudaSuccess;
+  if (smem + kStaticSmem <= 48 * 1024) return cudaSuccess;
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem);
 }
 
 // Allocator (context.cu).
