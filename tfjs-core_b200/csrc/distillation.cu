@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(G > 32 ? kThreads : 256) distillation_kernel(
     l = group_reduce<G, false>(l, 0.f, scratch[2]).x * kLn2;
   }
   if (t == 0) {
-    loss[row] = temperature * temperature * l;
+    loss[row] = temperature * (temperature * l);  // the square alone may leave the range that the loss is in
     if (stats) *reinterpret_cast<float4*>(stats + 4 * row) = make_float4(all, ls, um, uls);
   }
 }
@@ -417,8 +417,9 @@ int get_operands(tfjs_cuda_ctx* ctx, tfjs_tensor_id z, tfjs_tensor_id u, tfjs_te
                "distillationLoss: too many rows or classes");
   TFJS_REQUIRE(ctx, top <= kMaxTop, "distillationLoss: a teacher's list holds at most %d entries, got %lld", kMaxTop,
                (long long)top);
-  TFJS_REQUIRE(ctx, temperature > 0.f && temperature - temperature == 0.f && 1.f / temperature - 1.f / temperature == 0.f,
-               "distillationLoss: the temperature must be positive and finite");
+  const float k2 = kLog2e * (1.f / temperature);
+  TFJS_REQUIRE(ctx, temperature > 0.f && temperature - temperature == 0.f && k2 - k2 == 0.f,
+               "distillationLoss: the temperature and its reciprocal must be positive and finite");
   int rc;
   if ((rc = get_activation(ctx, z, rows * classes, "logits", &o->z))) return rc;
   if ((rc = get_activation(ctx, u, rows * top, "teacherLogits", &o->u))) return rc;
