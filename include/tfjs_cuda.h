@@ -180,6 +180,11 @@ int tfjs_cuda_tensor_dispose(tfjs_cuda_ctx* ctx, tfjs_tensor_id id);
 /* Device pointer and byte size of a tensor's storage (zero-copy interop, benchmarks).  Work enqueued on the
  * context's stream from now on runs after an asynchronous upload of the tensor. */
 int tfjs_cuda_tensor_device_ptr(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, void** ptr, size_t* nbytes);
+/* The same for a holder who may write the storage, now or later, without telling the library: from now on
+ * no repacked or decoded form of the tensor is kept from one call for the next.  As a weight it is repacked by
+ * each call, and by every replay of a captured one; only the decoded copy that some kernels take of a quantised
+ * tensor cannot be made within a capture, and such a call is refused there. */
+int tfjs_cuda_tensor_share(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, void** ptr, size_t* nbytes);
 /* Pinned host staging memory for write/read_async callers. */
 int tfjs_cuda_host_alloc(void** ptr, size_t nbytes);
 int tfjs_cuda_host_free(void* ptr);

@@ -347,9 +347,10 @@ export class BackendCuda extends KernelBackend {
   }
 
   /** Extension: the address and byte size of `t`'s storage, for another CUDA library on the same
-   * device.  Valid until `t`'s data is disposed; work on another stream is ordered by the caller. */
+   * device.  Valid until `t`'s data is disposed; work on another stream is ordered by the caller.  As
+   * weights the tensor is repacked by every call from now on. */
   deviceArray(t: Tensor): {ptr: bigint, nbytes: number, stream: bigint} {
-    const r = binding.tensorDevicePtr(this.ctx, this.data.get(t.dataId).id);
+    const r = binding.tensorShare(this.ctx, this.data.get(t.dataId).id);
     this.check(r.status);
     return {ptr: r.ptr, nbytes: r.nbytes, stream: this.stream()};
   }

@@ -579,6 +579,20 @@ napi_value TensorDevicePtr(napi_env env, napi_callback_info cbinfo) {
   return r.obj;
 }
 
+// tfjs_cuda_tensor_share
+napi_value TensorShare(napi_env env, napi_callback_info cbinfo) {
+  Args argz(env, cbinfo);
+  tfjs_cuda_ctx* ctx = (tfjs_cuda_ctx*)argz.handle(0);
+  const tfjs_tensor_id id = (tfjs_tensor_id)argz.integer(1);
+  void* ptr = nullptr;
+  size_t nbytes = 0;
+  if (!argz.ok) return nullptr;
+  Result r(env, (int)tfjs_cuda_tensor_share(ctx, id, &ptr, &nbytes));
+  r.set_ptr("ptr", ptr);
+  r.set_i64("nbytes", (int64_t)nbytes);
+  return r.obj;
+}
+
 // tfjs_cuda_tensor_register_quantized
 napi_value TensorRegisterQuantized(napi_env env, napi_callback_info cbinfo) {
   Args argz(env, cbinfo);
@@ -1016,6 +1030,7 @@ static napi_value Init(napi_env env, napi_value exports) {
   EXPORT("eventDestroy", EventDestroy);
   EXPORT("tensorDispose", TensorDispose);
   EXPORT("tensorDevicePtr", TensorDevicePtr);
+  EXPORT("tensorShare", TensorShare);
   EXPORT("tensorRegisterQuantized", TensorRegisterQuantized);
   EXPORT("batchMatmul", BatchMatmul);
   EXPORT("conv2d", Conv2d);

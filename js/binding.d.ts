@@ -41,6 +41,7 @@ export function eventWait(ev: Handle, timeout_ms: number): number;  // tfjs_cuda
 export function eventDestroy(ev: Handle): number;  // tfjs_cuda_event_destroy
 export function tensorDispose(ctx: Handle, id: number): number;  // tfjs_cuda_tensor_dispose
 export function tensorDevicePtr(ctx: Handle, id: number): {status: number, ptr: bigint, nbytes: number};  // tfjs_cuda_tensor_device_ptr
+export function tensorShare(ctx: Handle, id: number): {status: number, ptr: bigint, nbytes: number};  // tfjs_cuda_tensor_share
 export function tensorRegisterQuantized(ctx: Handle, rank: number, shape: number[], q: Uint8Array, scale: number, min: number): {status: number, out_id: number};  // tfjs_cuda_tensor_register_quantized
 export function batchMatmul(ctx: Handle, a: number, b: number, out: number, batch: number, a_d1: number, a_d2: number, b_d1: number, b_d2: number, transpose_a: number, transpose_b: number, epi: EpilogueLike|null): number;  // tfjs_cuda_batch_matmul
 export function conv2d(ctx: Handle, x: number, filter: number, out: number, info: Conv2DInfoLike, epi: EpilogueLike|null): number;  // tfjs_cuda_conv2d

@@ -18,8 +18,8 @@ Conventions of the generated functions (camelCase of the C name without the `tfj
     or null;
   * a function without output parameters returns the status number; one with output parameters
     returns `{status, <name>: value, ...}`;
-  * raw device pointers (tfjs_cuda_matmul_static_scratch, tensor_device_ptr, ctx_stream) are
-    BigInt addresses.
+  * raw device pointers (tfjs_cuda_matmul_static_scratch, tensor_device_ptr, tensor_share,
+    ctx_stream) are BigInt addresses.
 Three entry points are written by hand below because they are not plain marshalling:
 tensorReadPromise (KernelBackend.read: the wait for the copy's event runs in a napi_async_work so
 the event loop is never blocked), hostAlloc / hostFree (pinned memory surfaced as an external

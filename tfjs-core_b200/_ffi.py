@@ -77,6 +77,7 @@ SIGNATURES = {
     "tfjs_cuda_event_destroy": (C.c_int, [_P]),
     "tfjs_cuda_tensor_dispose": (C.c_int, [_P, C.c_int64]),
     "tfjs_cuda_tensor_device_ptr": (C.c_int, [_P, C.c_int64, C.POINTER(_P), C.POINTER(C.c_size_t)]),
+    "tfjs_cuda_tensor_share": (C.c_int, [_P, C.c_int64, C.POINTER(_P), C.POINTER(C.c_size_t)]),
     "tfjs_cuda_host_alloc": (C.c_int, [C.POINTER(_P), C.c_size_t]),
     "tfjs_cuda_host_free": (C.c_int, [_P]),
     "tfjs_cuda_tensor_register_quantized": (C.c_int, [_P, _I64P, C.c_int, _I64P, _P, C.c_double,

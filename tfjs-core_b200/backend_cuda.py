@@ -332,11 +332,12 @@ class BackendCuda:
         """Extension: `t`'s storage in place, for another library on the same device (half-stored tensors
         appear as float16, quantised ones as their bytes).  The array is valid until `t`'s data is
         disposed.  Work that another stream does on it is ordered by the caller: after sync(), or on
-        stream(); a tensor whose contents are written through it must not have been a contraction's or
-        convolution's weights before, whose repacked form is kept."""
+        stream().  As the weights of a contraction or convolution the tensor is repacked by every call from
+        now on, since its contents may change through the array; a graph captured with its repacked form
+        before does not see such changes."""
         t._throw_if_disposed()
         rec = self._rec(t.dataId)
-        self._check(self._lib.tfjs_cuda_tensor_device_ptr(self._ctx, rec["id"], self._out_ptr_ref, None))
+        self._check(self._lib.tfjs_cuda_tensor_share(self._ctx, rec["id"], self._out_ptr_ref, None))
         typestr = "|u1" if "quantized" in rec else _TYPESTR[rec["dtype"]]
         return DeviceArray({"shape": tuple(t.shape), "typestr": typestr, "data": (self._out_ptr.value or 0, False),
                             "version": 3, "stream": self._stream})

@@ -9,6 +9,8 @@ namespace {
 // recorded, not run, so a cache filled during capture would be marked valid without ever having
 // been written: an eager call on the same tensor before the first replay would read garbage, and
 // every replay would redo the repack.  A miss during capture is therefore refused.
+// A shared tensor's contents may change without notice, so its forms are made anew by every call: the tf32
+// planes and the half plane as temporaries of the call, the dequantised copy in place.
 int refuse_miss_during_capture(tfjs_cuda_ctx* ctx, const char* what) {
   if (!ctx->capturing) return TFJS_CUDA_OK;
   return set_error(ctx, TFJS_CUDA_ERR_UNSUPPORTED,
@@ -24,7 +26,7 @@ int float_view(tfjs_cuda_ctx* ctx, TensorEntry* t, const float** out) {
     *out = (const float*)t->ptr;
     return TFJS_CUDA_OK;
   }
-  if (!t->deq || t->deq_version != t->version) {
+  if (!t->deq || t->deq_version != t->version || t->shared) {
     int miss = refuse_miss_during_capture(ctx, "the dequantised copy");
     if (miss) return miss;
     if (!t->deq) {
@@ -50,6 +52,7 @@ int packed_weights(tfjs_cuda_ctx* ctx, TensorEntry* w, int64_t offset_elems, int
   // row_pad > 0: each run of row_len source rows becomes row_pad packed columns (k_packed total)
   const int64_t kp = row_pad > 0 ? k_packed : (K + 3) / 4 * 4;
   PackedWeights& c = w->packed;
+  cacheable = cacheable && !w->shared;
   *temporary = !cacheable;
   if (cacheable && c.hi && c.version == w->version && c.n == N && c.k == K &&
       c.transposed_source == source_is_nk && c.row_pad == row_pad) {
@@ -151,9 +154,25 @@ int finish_out(tfjs_cuda_ctx* ctx, F32Out* v, int rc) {
   return rc;
 }
 
-// K-major IEEE half plane [N, kp] of a [K, N] contraction operand, cached on the tensor.
-int half_weights(tfjs_cuda_ctx* ctx, TensorEntry* w, int64_t K, int64_t N, const void** plane, int64_t* kp_out) {
+// K-major IEEE half plane [N, kp] of a [K, N] contraction operand, cached on the tensor; a shared tensor's is
+// a temporary, which the caller frees (*tmp, null if there is none).
+int half_weights(tfjs_cuda_ctx* ctx, TensorEntry* w, int64_t K, int64_t N, const void** plane, int64_t* kp_out,
+                 void** tmp, size_t* tmp_cap) {
   const int64_t kp = (K + 7) / 8 * 8;
+  *tmp = nullptr;
+  *kp_out = kp;
+  const bool u8 = w->quant.quantized;
+  if (w->shared) {
+    int rc = ctx_alloc(ctx, (size_t)(N * kp) * 2, tmp, tmp_cap);
+    if (rc) return rc;
+    *plane = *tmp;
+    rc = launch_pack_weights_f16(ctx, w->ptr, u8, w->quant.scale, w->quant.min, K, N, N, 1, kp, *tmp);
+    if (rc) {
+      ctx_free(ctx, *tmp, *tmp_cap);
+      *tmp = nullptr;
+    }
+    return rc;
+  }
   if (!w->w16 || w->w16_version != w->version || w->w16_n != N || w->w16_k != K) {
     int miss = refuse_miss_during_capture(ctx, "the half-precision tensor-core layout");
     if (miss) return miss;
@@ -161,8 +180,7 @@ int half_weights(tfjs_cuda_ctx* ctx, TensorEntry* w, int64_t K, int64_t N, const
     w->w16 = nullptr;
     int rc = ctx_alloc(ctx, (size_t)(N * kp) * 2, &w->w16, &w->w16_capacity);
     if (rc) return rc;
-    rc = launch_pack_weights_f16(ctx, w->ptr, w->quant.quantized, w->quant.scale, w->quant.min, K, N, N, 1, kp,
-                                 w->w16);
+    rc = launch_pack_weights_f16(ctx, w->ptr, u8, w->quant.scale, w->quant.min, K, N, N, 1, kp, w->w16);
     if (rc) return rc;
     w->w16_version = w->version;
     w->w16_n = N;
@@ -170,7 +188,6 @@ int half_weights(tfjs_cuda_ctx* ctx, TensorEntry* w, int64_t K, int64_t N, const
     w->w16_kp = kp;
   }
   *plane = w->w16;
-  *kp_out = kp;
   return TFJS_CUDA_OK;
 }
 
@@ -193,7 +210,7 @@ int gemm_dispatch(tfjs_cuda_ctx* ctx, const float* a, int64_t M, int64_t K, Tens
                   int64_t w_offset, bool source_is_nk, bool cacheable, float* out, int64_t N,
                   const EpilogueArgs& epi, bool a_tf32_exact = false) {
   if (ctx->use_tensor_cores && tcgen05_gemm_supported(M, N, K)) {
-    if (ctx->dequant_in_gemm && w->quant.quantized && cacheable && w_offset == 0) {
+    if (ctx->dequant_in_gemm && w->quant.quantized && cacheable && !w->shared && w_offset == 0) {
       // Quantised weights stay uint8 in HBM: a K-major byte copy is cached once and the kernel
       // dequantises each tile in shared memory.
       const int64_t kq = (K + 15) / 16 * 16;
@@ -344,9 +361,13 @@ extern "C" int tfjs_cuda_conv2d(tfjs_cuda_ctx* ctx, tfjs_tensor_id x_id, tfjs_te
       tcgen05_gemm_f16_supported(pixels, ci->outChannels, ci->inChannels, o16)) {
     const void* plane;
     int64_t kp;
-    rc = half_weights(ctx, w, ci->inChannels, ci->outChannels, &plane, &kp);
+    void* tmp;
+    size_t tmp_cap;
+    rc = half_weights(ctx, w, ci->inChannels, ci->outChannels, &plane, &kp, &tmp, &tmp_cap);
     if (rc) return rc;
-    return launch_gemm_tcgen05_f16(ctx, x->ptr, pixels, ci->inChannels, plane, kp, o->ptr, o16, ci->outChannels, e);
+    rc = launch_gemm_tcgen05_f16(ctx, x->ptr, pixels, ci->inChannels, plane, kp, o->ptr, o16, ci->outChannels, e);
+    if (tmp) ctx_free(ctx, tmp, tmp_cap);
+    return rc;
   }
   // The 3-channel 3x3 stem: the image window of a patch arrives by TMA and is rearranged into
   // im2col rows in shared memory (TF32; other modes take the gather path below).  It can store
@@ -360,8 +381,10 @@ extern "C" int tfjs_cuda_conv2d(tfjs_cuda_ctx* ctx, tfjs_tensor_id x_id, tfjs_te
     bool temporary;
     rc = packed_weights(ctx, w, 0, 27, ci->outChannels, false, true, &pw, &temporary, 9, 10, 32);
     if (rc) return rc;
-    return launch_conv_rgb_tcgen05(ctx, x->ptr, *ci, pw.hi, pw.kp, o->ptr, e, o16, x8, x->quant.scale, x->quant.min,
-                                   split3 ? pw.lo : nullptr);
+    rc = launch_conv_rgb_tcgen05(ctx, x->ptr, *ci, pw.hi, pw.kp, o->ptr, e, o16, x8, x->quant.scale, x->quant.min,
+                                 split3 ? pw.lo : nullptr);
+    release_temporary(ctx, pw, temporary);
+    return rc;
   }
   // Every other kernel computes on float32 storage.
   F32View xv;
@@ -390,7 +413,9 @@ extern "C" int tfjs_cuda_conv2d(tfjs_cuda_ctx* ctx, tfjs_tensor_id x_id, tfjs_te
     rc = packed_weights(ctx, w, 0, (int64_t)ci->filterHeight * ci->filterWidth * ci->inChannels,
                         ci->outChannels, false, true, &pw, &temporary);
     if (rc) return done(rc);
-    return done(launch_conv_tma_tcgen05(ctx, xv.ptr, *ci, pw.hi, pw.kp, ov.ptr, e, split3 ? pw.lo : nullptr));
+    rc = launch_conv_tma_tcgen05(ctx, xv.ptr, *ci, pw.hi, pw.kp, ov.ptr, e, split3 ? pw.lo : nullptr);
+    release_temporary(ctx, pw, temporary);
+    return done(rc);
   }
   // Everything else with Cin % 4 == 0 (or a 3-channel, 3-wide filter) is an implicit GEMM: the
   // A tile is gathered from the image by the kernel itself, K = fH * fW * Cin.
@@ -404,7 +429,9 @@ extern "C" int tfjs_cuda_conv2d(tfjs_cuda_ctx* ctx, tfjs_tensor_id x_id, tfjs_te
                         rgb ? ci->filterWidth * ci->inChannels : 0, rgb ? 10 : 0,
                         rgb ? tcgen05_conv_k(*ci, mode) : 0);
     if (rc) return done(rc);
-    return done(launch_conv_tcgen05(ctx, mode, xv.ptr, *ci, pw.hi, pw.lo, pw.kp, ov.ptr, e, ctx->math_mode));
+    rc = launch_conv_tcgen05(ctx, mode, xv.ptr, *ci, pw.hi, pw.lo, pw.kp, ov.ptr, e, ctx->math_mode);
+    release_temporary(ctx, pw, temporary);
+    return done(rc);
   }
   const float* wf;
   rc = float_view(ctx, w, &wf);
@@ -531,7 +558,9 @@ extern "C" int tfjs_cuda_separable_conv2d(tfjs_cuda_ctx* ctx, tfjs_tensor_id x_i
     bool temporary;
     rc = packed_weights(ctx, wp, 0, C, N, false, true, &pw, &temporary);
     if (rc) return rc;
-    return launch_sepconv_tcgen05(ctx, x->ptr, *dw, wdf, de, pw.hi, pw.kp, o->ptr, N, pe, half);
+    rc = launch_sepconv_tcgen05(ctx, x->ptr, *dw, wdf, de, pw.hi, pw.kp, o->ptr, N, pe, half);
+    release_temporary(ctx, pw, temporary);
+    return rc;
   }
   // Half storage, two kernels: whole-image depthwise into a half intermediate, f16 tensor-core GEMM.
   if (half && ctx->use_tensor_cores && pe.activation != TFJS_ACT_PRELU &&
@@ -557,8 +586,11 @@ extern "C" int tfjs_cuda_separable_conv2d(tfjs_cuda_ctx* ctx, tfjs_tensor_id x_i
     if (!rc) {
       const void* plane;
       int64_t kp;
-      rc = half_weights(ctx, wp, C, N, &plane, &kp);
+      void* tmp;
+      size_t tmp_cap;
+      rc = half_weights(ctx, wp, C, N, &plane, &kp, &tmp, &tmp_cap);
       if (!rc) rc = launch_gemm_tcgen05_f16(ctx, mid, pixels, C, plane, kp, o->ptr, true, N, pe);
+      if (tmp) ctx_free(ctx, tmp, tmp_cap);
     }
     ctx_free(ctx, mid, mid_cap);
     return rc;

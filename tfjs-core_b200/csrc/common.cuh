@@ -63,6 +63,9 @@ struct TensorEntry {
   size_t w16_capacity = 0;
   int64_t w16_n = 0, w16_k = 0, w16_kp = 0;
   uint64_t w16_version = ~0ull;
+  // others hold the address and may write the contents at any time (tensor_share): a form derived from them
+  // is good for the call that made it
+  bool shared = false;
   // asynchronous upload in flight on the copy stream (tensor_write_async)
   cudaEvent_t copy_event = nullptr;
   bool copy_pending = false;
@@ -211,7 +214,7 @@ int ctx_alloc(tfjs_cuda_ctx* ctx, size_t nbytes, void** ptr, size_t* capacity);
 void ctx_free(tfjs_cuda_ctx* ctx, void* ptr, size_t capacity);
 
 TensorEntry* find_tensor(tfjs_cuda_ctx* ctx, tfjs_tensor_id id);
-inline bool known_finite(const TensorEntry* t) { return t->finite_version == t->version; }
+inline bool known_finite(const TensorEntry* t) { return t->finite_version == t->version && !t->shared; }
 // Looks the id up and checks dtype float32 with at least `min_elems` elements.
 int get_f32(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, int64_t min_elems, const char* what,
             TensorEntry** out);

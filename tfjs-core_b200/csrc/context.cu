@@ -705,6 +705,12 @@ extern "C" int tfjs_cuda_tensor_device_ptr(tfjs_cuda_ctx* ctx, tfjs_tensor_id id
   return wait_for_upload(ctx, t);  // whoever orders itself after the context's stream sees the upload too
 }
 
+extern "C" int tfjs_cuda_tensor_share(tfjs_cuda_ctx* ctx, tfjs_tensor_id id, void** ptr, size_t* nbytes) {
+  const int rc = tfjs_cuda_tensor_device_ptr(ctx, id, ptr, nbytes);
+  if (!rc) find_tensor(ctx, id)->shared = true;
+  return rc;
+}
+
 extern "C" int tfjs_cuda_host_alloc(void** ptr, size_t nbytes) {
   if (!ptr) return TFJS_CUDA_ERR_INVALID_ARG;
   cudaError_t e = cudaMallocHost(ptr, nbytes ? nbytes : 1);
