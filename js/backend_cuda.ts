@@ -97,7 +97,11 @@ export class BackendCuda extends KernelBackend {
     const rec = this.data.get(t.dataId);
     if (rec.dtype === want && !rec.half) return [rec.id, null];
     const tmp = this.newId(t.shape, want);
-    this.check(binding.cast(this.ctx, rec.id, tmp));
+    const rc = binding.cast(this.ctx, rec.id, tmp);
+    if (rc !== 0) {
+      this.freeTmp(tmp);
+      this.check(rc);
+    }
     return [tmp, tmp];
   }
 
@@ -731,19 +735,37 @@ export class BackendCuda extends KernelBackend {
   }
 
   // ---- normalisation, lookup and loss of token and feature models (extensions) ---------------------
-  /** Ends a kernel method: frees the converted operands and, if the call failed, its outputs. */
-  private enqueued(rc: number, outputs: Array<Tensor|null>, temporaries: Array<number|null>): void {
-    this.freeTmp(...temporaries);
-    if (rc !== 0) {
-      for (const t of outputs) {
-        if (t != null) t.dispose();
-      }
-      this.check(rc);
+  /** `run` converts its operands, makes its outputs (both go into the lists) and enqueues the kernel, whose
+   * status it returns.  The conversions are freed, and if a step fails the outputs made so far are disposed. */
+  private kernel(run: (temporaries: Array<number|null>, outputs: Tensor[]) => number): Tensor[] {
+    const temporaries: Array<number|null> = [];
+    const outputs: Tensor[] = [];
+    try {
+      this.check(run(temporaries, outputs));
+    } catch (e) {
+      for (const t of outputs) t.dispose();
+      throw e;
+    } finally {
+      this.freeTmp(...temporaries);
     }
+    return outputs;
   }
 
-  private optionalId(t: Tensor|null): [number, number|null] {
-    return t == null ? [0, null] : this.id(t);
+  private operand(t: Tensor, temporaries: Array<number|null>, want: DataType = 'float32'): number {
+    const [id, tmp] = this.id(t, want);
+    temporaries.push(tmp);
+    return id;
+  }
+
+  private activation(t: Tensor, temporaries: Array<number|null>): number {
+    const [id, tmp] = this.activationId(t);
+    temporaries.push(tmp);
+    return id;
+  }
+
+  private output(t: Tensor, outputs: Tensor[]): number {
+    outputs.push(t);
+    return this.outId(t);
   }
 
   /** (x - mean) * rstd * gamma + beta over the inner-most axis; gamma and beta are [width] or null.
@@ -753,15 +775,16 @@ export class BackendCuda extends KernelBackend {
     this.assertNumeric([x, gamma, beta], 'layerNorm');
     if (x.rank === 0) throw new Error('layerNorm needs a tensor of rank 1 or more');
     const outer = x.shape.slice(0, -1);
-    const [xid, tx] = this.activationId(x);
-    const [gid, tg] = this.optionalId(gamma);
-    const [bid, tb] = this.optionalId(beta);
-    const y = this.makeActivation<T>(x.shape, outputStorage);
-    const stats = withStats ? this.makeOutput<Tensor>([...outer, 2]) : null;
-    const rc = binding.layerNorm(this.ctx, xid, gid, bid, this.outId(y), stats == null ? 0 : this.outId(stats),
-                                 util.sizeFromShape(outer), x.shape[x.rank - 1], epsilon);
-    this.enqueued(rc, [y, stats], [tx, tg, tb]);
-    return [y, stats];
+    const out = this.kernel((tmp, out) => {
+      const xid = this.activation(x, tmp);
+      const gid = gamma == null ? 0 : this.operand(gamma, tmp);
+      const bid = beta == null ? 0 : this.operand(beta, tmp);
+      const yid = this.output(this.makeActivation<T>(x.shape, outputStorage), out);
+      const sid = withStats ? this.output(this.makeOutput([...outer, 2]), out) : 0;
+      return binding.layerNorm(this.ctx, xid, gid, bid, yid, sid, util.sizeFromShape(outer), x.shape[x.rank - 1],
+                               epsilon);
+    });
+    return [out[0] as T, withStats ? out[1] : null];
   }
 
   /** dx, dgamma and dbeta of layerNorm, from the statistics of its forward pass. */
@@ -769,30 +792,30 @@ export class BackendCuda extends KernelBackend {
     this.assertNumeric([dy, x, gamma, stats], 'layerNormBackprop');
     if (x.rank === 0) throw new Error('layerNorm needs a tensor of rank 1 or more');
     const width = x.shape[x.rank - 1];
-    const [did, td] = this.activationId(dy);
-    const [xid, tx] = this.activationId(x);
-    const [gid, tg] = this.optionalId(gamma);
-    const [sid, ts] = this.id(stats);
-    const dx = this.makeOutput<T>(x.shape);
-    const dgamma = this.makeOutput<Tensor>([width]);
-    const dbeta = this.makeOutput<Tensor>([width]);
-    const rc = binding.layerNormBackprop(this.ctx, did, xid, gid, sid, this.outId(dx), this.outId(dgamma),
-                                         this.outId(dbeta), util.sizeFromShape(x.shape.slice(0, -1)), width);
-    this.enqueued(rc, [dx, dgamma, dbeta], [td, tx, tg, ts]);
-    return [dx, dgamma, dbeta];
+    const out = this.kernel((tmp, out) => {
+      const did = this.activation(dy, tmp);
+      const xid = this.activation(x, tmp);
+      const gid = gamma == null ? 0 : this.operand(gamma, tmp);
+      const sid = this.operand(stats, tmp);
+      const dx = this.output(this.makeOutput(x.shape), out);
+      const dgamma = this.output(this.makeOutput([width]), out);
+      const dbeta = this.output(this.makeOutput([width]), out);
+      return binding.layerNormBackprop(this.ctx, did, xid, gid, sid, dx, dgamma, dbeta,
+                                       util.sizeFromShape(x.shape.slice(0, -1)), width);
+    });
+    return [out[0] as T, out[1], out[2]];
   }
 
   /** scale * table[indices]; a row of zeros where the index lies outside the table (padding). */
   embeddingLookup(table: Tensor, indices: Tensor, scale = 1, outputStorage?: 'float32'|'float16'): Tensor {
     this.assertNumeric([table], 'embeddingLookup');
     if (table.rank !== 2) throw new Error(`embeddingLookup needs a table of rank 2, got rank ${table.rank}`);
-    const [tid, tt] = this.activationId(table);
-    const [iid, ti] = this.id(indices, 'int32');
-    const out = this.makeActivation<Tensor>([...indices.shape, table.shape[1]], outputStorage);
-    const rc = binding.embeddingLookup(this.ctx, tid, iid, this.outId(out), indices.size, table.shape[0],
-                                       table.shape[1], scale);
-    this.enqueued(rc, [out], [tt, ti]);
-    return out;
+    return this.kernel((tmp, out) => {
+      const tid = this.activation(table, tmp);
+      const iid = this.operand(indices, tmp, 'int32');
+      const oid = this.output(this.makeActivation([...indices.shape, table.shape[1]], outputStorage), out);
+      return binding.embeddingLookup(this.ctx, tid, iid, oid, indices.size, table.shape[0], table.shape[1], scale);
+    })[0];
   }
 
   /** The gradient of embeddingLookup's table, [vocab, width]. */
@@ -802,12 +825,12 @@ export class BackendCuda extends KernelBackend {
       throw new Error(`embeddingLookupBackprop: dy's shape ${dy.shape} does not match indices ${indices.shape}`);
     }
     const width = dy.shape[dy.rank - 1];
-    const [did, td] = this.activationId(dy);
-    const [iid, ti] = this.id(indices, 'int32');
-    const out = this.makeOutput<Tensor>([vocab, width]);
-    const rc = binding.embeddingLookupBackprop(this.ctx, did, iid, this.outId(out), indices.size, vocab, width, scale);
-    this.enqueued(rc, [out], [td, ti]);
-    return out;
+    return this.kernel((tmp, out) => {
+      const did = this.activation(dy, tmp);
+      const iid = this.operand(indices, tmp, 'int32');
+      const oid = this.output(this.makeOutput([vocab, width]), out);
+      return binding.embeddingLookupBackprop(this.ctx, did, iid, oid, indices.size, vocab, width, scale);
+    })[0];
   }
 
   private static distillationExtent(logits: Tensor, teacherLogits: Tensor, teacherIndices: Tensor): [number, number, number] {
@@ -826,16 +849,16 @@ export class BackendCuda extends KernelBackend {
                    withStats = true): [Tensor, Tensor|null] {
     this.assertNumeric([logits, teacherLogits], 'distillationLoss');
     const [rows, classes, top] = BackendCuda.distillationExtent(logits, teacherLogits, teacherIndices);
-    const [zid, tz] = this.activationId(logits);
-    const [uid, tu] = this.activationId(teacherLogits);
-    const [iid, ti] = this.id(teacherIndices, 'int32');
     const outer = logits.shape.slice(0, -1);
-    const loss = this.makeOutput<Tensor>(outer);
-    const stats = withStats ? this.makeOutput<Tensor>([...outer, 4]) : null;
-    const rc = binding.distillationLoss(this.ctx, zid, uid, iid, this.outId(loss), stats == null ? 0 : this.outId(stats),
-                                        rows, classes, top, temperature);
-    this.enqueued(rc, [loss, stats], [tz, tu, ti]);
-    return [loss, stats];
+    const out = this.kernel((tmp, out) => {
+      const zid = this.activation(logits, tmp);
+      const uid = this.activation(teacherLogits, tmp);
+      const iid = this.operand(teacherIndices, tmp, 'int32');
+      const lid = this.output(this.makeOutput(outer), out);
+      const sid = withStats ? this.output(this.makeOutput([...outer, 4]), out) : 0;
+      return binding.distillationLoss(this.ctx, zid, uid, iid, lid, sid, rows, classes, top, temperature);
+    });
+    return [out[0], withStats ? out[1] : null];
   }
 
   /** The gradient of distillationLoss's logits, from the statistics of its forward pass. */
@@ -843,16 +866,15 @@ export class BackendCuda extends KernelBackend {
                            stats: Tensor, temperature = 1): Tensor {
     this.assertNumeric([dloss, logits, teacherLogits, stats], 'distillationLossBackprop');
     const [rows, classes, top] = BackendCuda.distillationExtent(logits, teacherLogits, teacherIndices);
-    const [did, td] = this.id(dloss);
-    const [zid, tz] = this.activationId(logits);
-    const [uid, tu] = this.activationId(teacherLogits);
-    const [iid, ti] = this.id(teacherIndices, 'int32');
-    const [sid, ts] = this.id(stats);
-    const out = this.makeOutput<Tensor>(logits.shape);
-    const rc = binding.distillationLossBackprop(this.ctx, did, zid, uid, iid, sid, this.outId(out), rows, classes, top,
-                                                temperature);
-    this.enqueued(rc, [out], [td, tz, tu, ti, ts]);
-    return out;
+    return this.kernel((tmp, out) => {
+      const did = this.operand(dloss, tmp);
+      const zid = this.activation(logits, tmp);
+      const uid = this.activation(teacherLogits, tmp);
+      const iid = this.operand(teacherIndices, tmp, 'int32');
+      const sid = this.operand(stats, tmp);
+      const oid = this.output(this.makeOutput(logits.shape), out);
+      return binding.distillationLossBackprop(this.ctx, did, zid, uid, iid, sid, oid, rows, classes, top, temperature);
+    })[0];
   }
 
   // ---- metadata ops (backend.ts:480-486; backend_util.ts:36-76): free, no device work -------------

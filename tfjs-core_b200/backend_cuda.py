@@ -111,7 +111,10 @@ class BackendCuda:
         if rec["dtype"] == want:
             return rec["id"], None
         tmp = self._new_id(t.shape, want)
-        self._check(self._lib.tfjs_cuda_cast(self._ctx, rec["id"], tmp))
+        rc = self._lib.tfjs_cuda_cast(self._ctx, rec["id"], tmp)
+        if rc != 0:
+            self._free_tmp(tmp)
+            self._check(rc)
         return tmp, tmp
 
     def _new_id(self, shape, dtype):
@@ -684,19 +687,33 @@ class BackendCuda:
         return out
 
     # ---- normalisation, lookup and loss of token and feature models (extensions) -----------
-    def _enqueue(self, rc, outputs, temporaries):
-        """Ends a kernel method: frees the converted operands and, if the call failed, its outputs."""
-        for i in temporaries:
-            if i is not None:
-                self._lib.tfjs_cuda_tensor_dispose(self._ctx, i)
-        if rc != 0:
-            for t in outputs:
-                if t is not None:
-                    t.dispose()
-            self._check(rc)
+    # Each method converts operands (temporaries), makes its outputs and enqueues one kernel; a step that
+    # fails leaves none of them behind.
+    def _give_up(self, outputs):
+        for t in outputs:
+            t.dispose()
+
+    def _operand(self, t, temporaries, want="float32"):
+        rec = self._data.get(t.dataId)
+        if rec is not None and rec["dtype"] == want:   # the usual operand needs no conversion
+            return rec["id"]
+        i, tmp = self._id(t, want)
+        if tmp is not None:
+            temporaries.append(tmp)
+        return i
+
+    def _activation(self, t, temporaries):
+        rec = self._data.get(t.dataId)
+        if rec is not None and rec["dtype"] in ("float32", "float16"):
+            return rec["id"]
+        return self._operand(t, temporaries)
 
     def _oid(self, t):
         return 0 if t is None else self._data[t.dataId]["id"]
+
+    def _output(self, t, outputs):
+        outputs.append(t)
+        return self._data[t.dataId]["id"]
 
     def layerNorm(self, x, gamma, beta, epsilon, withStats=False, outputStorage=None):
         """Extension: (x - mean) * rstd * gamma + beta over the inner-most axis; gamma and beta are
@@ -707,15 +724,24 @@ class BackendCuda:
         if not x.shape:
             raise ValueError("layerNorm needs a tensor of rank 1 or more")
         width = x.shape[-1]
-        xid, tx = self._activation_id(x)
-        gid, tg = self._id(gamma) if gamma is not None else (0, None)
-        bid, tb = self._id(beta) if beta is not None else (0, None)
-        y = self._out_activation(x.shape, outputStorage)
-        stats = self._out(x.shape[:-1] + [2]) if withStats else None
-        rc = self._lib.tfjs_cuda_layer_norm(self._ctx, xid, gid, bid, self._oid(y), self._oid(stats),
-                                            size_from_shape(x.shape[:-1]), width, float(epsilon))
-        self._enqueue(rc, (y, stats), (tx, tg, tb))
-        return y, stats
+        tmp, out = [], []
+        try:
+            xid = self._activation(x, tmp)
+            gid = self._operand(gamma, tmp) if gamma is not None else 0
+            bid = self._operand(beta, tmp) if beta is not None else 0
+            yid = self._output(self._out_activation(x.shape, outputStorage), out)
+            sid = self._output(self._out(x.shape[:-1] + [2]), out) if withStats else 0
+            rc = self._lib.tfjs_cuda_layer_norm(self._ctx, xid, gid, bid, yid, sid, size_from_shape(x.shape[:-1]),
+                                                width, float(epsilon))
+            if rc != 0:
+                self._check(rc)
+            return out[0], out[1] if withStats else None
+        except BaseException:
+            self._give_up(out)
+            raise
+        finally:
+            if tmp:
+                self._free_tmp(*tmp)
 
     def layerNormBackprop(self, dy, x, gamma, stats):
         """Extension: (dx, dgamma, dbeta) of layerNorm, from the stats of its forward pass."""
@@ -723,15 +749,23 @@ class BackendCuda:
         if not x.shape:
             raise ValueError("layerNorm needs a tensor of rank 1 or more")
         width = x.shape[-1]
-        did, td = self._activation_id(dy)
-        xid, tx = self._activation_id(x)
-        gid, tg = self._id(gamma) if gamma is not None else (0, None)
-        sid, ts = self._id(stats)
-        dx, dgamma, dbeta = outputs = (self._out(x.shape), self._out([width]), self._out([width]))
-        rc = self._lib.tfjs_cuda_layer_norm_backprop(self._ctx, did, xid, gid, sid, self._oid(dx), self._oid(dgamma),
-                                                     self._oid(dbeta), size_from_shape(x.shape[:-1]), width)
-        self._enqueue(rc, outputs, (td, tx, tg, ts))
-        return outputs
+        tmp, out = [], []
+        try:
+            did, xid = self._activation(dy, tmp), self._activation(x, tmp)
+            gid = self._operand(gamma, tmp) if gamma is not None else 0
+            sid = self._operand(stats, tmp)
+            ids = [self._output(self._out(shape), out) for shape in (x.shape, [width], [width])]
+            rc = self._lib.tfjs_cuda_layer_norm_backprop(self._ctx, did, xid, gid, sid, *ids,
+                                                         size_from_shape(x.shape[:-1]), width)
+            if rc != 0:
+                self._check(rc)
+            return tuple(out)
+        except BaseException:
+            self._give_up(out)
+            raise
+        finally:
+            if tmp:
+                self._free_tmp(*tmp)
 
     def embeddingLookup(self, table, indices, scale=1.0, outputStorage=None):
         """Extension: scale * table[indices], [..., width]; a row of zeros where the index lies outside
@@ -740,13 +774,21 @@ class BackendCuda:
         self._assert_numeric(table, "embeddingLookup")
         if len(table.shape) != 2:
             raise ValueError(f"embeddingLookup needs a table of rank 2, got rank {len(table.shape)}")
-        tid, tt = self._activation_id(table)
-        iid, ti = self._id(indices, "int32")
-        out = self._out_activation(indices.shape + [table.shape[1]], outputStorage)
-        rc = self._lib.tfjs_cuda_embedding_lookup(self._ctx, tid, iid, self._oid(out), indices.size, table.shape[0],
-                                                  table.shape[1], float(scale))
-        self._enqueue(rc, (out,), (tt, ti))
-        return out
+        tmp, out = [], []
+        try:
+            tid, iid = self._activation(table, tmp), self._operand(indices, tmp, "int32")
+            oid = self._output(self._out_activation(indices.shape + [table.shape[1]], outputStorage), out)
+            rc = self._lib.tfjs_cuda_embedding_lookup(self._ctx, tid, iid, oid, indices.size, table.shape[0],
+                                                      table.shape[1], float(scale))
+            if rc != 0:
+                self._check(rc)
+            return out[0]
+        except BaseException:
+            self._give_up(out)
+            raise
+        finally:
+            if tmp:
+                self._free_tmp(*tmp)
 
     def embeddingLookupBackprop(self, dy, indices, vocab, scale=1.0):
         """Extension: the gradient of embeddingLookup's table, [vocab, width]: scale times the sum of the
@@ -754,13 +796,21 @@ class BackendCuda:
         self._assert_numeric(dy, "embeddingLookupBackprop")
         if dy.shape[:-1] != indices.shape or not dy.shape:
             raise ValueError(f"embeddingLookupBackprop: dy's shape {dy.shape} does not match indices {indices.shape}")
-        did, td = self._activation_id(dy)
-        iid, ti = self._id(indices, "int32")
-        out = self._out([int(vocab), dy.shape[-1]])
-        rc = self._lib.tfjs_cuda_embedding_lookup_backprop(self._ctx, did, iid, self._oid(out), indices.size,
-                                                           int(vocab), dy.shape[-1], float(scale))
-        self._enqueue(rc, (out,), (td, ti))
-        return out
+        tmp, out = [], []
+        try:
+            did, iid = self._activation(dy, tmp), self._operand(indices, tmp, "int32")
+            oid = self._output(self._out([int(vocab), dy.shape[-1]]), out)
+            rc = self._lib.tfjs_cuda_embedding_lookup_backprop(self._ctx, did, iid, oid, indices.size, int(vocab),
+                                                               dy.shape[-1], float(scale))
+            if rc != 0:
+                self._check(rc)
+            return out[0]
+        except BaseException:
+            self._give_up(out)
+            raise
+        finally:
+            if tmp:
+                self._free_tmp(*tmp)
 
     @staticmethod
     def _distillation_extent(logits, teacherLogits, teacherIndices):
@@ -776,31 +826,44 @@ class BackendCuda:
         does not count; a row without any gives 0).  Returns (loss, stats): stats, [..., 4], is what the
         gradient reads, or None unless `withStats`."""
         self._assert_numeric([logits, teacherLogits], "distillationLoss")
-        rows, classes, top = self._distillation_extent(logits, teacherLogits, teacherIndices)
-        zid, tz = self._activation_id(logits)
-        uid, tu = self._activation_id(teacherLogits)
-        iid, ti = self._id(teacherIndices, "int32")
-        loss = self._out(logits.shape[:-1])
-        stats = self._out(logits.shape[:-1] + [4]) if withStats else None
-        rc = self._lib.tfjs_cuda_distillation_loss(self._ctx, zid, uid, iid, self._oid(loss), self._oid(stats), rows,
-                                                   classes, top, float(temperature))
-        self._enqueue(rc, (loss, stats), (tz, tu, ti))
-        return loss, stats
+        extent = self._distillation_extent(logits, teacherLogits, teacherIndices)
+        tmp, out = [], []
+        try:
+            zid, uid = self._activation(logits, tmp), self._activation(teacherLogits, tmp)
+            iid = self._operand(teacherIndices, tmp, "int32")
+            lid = self._output(self._out(logits.shape[:-1]), out)
+            sid = self._output(self._out(logits.shape[:-1] + [4]), out) if withStats else 0
+            rc = self._lib.tfjs_cuda_distillation_loss(self._ctx, zid, uid, iid, lid, sid, *extent, float(temperature))
+            if rc != 0:
+                self._check(rc)
+            return out[0], out[1] if withStats else None
+        except BaseException:
+            self._give_up(out)
+            raise
+        finally:
+            if tmp:
+                self._free_tmp(*tmp)
 
     def distillationLossBackprop(self, dloss, logits, teacherLogits, teacherIndices, stats, temperature=1.0):
         """Extension: the gradient of distillationLoss's logits, from the stats of its forward pass."""
         self._assert_numeric([dloss, logits, teacherLogits, stats], "distillationLossBackprop")
-        rows, classes, top = self._distillation_extent(logits, teacherLogits, teacherIndices)
-        did, td = self._id(dloss)
-        zid, tz = self._activation_id(logits)
-        uid, tu = self._activation_id(teacherLogits)
-        iid, ti = self._id(teacherIndices, "int32")
-        sid, ts = self._id(stats)
-        out = self._out(logits.shape)
-        rc = self._lib.tfjs_cuda_distillation_loss_backprop(self._ctx, did, zid, uid, iid, sid, self._oid(out), rows,
-                                                            classes, top, float(temperature))
-        self._enqueue(rc, (out,), (td, tz, tu, ti, ts))
-        return out
+        extent = self._distillation_extent(logits, teacherLogits, teacherIndices)
+        tmp, out = [], []
+        try:
+            did, zid, uid = self._operand(dloss, tmp), self._activation(logits, tmp), self._activation(teacherLogits, tmp)
+            iid, sid = self._operand(teacherIndices, tmp, "int32"), self._operand(stats, tmp)
+            oid = self._output(self._out(logits.shape), out)
+            rc = self._lib.tfjs_cuda_distillation_loss_backprop(self._ctx, did, zid, uid, iid, sid, oid, *extent,
+                                                                float(temperature))
+            if rc != 0:
+                self._check(rc)
+            return out[0]
+        except BaseException:
+            self._give_up(out)
+            raise
+        finally:
+            if tmp:
+                self._free_tmp(*tmp)
 
     # ---- metadata ops (backend.ts:480-486; backend_util.ts:36-76) ------------------------
     def reshape(self, x, shape):

@@ -180,7 +180,14 @@ class Engine:
             self.tensorInfo[t.dataId] = info
             self.numBytes += nbytes
             self.numDataBuffers += 1
-            b.register(t.dataId, t.shape, t.dtype)
+            try:
+                b.register(t.dataId, t.shape, t.dtype)
+            except BaseException:   # nothing was made: nothing to count
+                self.numTensors -= 1
+                self.numBytes -= nbytes
+                self.numDataBuffers -= 1
+                del self.tensorInfo[t.dataId]
+                raise
         info["refCount"] += 1
         if self.scopeStack:
             self.scopeStack[-1]["track"].append(t)
