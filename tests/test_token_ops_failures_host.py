@@ -90,3 +90,34 @@ def test_a_failed_step_leaves_nothing_behind(fake, name):
     for t in made if isinstance(made, tuple) else (made,):
         t.dispose()
     assert state() == before
+
+
+def test_out_parameters_belong_to_their_call(fake):
+    """Another thread's call may fill its out-parameter between this call and the reading of its own; played
+    here by a library that makes that call before it returns."""
+    lib, bk = fake
+    t = ops.tensor(np.zeros(3, np.float32))
+    inner, register, share = [], lib.tfjs_cuda_tensor_register, {bk._data[t.dataId]["id"]: 0x1000}
+
+    def registering(ctx, out, *rest):
+        rc = register(ctx, out, *rest)
+        if not inner:
+            inner.append(None)
+            inner[0] = bk._new_id([2], "float32")
+        return rc
+    lib.tfjs_cuda_tensor_register = registering
+    outer = bk._new_id([2], "float32")
+    assert outer != inner[0] and {outer, inner[0]} <= lib.live
+    other = ops.tensor(np.zeros(3, np.float32))
+    share[bk._data[other.dataId]["id"]] = 0x2000
+    nested = []
+
+    def sharing(ctx, i, ptr, nbytes):
+        ptr._obj.value = share[i]
+        if not nested:
+            nested.append(None)
+            nested[0] = bk.deviceArray(other)
+        return 0
+    lib.tfjs_cuda_tensor_share = sharing
+    arrays = bk.deviceArray(t), nested[0]
+    assert [a.__cuda_array_interface__["data"][0] for a in arrays] == [0x1000, 0x2000]

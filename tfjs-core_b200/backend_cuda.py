@@ -79,9 +79,6 @@ class BackendCuda:
         self.device = int(device)
         # DataStorage (backend.ts:47-70): dataId -> record; the engine disposes every dataId it registers
         self._data = {}
-        # out-parameters of the calls that every operator makes (one host thread a context)
-        self._out_id, self._out_ptr = C.c_int64(), C.c_void_p()
-        self._out_id_ref, self._out_ptr_ref = C.byref(self._out_id), C.byref(self._out_ptr)
         self._stream = self._lib.tfjs_cuda_ctx_stream(ctx)
         self.activation_storage = "float32"
         self._pending_storage = None
@@ -118,11 +115,12 @@ class BackendCuda:
         return tmp, tmp
 
     def _new_id(self, shape, dtype):
-        rc = self._lib.tfjs_cuda_tensor_register(self._ctx, self._out_id_ref, len(shape), _ffi.shape_array(shape),
+        out = C.c_int64()   # of this call alone: another thread may be in the library at the same time
+        rc = self._lib.tfjs_cuda_tensor_register(self._ctx, C.byref(out), len(shape), _ffi.shape_array(shape),
                                                  _DTYPE_CODE[dtype])
         if rc != 0:
             self._check(rc)
-        return self._out_id.value
+        return out.value
 
     def _free_tmp(self, *ids):
         for i in ids:
@@ -340,9 +338,10 @@ class BackendCuda:
         before does not see such changes."""
         t._throw_if_disposed()
         rec = self._rec(t.dataId)
-        self._check(self._lib.tfjs_cuda_tensor_share(self._ctx, rec["id"], self._out_ptr_ref, None))
+        ptr = C.c_void_p()
+        self._check(self._lib.tfjs_cuda_tensor_share(self._ctx, rec["id"], C.byref(ptr), None))
         typestr = "|u1" if "quantized" in rec else _TYPESTR[rec["dtype"]]
-        return DeviceArray({"shape": tuple(t.shape), "typestr": typestr, "data": (self._out_ptr.value or 0, False),
+        return DeviceArray({"shape": tuple(t.shape), "typestr": typestr, "data": (ptr.value or 0, False),
                             "version": 3, "stream": self._stream})
 
     # ---- fused epilogue marshalling ------------------------------------------------------
@@ -711,7 +710,13 @@ class BackendCuda:
     def _oid(self, t):
         return 0 if t is None else self._data[t.dataId]["id"]
 
-    def _output(self, t, outputs):
+    def _output(self, shape, outputs):
+        t = Tensor(shape, "float32", None, None, self)
+        outputs.append(t)
+        return self._data[t.dataId]["id"]
+
+    def _activation_output(self, shape, storage, outputs):
+        t = self._out_activation(shape, storage)
         outputs.append(t)
         return self._data[t.dataId]["id"]
 
@@ -729,8 +734,8 @@ class BackendCuda:
             xid = self._activation(x, tmp)
             gid = self._operand(gamma, tmp) if gamma is not None else 0
             bid = self._operand(beta, tmp) if beta is not None else 0
-            yid = self._output(self._out_activation(x.shape, outputStorage), out)
-            sid = self._output(self._out(x.shape[:-1] + [2]), out) if withStats else 0
+            yid = self._activation_output(x.shape, outputStorage, out)
+            sid = self._output(x.shape[:-1] + [2], out) if withStats else 0
             rc = self._lib.tfjs_cuda_layer_norm(self._ctx, xid, gid, bid, yid, sid, size_from_shape(x.shape[:-1]),
                                                 width, float(epsilon))
             if rc != 0:
@@ -754,7 +759,7 @@ class BackendCuda:
             did, xid = self._activation(dy, tmp), self._activation(x, tmp)
             gid = self._operand(gamma, tmp) if gamma is not None else 0
             sid = self._operand(stats, tmp)
-            ids = [self._output(self._out(shape), out) for shape in (x.shape, [width], [width])]
+            ids = [self._output(shape, out) for shape in (x.shape, [width], [width])]
             rc = self._lib.tfjs_cuda_layer_norm_backprop(self._ctx, did, xid, gid, sid, *ids,
                                                          size_from_shape(x.shape[:-1]), width)
             if rc != 0:
@@ -777,7 +782,7 @@ class BackendCuda:
         tmp, out = [], []
         try:
             tid, iid = self._activation(table, tmp), self._operand(indices, tmp, "int32")
-            oid = self._output(self._out_activation(indices.shape + [table.shape[1]], outputStorage), out)
+            oid = self._activation_output(indices.shape + [table.shape[1]], outputStorage, out)
             rc = self._lib.tfjs_cuda_embedding_lookup(self._ctx, tid, iid, oid, indices.size, table.shape[0],
                                                       table.shape[1], float(scale))
             if rc != 0:
@@ -799,7 +804,7 @@ class BackendCuda:
         tmp, out = [], []
         try:
             did, iid = self._activation(dy, tmp), self._operand(indices, tmp, "int32")
-            oid = self._output(self._out([int(vocab), dy.shape[-1]]), out)
+            oid = self._output([int(vocab), dy.shape[-1]], out)
             rc = self._lib.tfjs_cuda_embedding_lookup_backprop(self._ctx, did, iid, oid, indices.size, int(vocab),
                                                                dy.shape[-1], float(scale))
             if rc != 0:
@@ -831,8 +836,8 @@ class BackendCuda:
         try:
             zid, uid = self._activation(logits, tmp), self._activation(teacherLogits, tmp)
             iid = self._operand(teacherIndices, tmp, "int32")
-            lid = self._output(self._out(logits.shape[:-1]), out)
-            sid = self._output(self._out(logits.shape[:-1] + [4]), out) if withStats else 0
+            lid = self._output(logits.shape[:-1], out)
+            sid = self._output(logits.shape[:-1] + [4], out) if withStats else 0
             rc = self._lib.tfjs_cuda_distillation_loss(self._ctx, zid, uid, iid, lid, sid, *extent, float(temperature))
             if rc != 0:
                 self._check(rc)
@@ -852,7 +857,7 @@ class BackendCuda:
         try:
             did, zid, uid = self._operand(dloss, tmp), self._activation(logits, tmp), self._activation(teacherLogits, tmp)
             iid, sid = self._operand(teacherIndices, tmp, "int32"), self._operand(stats, tmp)
-            oid = self._output(self._out(logits.shape), out)
+            oid = self._output(logits.shape, out)
             rc = self._lib.tfjs_cuda_distillation_loss_backprop(self._ctx, did, zid, uid, iid, sid, oid, *extent,
                                                                 float(temperature))
             if rc != 0:
