@@ -303,7 +303,8 @@ constexpr int STATUS_SMEM_LAYOUT = 91;  // a kernel's dynamic shared-memory wind
 // every access to global memory.  pdl_launch_dependents() then lets the next kernel's blocks be
 // scheduled as this kernel's blocks retire, so that its launch latency and prologue overlap
 // this kernel's tail.  It is called after pdl_wait(), which keeps the chain transitive: when a
-// kernel starts, all kernels before its predecessor have finished.
+// kernel starts, all kernels before its predecessor have finished.  (A kernel that is always launched
+// without the attribute starts after its predecessor's end and may trigger at once.)
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

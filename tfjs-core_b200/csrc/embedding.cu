@@ -335,8 +335,8 @@ __global__ void __launch_bounds__(kSumThreads) embedding_sum_kernel(const TD* __
                                                                 int64_t tiles, int64_t items) {
   const int lane = threadIdx.x & 31;
   const int64_t item = (int64_t)blockIdx.x * (kSumThreads / 32) + (threadIdx.x >> 5);
-  pdl_launch_dependents();  // the join waits for this kernel's end
   pdl_wait();
+  pdl_launch_dependents();  // the join waits for this kernel's end
   if (item >= items) return;
   const int64_t chunk = item / tiles, col = ((item - chunk * tiles) * 32 + lane) * V;
   const int64_t p0 = chunk * CH;
