@@ -180,7 +180,7 @@ struct RowSplit {
   __device__ int loose(int i) const { return i < head ? i : i + vecs * V; }
 };
 
-// max m and s = sum of 2^((z - m) k), joined with another pair
+// 2^((z - m) k) of a value (or a part's maximum) z relative to the maximum m, 0 where all is -inf
 __device__ __forceinline__ float shifted(float z, float m, float k) { return exp2_approx((z - (m == -INFINITY ? 0.f : m)) * k); }
 
 // G threads a row (a warp, or a block), C blocks a row (only with whole blocks).  NK: teacher entries a
@@ -201,20 +201,18 @@ __global__ void __launch_bounds__(G > 32 ? kThreads : 256) distillation_kernel(
   const TZ* zr = z + first;
   const RowSplit<V> split(first, classes);
 
-  // the teacher's entries, fetched ahead of the row (by the row's first block)
+  // the teacher's entries, fetched ahead of the row (by the row's first block; the others have none)
   float tu[NK], tz[NK];
-  if (rank == 0) {
 #pragma unroll
-    for (int i = 0; i < NK; i++) {
-      const int e = t + i * G;
-      tu[i] = -INFINITY;
-      tz[i] = 0.f;
-      if (e < top) {
-        const int32_t at = indices[row * top + e];
-        if (at >= 0 && at < classes) {
-          tu[i] = load_one(u + row * top + e);
-          tz[i] = load_one(zr + at);
-        }
+  for (int i = 0; i < NK; i++) {
+    const int e = t + i * G;
+    tu[i] = -INFINITY;
+    tz[i] = 0.f;
+    if (rank == 0 && e < top) {
+      const int32_t at = indices[row * top + e];
+      if (at >= 0 && at < classes) {
+        tu[i] = load_one(u + row * top + e);
+        tz[i] = load_one(zr + at);
       }
     }
   }
