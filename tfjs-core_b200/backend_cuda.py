@@ -728,16 +728,16 @@ class BackendCuda:
         self._assert_numeric([x, gamma, beta], "layerNorm")
         if not x.shape:
             raise ValueError("layerNorm needs a tensor of rank 1 or more")
-        width = x.shape[-1]
+        outer, width = x.shape[:-1], x.shape[-1]
         tmp, out = [], []
         try:
             xid = self._activation(x, tmp)
             gid = self._operand(gamma, tmp) if gamma is not None else 0
             bid = self._operand(beta, tmp) if beta is not None else 0
             yid = self._activation_output(x.shape, outputStorage, out)
-            sid = self._output(x.shape[:-1] + [2], out) if withStats else 0
-            rc = self._lib.tfjs_cuda_layer_norm(self._ctx, xid, gid, bid, yid, sid, size_from_shape(x.shape[:-1]),
-                                                width, float(epsilon))
+            sid = self._output(outer + [2], out) if withStats else 0
+            rc = self._lib.tfjs_cuda_layer_norm(self._ctx, xid, gid, bid, yid, sid, size_from_shape(outer), width,
+                                                float(epsilon))
             if rc != 0:
                 self._check(rc)
             return out[0], out[1] if withStats else None
@@ -819,11 +819,11 @@ class BackendCuda:
 
     @staticmethod
     def _distillation_extent(logits, teacherLogits, teacherIndices):
-        if not logits.shape or logits.shape[:-1] != teacherLogits.shape[:-1] or \
-                teacherLogits.shape != teacherIndices.shape:
+        outer = logits.shape[:-1]
+        if not logits.shape or outer != teacherLogits.shape[:-1] or teacherLogits.shape != teacherIndices.shape:
             raise ValueError(f"distillationLoss: logits {logits.shape}, teacherLogits {teacherLogits.shape} and "
                              f"teacherIndices {teacherIndices.shape} must be [..., classes], [..., top] and [..., top]")
-        return size_from_shape(logits.shape[:-1]), logits.shape[-1], teacherLogits.shape[-1]
+        return outer, (size_from_shape(outer), logits.shape[-1], teacherLogits.shape[-1])
 
     def distillationLoss(self, logits, teacherLogits, teacherIndices, temperature=1.0, withStats=True):
         """Extension: T^2 * KL(p || q) of each row, q = softmax(logits / T) over all classes and
@@ -831,13 +831,13 @@ class BackendCuda:
         does not count; a row without any gives 0).  Returns (loss, stats): stats, [..., 4], is what the
         gradient reads, or None unless `withStats`."""
         self._assert_numeric([logits, teacherLogits], "distillationLoss")
-        extent = self._distillation_extent(logits, teacherLogits, teacherIndices)
+        outer, extent = self._distillation_extent(logits, teacherLogits, teacherIndices)
         tmp, out = [], []
         try:
             zid, uid = self._activation(logits, tmp), self._activation(teacherLogits, tmp)
             iid = self._operand(teacherIndices, tmp, "int32")
-            lid = self._output(logits.shape[:-1], out)
-            sid = self._output(logits.shape[:-1] + [4], out) if withStats else 0
+            lid = self._output(outer, out)
+            sid = self._output(outer + [4], out) if withStats else 0
             rc = self._lib.tfjs_cuda_distillation_loss(self._ctx, zid, uid, iid, lid, sid, *extent, float(temperature))
             if rc != 0:
                 self._check(rc)
@@ -852,7 +852,7 @@ class BackendCuda:
     def distillationLossBackprop(self, dloss, logits, teacherLogits, teacherIndices, stats, temperature=1.0):
         """Extension: the gradient of distillationLoss's logits, from the stats of its forward pass."""
         self._assert_numeric([dloss, logits, teacherLogits, stats], "distillationLossBackprop")
-        extent = self._distillation_extent(logits, teacherLogits, teacherIndices)
+        _, extent = self._distillation_extent(logits, teacherLogits, teacherIndices)
         tmp, out = [], []
         try:
             did, zid, uid = self._operand(dloss, tmp), self._activation(logits, tmp), self._activation(teacherLogits, tmp)
