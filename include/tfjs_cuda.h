@@ -305,7 +305,8 @@ int tfjs_cuda_embedding_lookup_backprop(tfjs_cuda_ctx* ctx, tfjs_tensor_id dy, t
  *   loss[r] = T^2 sum_k p_k (log p_k - log q[i_k]),
  * q = softmax(logits[r] / T) over all classes, p = softmax(teacher_logits[r] / T) over the entries
  * whose index lies in [0, classes) and whose logit is above -inf (so -1 ends a shorter list; a class
- * named twice counts twice).  A row without such an entry has loss 0 and gradient 0.  top <= 1024.
+ * named twice counts twice).  A row without such an entry has loss 0 and gradient 0.  top <= 1024; T and
+ * log2(e) / T positive and finite.
  * stats, [rows, 4] (the largest logit and log2 of the sum beside it, of the student and of the teacher)
  * or 0, is what the gradient reads. */
 int tfjs_cuda_distillation_loss(tfjs_cuda_ctx* ctx, tfjs_tensor_id logits, tfjs_tensor_id teacher_logits,

@@ -11,6 +11,8 @@
 //   sum    a warp adds 16 or 32 sorted tokens over 128 columns and writes the rows that end within them
 //          (12 us: 50 MB of dy, latency as much as bandwidth)
 //   join   rows that go on over several warps' tokens have their shares added, in order (6 us)
+// Above 65536 tokens the table's zeros, then a count, a scan and a placing for each digit: 100000 x 256 of 50000 rows
+// 47 us for the sort, 22 for the sums, 8 for the join.
 // Sums are float32; the scale multiplies each finished sum.
 #include <cooperative_groups.h>
 

@@ -20,11 +20,11 @@
 // Gradient.  One pass over dy and x gives dx and, per block, the weights' gradients:
 //   up to 8192     persistent blocks; a ring of stages (several rows each) filled by cp.async.  First
 //                  the lanes of a row sum a and a n, then every thread takes the same columns of every
-//                  row: it writes dx and keeps its columns' dg, db in registers.  16384 x 1024: 37 us, 5.4 TB/s
+//                  row: it writes dx and keeps its columns' dg, db in registers.  16384 x 1024: 38 us, 5.3 TB/s
 //                  (with 8 KB rows and 512 threads, whose fixed cost a stage was 60 % of all instructions, 68);
 //                  4096 x 8192: 79 us, clusters 141
 //   above          a cluster of 1 to 8 blocks a row; dg, db add up in the blocks' shared memory.  1000 x 33000:
-//                  185 us, bound by the latency of a row
+//                  186 us, bound by the latency of a row (a quarter of the DRAM rate, 36 % of the issue slots)
 // and a second kernel adds the blocks' partial dg, db in order (4 us at 16384 x 1024, 2.4 MB from L2).
 #include <cooperative_groups.h>
 
@@ -668,6 +668,8 @@ __global__ void __launch_bounds__(kClusterThreads, 2) layer_norm_backprop_cluste
 
 // out[j] = sum over the blocks of partial[block][j]; j runs over dg and then db.  Many blocks: 32 columns a
 // block, 32 threads a column take every 32nd block's row and join theirs in order.  Up to 64: a thread a column.
+// (40 blocks of 20000 columns: 2 us with a thread a column, 6 with 32; 60 of 200000: 10 and 66; 100 of 8000: 6 and
+// 4; 296 of 1024: 12 and 4.)
 // `partial` comes without __restrict__: a load that the compiler may take for one of constant data could be moved
 // ahead of pdl_wait().
 constexpr int kJoinThreads = 1024, kFewBlocks = 64;
@@ -729,6 +731,8 @@ void lanes_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   layer_norm_lanes_kernel<TX, TY, V, NV, L><<<(unsigned)ceil_div64(a.rows, 256 / L), 256, 0, ctx->stream>>>(
       (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon);
 }
+// Eight blocks an SM go on to further rows: 16384 x 2048 45 us, 57 with four, 90 with two.  (A block for every row
+// measures the same there and is ahead with more rows: 65536 x 1536 half 160 us, 191 with eight.)
 template <typename TX, typename TY, int V, int NV, int NT>
 void block_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   layer_norm_block_kernel<TX, TY, V, NV, NT><<<grid_rows(ctx, a.rows, 8), NT, 0, ctx->stream>>>(
@@ -770,7 +774,8 @@ template <typename TX, typename TY, int V>
 int cluster_form(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   // Blocks a row: so many that three blocks' shares fit into an SM's shared memory (one loads while another
   // sums), and with few rows so many that the SMs have a block each.  1000 x 33000: 76 us with the two that
-  // gives, 94 with one, 151 with eight; 8 x 33000: 7 us with eight, 12 with one.
+  // gives, 94 with one, 151 with eight; 8 x 33000: 7 us with eight, 12 with one.  Half: 1000 x 33000 45 us with one,
+  // as shares of 72 or 144 KB give, 59 with two; 1000 x 65536 86 with two, 111 with one, 119 with four.
   const auto share_of = [&](int C) { return (ceil_div64(a.width / V, C) * V * (int64_t)sizeof(TX) + 31) / 16 * 16; };
   int C = 1;
   while (C < 8 && (share_of(C) > 72 * 1024 || a.rows * C < ctx->sm_count)) C *= 2;
@@ -810,6 +815,8 @@ int ring_launch(tfjs_cuda_ctx* ctx, const ForwardArgs& a) {
   const int smem = groups * 2 * slot_bytes + (G == 32 ? P * ((int)a.width / P + 1) * 2 * P * 4 : 0);
   auto kernel = layer_norm_ring_kernel<TX, TY, NW, G>;
   TFJS_CHECK_CUDA(ctx, allow_smem(kernel, smem));
+  // as many blocks an SM as fit, up to six: 100000 x 131 half 41 us, 43 with up to four, 49 with two; 4000 x 7001 half
+  // 47 and 57 with two; with three (33000 x 1001 float32, 59 us) two would be ahead, 47
   const int per_sm = smem <= 36 * 1024 ? 6 : smem <= 55 * 1024 ? 4 : smem <= 74 * 1024 ? 3 : 2;
   kernel<<<grid_rows(ctx, ceil_div64(a.rows, groups), per_sm), kRingThreads, smem, ctx->stream>>>(
       (const TX*)a.x, a.gamma, a.beta, (TY*)a.y, a.stats, a.rows, (int)a.width, a.epsilon, slot_bytes);
@@ -935,7 +942,9 @@ int backward_cluster_form(tfjs_cuda_ctx* ctx, const BackwardArgs& a) {
     p.slot_bytes = p.d_bytes + (int)((share * (int64_t)sizeof(TX) + 31) / 16 * 16);
     return 2 * (int64_t)p.slot_bytes + share * 8;
   };
-  // as for the forward pass: two blocks an SM, and with few rows a block for every SM
+  // as for the forward pass: two blocks an SM, and with few rows a block for every SM (1000 x 20000 half 82 us with
+  // shares of 112 KB, 146 with 56, 84 with 224; 1000 x 33000 float32 186, 186 and 205, but 1000 x 20000 float32 154,
+  // 156 and 139)
   int C = 1;
   int64_t smem = a.width < (1 << 22) ? bytes_of(C) : INT64_MAX;
   while (C < 8 && (smem > 112 * 1024 || a.rows * C < ctx->sm_count)) {
