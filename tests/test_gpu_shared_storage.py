@@ -117,3 +117,18 @@ def test_separable_filters_written_through_the_array(tf, which):
             assert hit[1:, 1:].all() and not hit[0].any() and not hit[:, 0].any()
     finally:
         bk.setMathMode(before)
+
+
+def test_a_shared_quantised_tensor_that_needs_decoding_cannot_be_captured(tf):
+    bk = tf.ENGINE.backend
+    q = _rng(7).integers(0, 256, (5, 3)).astype(np.uint8)
+    x, w = tf.ops.tensor(np.ones((2, 5), np.float32)), bk.registerQuantized([5, 3], q, 0.5, -1.0)
+    want = tf.ops.matmul(x, w).dataSync()
+    bk.deviceArray(w)
+    bk.graphBegin()
+    try:
+        with pytest.raises(NotImplementedError, match="shared"):
+            tf.ops.matmul(x, w)
+    finally:
+        bk.graphDestroy(bk.graphEnd())
+    assert np.array_equal(tf.ops.matmul(x, w).dataSync(), want)

@@ -246,3 +246,21 @@ def test_distillation_loss_three_times(host):
     for want in (first, s * (1 - s), s * (1 - s) * (1 - 2 * s)):
         f = along(f)
         np.testing.assert_allclose(f(x).dataSync(), want, rtol=0, atol=TOL)
+
+
+def test_single_rows_without_a_batch_axis(host):
+    rng = np.random.default_rng(6)
+    z, u = rng.normal(0, 1, 5).astype(np.float32), rng.normal(0, 1, 2).astype(np.float32)
+    idx = np.array([4, 1], np.int32)
+    tu, ti = ops.tensor(u), ops.tensor(idx, dtype="int32")
+    f = lambda v: ops.distillation_loss(ops.layer_norm(v, epsilon=0.1), tu, ti, 2.0)  # noqa: E731
+
+    def gradients(v):
+        n, _ = _normalised(v[None], 0.1)
+        dz = _distillation_gradient(n, u[None], idx[None], np.ones(1), 2.0)
+        return [_layer_norm_gradients(dz, v[None], np.ones(5), 0.1)[0][0]]
+    _check(f, gradients, [z], rng)
+    table = rng.normal(0, 1, (3, 2)).astype(np.float32)
+    at = ops.scalar(2, "int32")
+    got = ops.grad(lambda t: ops.sum(ops.grad(lambda s: ops.sum(ops.square(ops.embedding_lookup(s, at))))(t)))(ops.tensor(table))
+    np.testing.assert_array_equal(got.dataSync().reshape(3, 2), [[0, 0], [0, 0], [2, 2]])

@@ -27,6 +27,10 @@ int float_view(tfjs_cuda_ctx* ctx, TensorEntry* t, const float** out) {
     return TFJS_CUDA_OK;
   }
   if (!t->deq || t->deq_version != t->version || t->shared) {
+    if (t->shared && ctx->capturing)
+      return set_error(ctx, TFJS_CUDA_ERR_UNSUPPORTED,
+                       "the dequantised copy of a tensor whose storage is shared is made anew by every call, which "
+                       "cannot be captured into a graph");
     int miss = refuse_miss_during_capture(ctx, "the dequantised copy");
     if (miss) return miss;
     if (!t->deq) {
